@@ -192,5 +192,6 @@ inline PyObject* wrap(Tensor t) { return THPVariable_Wrap(std::move(t)); }
 
 PyMethodDef* model_methods();   // lm.cpp
 PyMethodDef* train_methods();   // train.cpp
+PyMethodDef* ends_methods();    // ends.cpp
 
 }  // namespace cdssm_host

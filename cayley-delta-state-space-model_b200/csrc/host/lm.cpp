@@ -433,6 +433,26 @@ PyObject* py_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// lm_hidden(plan, ids, per_token_group_norm, scan_flags) -> what the head reads (B,L,d_model): lm_forward before its last product
+PyObject* py_hidden(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Args in{a, n};
+        Plan& p = plan_of(in.next());
+        const Tensor ids = in.tensor("input_ids");
+        const bool per_token = in.flag();
+        const int64_t flags = in.integer();
+        need_batch(ids);
+        const NoGrad ng;
+        const auto lay = layout_of(p);
+        return wrap(without_gil([&] {
+            const c10::cuda::CUDAGuard guard(p.embedding.device());
+            const Tensor x = embed(p, ids), ws = gemm_workspace(x);
+            run_blocks(p, *lay, x, nullptr, per_token, flags, ws);
+            return rms_norm(x, p.final_norm_w, kFinalEps);
+        }));
+    });
+}
+
 // lm_prefill(plan, ids, last_only) -> (logits, [state, conv, state, conv, ...])
 PyObject* py_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
@@ -506,6 +526,7 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef g_model_methods[] = {
     {"lm_plan", FAST(py_plan)},
     {"lm_forward", FAST(py_forward)},
+    {"lm_hidden", FAST(py_hidden)},
     {"lm_prefill", FAST(py_prefill)},
     {"lm_decode", FAST(py_decode)},
     {nullptr, nullptr, 0, nullptr},

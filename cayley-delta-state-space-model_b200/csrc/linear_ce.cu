@@ -1,0 +1,931 @@
+// Softmax cross entropy of hidden rows against a large vocabulary, and its gradients, without the logits in memory.
+//
+// With z = x W^T (x: rows x d, W: vocab x d), m_t = max_v z_tv and s_t = sum_v exp(z_tv - m_t):
+//     loss_t = (m_t - z_t,y(t)) + log s_t
+//     dz_tv  = g_t (exp(z_tv - m_t) / s_t - [v = y(t)])        g_t: the upstream gradient of row t
+//     dx = dz W,   dW = dz^T x
+// Forward: one product whose epilogue keeps the running maximum and sum of a row over a run of vocabulary tiles; the runs of a row are
+// joined by a small kernel.  Backward, a piece of the vocabulary at a time: z of the piece anew, dz of it rounded to the products'
+// type into scratch, then both products that read it in one launch.  Rows without a target are left out before the first product.
+//
+// All products are tcgen05 ones of TMA tiles: 128 x 256 outputs a block, fp32 accumulators, two of them in tensor memory so that the
+// epilogue of a tile runs beside the products of the next.  float32 operands enter as three bf16 parts (exact to 24 bits) and six of
+// the nine part products, the small ones first.
+#include "cdssm_common.cuh"
+#include "sm100_ptx.cuh"
+#include "tile_map.cuh"
+#include <cuda_bf16.h>
+
+namespace cdssm {
+
+unsigned long long wait_limit_ns();
+
+namespace ce {
+
+using namespace sm100;
+
+constexpr int kM = 128, kN = 256, kK = 64;              // rows and columns of a block's tile, depth of a stage
+constexpr int kStages = 4;
+constexpr int kEpilogueWarps = 8, kThreads = 128 + 32 * kEpilogueWarps;
+constexpr int kRowTile = 256;                           // packed rows come in multiples of this
+constexpr int kTmemCols = 2 * kN;
+
+enum Mode { kStats, kGradLogits, kGradProducts };
+
+// Part products of float32 operands in the order in which they are added up: the small ones first, so that they are not lost beside
+// the large one's rounding.  (2,1), (1,2), (2,2) are below 2^-24 of the whole.
+constexpr int kTerms3 = 6;
+__device__ __forceinline__ void term_planes(int planes, int term, int& pa, int& pb) {
+    if (planes == 1) { pa = pb = 0; return; }
+    constexpr uint32_t a = 2u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 0u << 10, b = 0u | 2u << 2 | 1u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
+    pa = (a >> (2 * term)) & 3;
+    pb = (b >> (2 * term)) & 3;
+}
+
+struct Args {
+    // what the forward leaves for the backward; Tp: rows padded to kRowTile
+    const int* count;            // rows that have a target
+    const int* rows;             // (Tp) compact row -> row of the caller, -1 behind the last
+    const int* target;           // (Tp) its word, -2: outside of the vocabulary
+    float *row_max, *row_inv;    // (Tp) m and 1 / s
+    float* hit;                  // (Tp) z of the target
+    float2* part;                // (runs x 2, Tp) maximum and sum of a run of tiles
+    const float* grad;           // upstream gradient: one value, or one a row of the caller
+    int grad_rows, mean;
+    int planes, terms;
+    int Tp, d, V;
+    int run, n_tiles, n_runs;    // forward: tiles of a run, tiles and runs of a row
+    int v0, vn, vn_tiles;        // backward: first word and words of the piece
+    void *dx, *dw;
+    float* acc;                  // (Tp, acc_pitch) dx of the pieces before, summed
+    int acc_pitch, d_tiles, f32, first, last, vec_dx, vec_dw;
+    float4* slots;               // partial tiles of the split ones: two a block
+    int* status;
+    unsigned long long wait_ns;
+    int withhold;
+};
+
+struct __align__(1024) Smem {
+    uint8_t a[kStages][kM * kK * 2];
+    uint8_t b[kStages][kN * kK * 2];
+    uint8_t out[kEpilogueWarps][4096];
+    uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ---- the blocks' shares of the work ---------------------------------------------------------
+// A segment: depth blocks [k0, k1) of one tile.
+struct Segment {
+    int dw;          // kGradProducts: 0 a tile of dx, 1 of dW
+    int m, n;        // row and column tile
+    int k0, k1, kt;  // of kt in all
+    bool last;       // kStats: of its run
+    int run;
+};
+
+__device__ __forceinline__ int row_tiles(int count) { return max(1, (count + kRowTile - 1) / kRowTile) * (kRowTile / kM); }
+
+// Forward and dz: a run of vocabulary tiles of one row tile is a block's unit.  Row tiles change fastest, so the blocks that run
+// beside each other read the same rows of W and every row of W leaves DRAM about once.
+struct RunWalk {
+    int unit, units, mt, run_len, n_tiles, kt, n, n_end, m, run;
+    __device__ RunWalk(const Args& a, int count, int n_tiles_, int run_len_) : run_len(run_len_), n_tiles(n_tiles_) {
+        mt = row_tiles(count);
+        units = mt * ((n_tiles + run_len - 1) / run_len);
+        kt = (a.d + kK - 1) / kK * a.terms;
+        unit = (int)blockIdx.x - (int)gridDim.x;
+        n = n_end = 0;
+    }
+    __device__ bool next(Segment& s) {
+        if (n >= n_end) {
+            unit += gridDim.x;
+            if (unit >= units) return false;
+            run = unit / mt;
+            m = unit - run * mt;
+            n = run * run_len;
+            n_end = min(n + run_len, n_tiles);
+        }
+        s = {0, m, n, 0, kt, kt, n + 1 == n_end, run};
+        n++;
+        return true;
+    }
+};
+
+// dx and dW: as many whole tiles as fill the grid evenly, column tiles fastest (the blocks beside each other read the same rows of
+// dz); the depth blocks of the tiles that are left, dx before dW, are cut into as many equal shares as there are blocks.
+struct SplitTiles {
+    int nx, nw, fx, fw, kx, kw, G, d_tiles;
+    long long rest;
+    __device__ SplitTiles(int mt, int vt, int d_tiles_, int kx_, int kw_, int grid) : kx(kx_), kw(kw_), G(grid), d_tiles(d_tiles_) {
+        nx = mt * d_tiles;
+        nw = vt * d_tiles;
+        fx = nx / G * G;
+        fw = nw / G * G;
+        rest = (long long)(nx - fx) * kx + (long long)(nw - fw) * kw;
+    }
+    __device__ long long begin(int block) const { return rest * block / G; }
+    // the tile that depth block i of the rest belongs to, and where it begins
+    __device__ void at(long long i, int& dw, int& tile, long long& start) const {
+        const long long x = (long long)(nx - fx) * kx;
+        dw = i >= x;
+        const long long j = dw ? (i - x) / kw : i / kx;
+        tile = (dw ? fw : fx) + (int)j;
+        start = dw ? x + j * kw : j * kx;
+    }
+};
+__device__ __forceinline__ SplitTiles split_tiles(const Args& a, int count, int grid) {
+    const int mt = row_tiles(count);
+    return SplitTiles(a.dx ? mt : 0, a.dw ? (a.vn + kM - 1) / kM : 0, a.d_tiles, (a.vn + kK - 1) / kK * a.terms, mt * (kM / kK) * a.terms, grid);
+}
+struct SplitWalk {
+    SplitTiles t;
+    int phase = 0, i;
+    long long at, end;
+    __device__ SplitWalk(const Args& a, int count) : t(split_tiles(a, count, gridDim.x)) {
+        i = blockIdx.x;
+        at = t.begin(blockIdx.x);
+        end = t.begin(blockIdx.x + 1);
+    }
+    __device__ bool next(Segment& s) {
+        while (phase < 2) {
+            if (i < (phase ? t.fw : t.fx)) {
+                const int k = phase ? t.kw : t.kx;
+                s = {phase, i / t.d_tiles, i % t.d_tiles, 0, k, k, true, 0};
+                i += t.G;
+                return true;
+            }
+            phase++;
+            i = blockIdx.x;
+        }
+        if (at >= end) return false;
+        int dw, tile;
+        long long start;
+        t.at(at, dw, tile, start);
+        const int k = dw ? t.kw : t.kx;
+        const long long stop = start + k < end ? start + k : end;
+        s = {dw, tile / t.d_tiles, tile % t.d_tiles, (int)(at - start), (int)(stop - start), k, true, 0};
+        at = stop;
+        return true;
+    }
+};
+template <int kMode> struct WalkOf { using type = RunWalk; };
+template <> struct WalkOf<kGradProducts> { using type = SplitWalk; };
+template <int kMode>
+__device__ __forceinline__ typename WalkOf<kMode>::type make_walk(const Args& a, int count) {
+    if constexpr (kMode == kGradProducts) return SplitWalk(a, count);
+    else return RunWalk(a, count, kMode == kStats ? a.n_tiles : a.vn_tiles, a.run);
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, const void* src, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(reinterpret_cast<uint64_t>(m)),
+                 "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+struct Maps {   // kStats, kGradLogits: a x, b W, out dz; kGradProducts: (a dz, b W) for dx, (a2 dz, b2 x) for dW
+    CUtensorMap a, b, a2, b2;
+};
+
+// ---- producer: one thread ------------------------------------------------------------------
+template <int kMode>
+__device__ __forceinline__ bool produce(Smem& sm, const Maps& maps, const Args& a, int count) {
+    volatile int* ab = &sm.abort_flag;
+    auto walk = make_walk<kMode>(a, count);
+    Segment s;
+    uint32_t it = 0;
+    while (walk.next(s)) {
+        const int depth = s.kt / a.terms;
+#pragma unroll 1
+        for (int k = s.k0; k < s.k1; k++, it++) {
+            const int st = it % kStages;
+            if (!mbar_wait_suspend(&sm.empty[st], (it / kStages & 1) ^ 1, ab, a.wait_ns)) return false;
+            mbar_arrive_expect_tx(&sm.full[st], (kM + kN) * kK * 2);
+            int pa, pb;
+            term_planes(a.planes, k / depth, pa, pb);
+            const int kc = (k % depth) * kK;
+            if (kMode != kGradProducts) {
+                tma_load_3d(sm.a[st], &maps.a, &sm.full[st], kc, s.m * kM, pa);
+                tma_load_3d(sm.b[st], &maps.b, &sm.full[st], kc, a.v0 + s.n * kN, pb);
+            } else if (!s.dw) {
+                tma_load_3d(sm.a[st], &maps.a, &sm.full[st], kc, s.m * kM, pa);
+#pragma unroll
+                for (int j = 0; j < kN / 64; j++)
+                    tma_load_3d(sm.b[st] + j * 64 * kK * 2, &maps.b, &sm.full[st], s.n * kN + j * 64, a.v0 + kc, pb);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kM / 64; j++)
+                    tma_load_3d(sm.a[st] + j * 64 * kK * 2, &maps.a2, &sm.full[st], s.m * kM + j * 64, kc, pa);
+#pragma unroll
+                for (int j = 0; j < kN / 64; j++)
+                    tma_load_3d(sm.b[st] + j * 64 * kK * 2, &maps.b2, &sm.full[st], s.n * kN + j * 64, kc, pb);
+            }
+        }
+    }
+    return true;
+}
+
+// ---- products: one warp ----------------------------------------------------------------------
+template <int kMode>
+__device__ __forceinline__ bool multiply(Smem& sm, const Args& a, int count) {
+    volatile int* ab = &sm.abort_flag;
+    auto walk = make_walk<kMode>(a, count);
+    Segment s;
+    uint32_t it = 0, tile = 0;
+    const uint32_t tm = sm.tmem_base;
+    while (walk.next(s)) {
+        const int acc = tile & 1;
+        if (!mbar_wait_suspend(&sm.acc_empty[acc], (tile >> 1 & 1) ^ 1, ab, a.wait_ns)) return false;
+        tc_fence_after();
+        // (a K-major row of a tile is 128 bytes: 16 columns are 32 bytes on; an MN-major one holds 64 rows of the operand: 16 of the
+        // depth are 16 rows of 128 bytes on, the next 64 rows of the operand 8192 bytes)
+        const bool a_mn = kMode == kGradProducts && s.dw, b_mn = kMode == kGradProducts;
+        const uint32_t idesc = umma_idesc_bf16(kM, kN, false, false) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+        const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;
+        const uint32_t a_lbo = a_mn ? 8192 : 16, b_lbo = b_mn ? 8192 : 16;
+#pragma unroll 1
+        for (int k = s.k0; k < s.k1; k++, it++) {
+            const int st = it % kStages;
+            if (!mbar_wait_suspend(&sm.full[st], it / kStages & 1, ab, a.wait_ns)) return false;
+            tc_fence_after();
+            const uint32_t da = desc_lo_sw128(smem_u32(sm.a[st]), a_lbo), db = desc_lo_sw128(smem_u32(sm.b[st]), b_lbo);
+#pragma unroll
+            for (int j = 0; j < kK / 16; j++)
+                umma_bf16_elect(tm + acc * kN, da + j * a_step, db + j * b_step, idesc, k > s.k0 || j > 0);
+            umma_commit_elect(&sm.empty[st]);
+        }
+        umma_commit_elect(&sm.acc_full[acc]);
+        tile++;
+    }
+    return true;
+}
+
+// ---- epilogues: eight warps, a row a thread, 128 columns ---------------------------------------
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return reinterpret_cast<const uint32_t&>(p);
+}
+
+// 32 columns of an output row from registers; vec: 16-byte aligned and a multiple of 16 bytes wide
+template <typename T>
+__device__ __forceinline__ void store_row(T* row, int col, int cols, const float (&v)[32], bool vec) {
+    if (vec) {
+        constexpr int kE = 16 / sizeof(T);
+#pragma unroll
+        for (int j = 0; j < 32; j += kE) {
+            if (col + j < cols) {
+                uint4 u;
+                if constexpr (sizeof(T) == 2)
+                    u = {pack2(v[j], v[j + 1]), pack2(v[j + 2], v[j + 3]), pack2(v[j + 4], v[j + 5]), pack2(v[j + 6], v[j + 7])};
+                else
+                    u = {__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3])};
+                *reinterpret_cast<uint4*>(row + col + j) = u;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+            if (col + j < cols) {
+                if constexpr (sizeof(T) == 2) row[col + j] = __float2bfloat16_rn(v[j]);
+                else row[col + j] = v[j];
+            }
+    }
+}
+
+// 32 columns of a row of a finished tile of dx or dW.  dx of several pieces is summed in float32 and rounded once, by the last.
+__device__ __forceinline__ void emit(const Args& a, int count, int dw, int row, int col, float (&v)[32]) {
+    if (col >= a.d) return;
+    if (dw) {
+        if (row >= a.vn) return;
+        const size_t at = (size_t)(a.v0 + row) * a.d;
+        if (a.f32) store_row(static_cast<float*>(a.dw) + at, col, a.d, v, a.vec_dw);
+        else store_row(static_cast<__nv_bfloat16*>(a.dw) + at, col, a.d, v, a.vec_dw);
+        return;
+    }
+    if (row >= count) return;
+    float* acc = a.acc + (size_t)row * a.acc_pitch + col;
+    if (!a.first) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+            const float4 p = *reinterpret_cast<const float4*>(acc + j);
+            v[j] += p.x; v[j + 1] += p.y; v[j + 2] += p.z; v[j + 3] += p.w;
+        }
+    }
+    if (!a.last) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(acc + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        return;
+    }
+    const size_t at = (size_t)a.rows[row] * a.d;
+    if (a.f32) store_row(static_cast<float*>(a.dx) + at, col, a.d, v, a.vec_dx);
+    else store_row(static_cast<__nv_bfloat16*>(a.dx) + at, col, a.d, v, a.vec_dx);
+}
+
+constexpr int kSlotFloat4 = kM * kN / 4;
+// where lane `lane` of a warp keeps four columns of a partial tile: a warp's store is 512 bytes in a row
+__device__ __forceinline__ size_t slot_at(int slot, int warp, int chunk, int j4, int lane) {
+    return (size_t)slot * kSlotFloat4 + ((warp * 4 + chunk) * 8 + j4) * 32 + lane;
+}
+
+template <int kMode>
+__device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, const Args& a, int count) {
+    volatile int* ab = &sm.abort_flag;
+    auto walk = make_walk<kMode>(a, count);
+    Segment s;
+    const int warp = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31, quarter = warp & 3, half = warp >> 2;
+    const int lrow = quarter * 32 + lane;                // row of the tile
+    const uint32_t tm = sm.tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
+    float top = -INFINITY, sum = 0.f;
+    int run_rows = -1, target = -1;                      // of the present row tile
+    float mx = 0.f, inv = 0.f, g = 0.f;
+    uint32_t tile = 0;
+    while (walk.next(s)) {
+        const int acc = tile & 1, row = s.m * kM + lrow;
+        if (kMode != kGradProducts && run_rows != s.m) {
+            run_rows = s.m;
+            target = a.target[row];
+            if (kMode == kGradLogits) {
+                mx = a.row_max[row];
+                inv = a.row_inv[row];
+                g = 0.f;
+                if (row < count) {
+                    g = a.grad_rows ? a.grad[a.rows[row]] : a.grad[0];
+                    if (a.mean) g /= (float)count;
+                    if (target == -2) g = NAN;           // (a target that is no word)
+                }
+            }
+        }
+        if (!mbar_wait_suspend(&sm.acc_full[acc], tile >> 1 & 1, ab, a.wait_ns)) return false;
+        tc_fence_after();
+        if (kMode == kStats) {
+#pragma unroll 1
+            for (int c = 0; c < 4; c++) {
+                const int v0 = s.n * kN + half * 128 + c * 32;
+                if (v0 >= a.V) break;
+                float z[32];
+                tmem_ld32(tm + acc * kN + c * 32, z);
+                if (v0 + 32 > a.V) {
+#pragma unroll
+                    for (int j = 0; j < 32; j++)
+                        if (v0 + j >= a.V) z[j] = -INFINITY;
+                }
+                const unsigned rel = (unsigned)(target - v0);
+                if (__any_sync(~0u, rel < 32u)) {
+                    float hit = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 32; j++) hit = rel == (unsigned)j ? z[j] : hit;
+                    if (rel < 32u) a.hit[row] = hit;
+                }
+                float best = z[0];
+#pragma unroll
+                for (int j = 1; j < 32; j++) best = fmaxf(best, z[j]);
+                best = fmaxf(best, top);
+                const float ref = best == -INFINITY ? 0.f : best;
+                float add = 0.f;
+#pragma unroll
+                for (int j = 0; j < 32; j++) add += ex2((z[j] - ref) * kLog2e);
+                sum = sum * ex2((top - ref) * kLog2e) + add;
+                top = best;
+            }
+        } else if (kMode == kGradLogits) {
+            const float scale = g * inv;
+#pragma unroll 1
+            for (int c = 0; c < 2; c++) {
+                const int col = s.n * kN + half * 128 + c * 64, v0 = a.v0 + col;
+                float z[64];
+                tmem_ld32x2(tm + acc * kN + c * 64, z, tm + acc * kN + c * 64 + 32, z + 32);
+#pragma unroll
+                for (int j = 0; j < 64; j++) z[j] = ex2((z[j] - mx) * kLog2e) * scale;
+                // (in the last step of the target's entry 1 - p is taken from p in float32: nothing is lost where p is near one)
+                const unsigned rel = (unsigned)(target - v0);
+                if (__any_sync(~0u, rel < 64u)) {
+#pragma unroll
+                    for (int j = 0; j < 64; j++) z[j] = rel == (unsigned)j ? z[j] - g : z[j];
+                }
+                if (v0 + 64 > a.V) {
+#pragma unroll
+                    for (int j = 0; j < 64; j++)
+                        if (v0 + j >= a.V) z[j] = 0.f;
+                }
+                const bool live = row < count;
+                uint8_t* const mine = sm.out[warp];
+                for (int p = 0; p < a.planes; p++) {
+                    if (lane == 0) tma_store_wait_read();
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        uint4 u = {pack2(z[8 * j], z[8 * j + 1]), pack2(z[8 * j + 2], z[8 * j + 3]), pack2(z[8 * j + 4], z[8 * j + 5]),
+                                   pack2(z[8 * j + 6], z[8 * j + 7])};
+                        if (!live) u = {0, 0, 0, 0};
+                        *reinterpret_cast<uint4*>(mine + lane * 128 + ((j ^ (lane & 7)) << 4)) = u;
+                        if (p + 1 < a.planes) {          // what the rounding has left
+                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                z[8 * j + 2 * e] -= __uint_as_float(w[e] << 16);
+                                z[8 * j + 2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
+                            }
+                        }
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) tma_store_3d(map_out, mine, col, s.m * kM + quarter * 32, p);
+                }
+            }
+        } else {
+            const bool whole = s.k0 == 0 && s.k1 == s.kt;
+            const int slot = 2 * blockIdx.x + (s.k0 == 0 ? 1 : 0);
+#pragma unroll 1
+            for (int c = 0; c < 4; c++) {
+                float v[32];
+                tmem_ld32(tm + acc * kN + c * 32, v);
+                if (whole) {
+                    emit(a, count, s.dw, row, s.n * kN + half * 128 + c * 32, v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        a.slots[slot_at(slot, warp, c, j, lane)] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                }
+            }
+        }
+        tc_fence_before();
+        mbar_arrive(&sm.acc_empty[acc]);
+        tile++;
+        if (kMode == kStats && s.last) {
+            a.part[(size_t)(2 * s.run + half) * a.Tp + row] = make_float2(top, sum);
+            top = -INFINITY;
+            sum = 0.f;
+        }
+    }
+    if (kMode == kGradLogits && lane == 0) tma_store_wait();
+    return true;
+}
+
+template <int kMode>
+__global__ void __launch_bounds__(kThreads, 1)
+product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtensorMap map_out, const Args a) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+    const int warp = threadIdx.x >> 5;
+    if ((smem_u32(smem_raw) & 1023u) != 0) {   // the swizzled tiles need 1024-byte alignment
+        if (threadIdx.x == 0) atomicCAS(a.status, 0, 499);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; i++) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
+        for (int i = 0; i < 2; i++) { mbar_init(&sm.acc_full[i], 1); mbar_init(&sm.acc_empty[i], 32 * kEpilogueWarps); }
+        sm.abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) tmem_alloc(&sm.tmem_base, kTmemCols);
+    fence_proxy_async();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const int count = *a.count;
+    bool ok = true;
+    if (warp == 0) {
+        if ((threadIdx.x & 31) == 0 && !a.withhold) ok = produce<kMode>(sm, maps, a, count);
+    } else if (warp == 1) {
+        ok = multiply<kMode>(sm, a, count);
+    } else if (warp >= 4) {
+        ok = finish<kMode>(sm, &map_out, a, count);
+    }
+    if (!ok) atomicCAS(a.status, 0, 400 + warp);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (sm.abort_flag) {   // copies and products that are under way end within microseconds: none outlives the block's memory
+        const uint64_t t0 = global_ns();
+        while (global_ns() - t0 < 2'000'000ull) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 1) tmem_dealloc(sm.tmem_base, kTmemCols);
+}
+
+// Sums the shares of the tiles that were split, in the order of their depth, and hands them out.  Block (boundary, group of
+// eight warps' chunks); the first boundary inside a tile does it.
+__global__ void __launch_bounds__(256) join_split_kernel(const Args a, int grid) {
+    const int count = *a.count, p = (int)blockIdx.x + 1, lane = threadIdx.x & 31, id = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int warp = id >> 2, chunk = id & 3;
+    const SplitTiles t = split_tiles(a, count, grid);
+    const long long at = t.begin(p);
+    if (at >= t.rest) return;
+    int dw, tile;
+    long long start;
+    t.at(at, dw, tile, start);
+    const long long stop = start + (dw ? t.kw : t.kx);
+    if (at == start || t.begin(p - 1) > start) return;
+    // (p - 1 may begin the tile or lie before it; blocks without a share are passed over)
+    float v[32];
+    bool any = false;
+    for (int q = p - 1; q < grid; q++) {
+        const long long b = t.begin(q), e = t.begin(q + 1);
+        if (q >= p && b >= stop) break;
+        if (e <= start || b == e) continue;
+        const int slot = 2 * q + (b <= start ? 1 : 0);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float4 x = a.slots[slot_at(slot, warp, chunk, j, lane)];
+            v[4 * j] = any ? v[4 * j] + x.x : x.x;
+            v[4 * j + 1] = any ? v[4 * j + 1] + x.y : x.y;
+            v[4 * j + 2] = any ? v[4 * j + 2] + x.z : x.z;
+            v[4 * j + 3] = any ? v[4 * j + 3] + x.w : x.w;
+        }
+        any = true;
+    }
+    emit(a, count, dw, tile / t.d_tiles * kM + (warp & 3) * 32 + lane, tile % t.d_tiles * kN + (warp >> 2) * 128 + chunk * 32, v);
+}
+
+// ---- rows in, losses out -------------------------------------------------------------------------
+constexpr int kIndexThreads = 1024;
+
+// Compact numbers of the rows that have a target, in their order: a block per 1024 rows counts the ones before its own anew (all
+// of the targets come from L2 and a second launch costs more, up to some 10^5 rows).  Rows without one lose 0.
+__global__ void __launch_bounds__(kIndexThreads)
+index_rows_kernel(const int64_t* __restrict__ target, int64_t ignore, int64_t n_rows, int Tp, int vocab, int* header, int* rows, int* words,
+                  float* loss_rows) {
+    __shared__ int warp_sum[32], before_sum[32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t base = (int64_t)blockIdx.x * kIndexThreads;
+    int n = 0;
+    for (int64_t i = tid; i < base; i += kIndexThreads) n += target[i] != ignore;
+    n = __reduce_add_sync(~0u, n);
+    const int64_t t = base + tid;
+    const int64_t y = t < n_rows ? target[t] : ignore;
+    const bool on = t < n_rows && y != ignore;
+    const unsigned ballot = __ballot_sync(~0u, on);
+    if (lane == 0) {
+        before_sum[warp] = n;
+        warp_sum[warp] = __popc(ballot);
+    }
+    __syncthreads();
+    int before = __reduce_add_sync(~0u, before_sum[lane]);
+    const int mine = warp_sum[lane];
+    const int total = before + __reduce_add_sync(~0u, mine);
+    before += __reduce_add_sync(~0u, lane < warp ? mine : 0) + __popc(ballot & ((1u << lane) - 1));
+    if (on) {
+        rows[before] = (int)t;
+        words[before] = y >= 0 && y < vocab ? (int)y : -2;
+    } else if (t < n_rows && loss_rows) {
+        loss_rows[t] = 0.f;
+    }
+    if (blockIdx.x + 1 == gridDim.x) {
+        if (tid == 0) {
+            header[0] = total;   // rows that have a target
+            header[1] = 0;       // status
+            header[2] = 0;       // blocks of join_runs_kernel that are done
+        }
+        for (int i = total + tid; i < Tp; i += kIndexThreads) {
+            rows[i] = -1;
+            words[i] = -1;
+        }
+    }
+}
+
+__device__ __forceinline__ float as_float(float x) { return x; }
+__device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// The parts of a float32 value: what each rounding has left.  Infinities and NaN are their first part alone.
+__device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
+    p[0] = __float2bfloat16_rn(x);
+    float r = x - __bfloat162float(p[0]);
+    if (!isfinite(r)) r = 0.f;
+    p[1] = __float2bfloat16_rn(r);
+    p[2] = __float2bfloat16_rn(r - __bfloat162float(p[1]));
+}
+
+// Rows of a matrix as the products read them: `pitch` bf16 values each, zeros behind the d-th, one plane a part.  rows: the caller's
+// row of each (NULL: the same), zeros where it is -1; up to *count, rounded up to a row tile, if count is given.  A warp per row.
+template <typename T, int kPlanes>
+__global__ void __launch_bounds__(256)
+pack_rows_kernel(const T* __restrict__ x, int64_t stride, const int* __restrict__ rows, const int* __restrict__ count, int64_t n_rows, int d,
+                 int pitch, __nv_bfloat16* __restrict__ out, int vec) {
+    const int lane = threadIdx.x & 31;
+    const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (r >= n_rows || (count && r >= (int64_t)row_tiles(*count) * kM)) return;
+    const int64_t from = rows ? rows[r] : r;
+    const T* const src = x + (from < 0 ? 0 : from) * stride;
+    __nv_bfloat16* const dst = out + r * pitch;
+    if (kPlanes == 1 && vec) {   // (bf16, 16-byte aligned rows: pitch is d)
+        const uint4* s = reinterpret_cast<const uint4*>(src);
+        for (int i = lane; i < pitch / 8; i += 32) reinterpret_cast<uint4*>(dst)[i] = from < 0 ? make_uint4(0, 0, 0, 0) : s[i];
+        return;
+    }
+    const int64_t plane = n_rows * (int64_t)pitch;
+    for (int i = 2 * lane; i < pitch; i += 64) {
+        __nv_bfloat16 p[2][3];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const float v = from >= 0 && i + e < d ? as_float(src[i + e]) : 0.f;
+            if (kPlanes == 3) split3(v, p[e]);
+            else p[e][0] = __float2bfloat16_rn(v);
+        }
+#pragma unroll
+        for (int q = 0; q < kPlanes; q++) {
+            const __nv_bfloat162 both = {p[0][q], p[1][q]};
+            *reinterpret_cast<__nv_bfloat162*>(dst + q * plane + i) = both;
+        }
+    }
+}
+
+// Joins the runs of a row: m, 1 / s and the loss, and (not kRows) the losses' sum or mean: every block leaves its sum, the last one to
+// come adds them up in their order.  A lane per row, a warp per eighth of the runs.
+constexpr int kJoinWarps = 8;
+__global__ void __launch_bounds__(32 * kJoinWarps)
+join_runs_kernel(const float2* __restrict__ part, int n_parts, int Tp, int* header, const int* __restrict__ rows, const int* __restrict__ words,
+                 float* __restrict__ row_max, float* __restrict__ row_inv, const float* __restrict__ hit, float* __restrict__ loss, int reduction,
+                 double* __restrict__ sums) {
+    __shared__ float2 join[kJoinWarps][32];
+    __shared__ double warp_sum[kJoinWarps];
+    __shared__ bool is_last;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.x * 32 + lane, count = header[0];
+    const bool failed = header[1] != 0;
+    float top = -INFINITY, sum = 0.f;
+    auto add = [&](float2 p) {
+        const float best = fmaxf(top, p.x), ref = best == -INFINITY ? 0.f : best;
+        sum = sum * ex2((top - ref) * kLog2e) + p.y * ex2((p.x - ref) * kLog2e);
+        top = best;
+    };
+    if (r < count)
+        for (int i = warp; i < n_parts; i += kJoinWarps) add(part[(size_t)i * Tp + r]);
+    join[warp][lane] = make_float2(top, sum);
+    __syncthreads();
+    double mine = 0.0;
+    if (warp == 0) {
+        if (r < count) {
+            top = -INFINITY;
+            sum = 0.f;
+            for (int i = 0; i < kJoinWarps; i++) add(join[i][lane]);
+            row_max[r] = top;
+            row_inv[r] = 1.f / sum;
+            // (a row without any logit that is a number: NaN, as exp(-inf - -inf))
+            float l = words[r] == -2 || failed || top == -INFINITY ? NAN : (top - hit[r]) + logf(sum);
+            if (reduction == CDSSM_CE_NONE) loss[rows[r]] = l;
+            mine = (double)l;
+        }
+        for (int o = 16; o; o >>= 1) mine += __shfl_down_sync(~0u, mine, o);
+    }
+    if (reduction == CDSSM_CE_NONE) return;
+    if (threadIdx.x == 0) {
+        sums[blockIdx.x] = mine;
+        __threadfence();
+        is_last = atomicAdd(&header[2], 1) + 1 == (int)gridDim.x;
+    }
+    __syncthreads();
+    if (!is_last) return;
+    __threadfence();
+    double total = 0.0;
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += 32 * kJoinWarps) total += __ldcg(&sums[i]);
+    for (int o = 16; o; o >>= 1) total += __shfl_down_sync(~0u, total, o);
+    if (lane == 0) warp_sum[warp] = total;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        total = 0.0;
+        for (int i = 0; i < kJoinWarps; i++) total += warp_sum[i];
+        *loss = (float)(reduction == CDSSM_CE_MEAN ? total / (double)count : total);   // (mean of no rows: NaN)
+    }
+}
+
+// dx of the rows without a target: zero.  After a wait that ran out everything is NaN.  A warp per row.
+template <typename T>
+__global__ void __launch_bounds__(256)
+blank_rows_kernel(const int64_t* __restrict__ target, int64_t ignore, int64_t n_rows, int d, const int* __restrict__ header, T* __restrict__ dx) {
+    const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (r >= n_rows) return;
+    const bool failed = header[1] != 0;
+    if (!failed && target[r] != ignore) return;
+    for (int i = threadIdx.x & 31; i < d; i += 32) dx[r * (int64_t)d + i] = failed ? T(NAN) : T(0.f);
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+inline size_t up(size_t n, size_t to) { return (n + to - 1) / to * to; }
+
+struct Sizes {
+    int64_t rows;
+    int d, V, planes, terms, Tp, pitch, n_tiles, run, n_runs, pieces, vn, d_tiles;
+    bool f32;
+    // saved
+    size_t o_rows, o_words, o_max, o_inv, o_hit, o_x, saved;
+    // scratch of the forward (W's planes if it is not read in place) and of the backward
+    size_t w_planes, o_part, o_sums, fwd, o_dz, o_acc, o_slots, bwd;
+};
+constexpr size_t kPieceBytes = 512ull << 20;   // of dz, beyond which the vocabulary is cut
+constexpr int kMostRun = 8;                    // vocabulary tiles of a run: a tenth of a per cent of the row sums' traffic, still even shares
+
+bool sizes_of(int64_t rows, int d, int vocab, int dtype, int sms, Sizes& s) {
+    if (rows < 1 || d < 1 || vocab < 1 || (dtype != CDSSM_BF16 && dtype != CDSSM_F32)) return false;
+    s.rows = rows; s.d = d; s.V = vocab;
+    s.f32 = dtype == CDSSM_F32;
+    s.planes = s.f32 ? 3 : 1;
+    s.terms = s.f32 ? kTerms3 : 1;
+    s.Tp = (int)up(rows, kRowTile);
+    s.pitch = (int)up(d, 8);
+    s.n_tiles = (vocab + kN - 1) / kN;
+    const int64_t tiles = (int64_t)(s.Tp / kM) * s.n_tiles;
+    s.run = (int)std::min<int64_t>(kMostRun, std::max<int64_t>(1, tiles / (8 * (int64_t)sms)));
+    s.n_runs = (s.n_tiles + s.run - 1) / s.run;
+    const size_t column = (size_t)s.Tp * 2 * s.planes;
+    const size_t most = std::max<size_t>(kN, kPieceBytes / column / kN * kN);
+    s.pieces = (int)((up(vocab, kN) + most - 1) / most);
+    s.vn = (int)up((vocab + s.pieces - 1) / s.pieces, kN);
+    s.pieces = (vocab + s.vn - 1) / s.vn;
+    s.d_tiles = (d + kN - 1) / kN;
+    size_t o = 256;
+    auto take = [&](size_t bytes) { const size_t at = o; o += up(bytes, 256); return at; };
+    s.o_rows = take(4ull * s.Tp); s.o_words = take(4ull * s.Tp); s.o_max = take(4ull * s.Tp); s.o_inv = take(4ull * s.Tp);
+    s.o_hit = take(4ull * s.Tp); s.o_x = take(2ull * s.planes * s.Tp * s.pitch);
+    s.saved = o;
+    s.w_planes = up(2ull * s.planes * (size_t)vocab * s.pitch, 256);
+    o = s.w_planes;
+    s.o_part = take(8ull * 2 * s.n_runs * s.Tp); s.o_sums = take(8ull * (s.Tp / 32));
+    s.fwd = o;
+    o = s.w_planes;
+    s.o_dz = take(column * s.vn); s.o_acc = take(s.pieces > 1 ? 4ull * s.Tp * s.d_tiles * kN : 0);
+    s.o_slots = take(2ull * sms * kM * kN * 4);
+    s.bwd = o;
+    return true;
+}
+
+int checked_sizes(int64_t rows, int d, int vocab, int dtype, Sizes& s) {
+    if (rows < 1 || d < 1 || vocab < 1) return CDSSM_ERR_BAD_ARG;
+    if (rows > (1 << 24) || d > (1 << 16) || vocab > (1 << 24)) return CDSSM_ERR_UNSUPPORTED;   // (tile numbers and row numbers in 32 bits)
+    int sms = 0;
+    if (int rc = sm_count(sms)) return rc;
+    return sizes_of(rows, d, vocab, dtype, sms, s) ? CDSSM_OK : CDSSM_ERR_BAD_ARG;
+}
+
+// (planes, rows, cols) bf16, boxes of box_r rows x box_c columns
+bool make_map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int planes, int64_t pitch, int box_c, int box_r) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)pitch * 2, (cuuint64_t)pitch * rows * 2};
+    const cuuint32_t box[3] = {(cuuint32_t)box_c, (cuuint32_t)box_r, 1}, step[3] = {1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int kMode> struct Tag {};
+template <int kMode>
+int launch_products(const Maps& maps, const CUtensorMap& out, const Args& a, int grid, cudaStream_t st) {
+    if (int rc = allow_smem<Tag<kMode>>((const void*)product_kernel<kMode>, sizeof(Smem))) return rc;
+    product_kernel<kMode><<<grid, kThreads, sizeof(Smem), st>>>(maps, out, a);
+    return check_launch();
+}
+
+bool in_place(const void* w, int64_t stride, int dtype) {   // a matrix that TMA reads as it lies
+    return dtype == CDSSM_BF16 && stride % 8 == 0 && ((uintptr_t)w & 15) == 0;
+}
+
+template <typename T, int kPlanes>
+int pack(const void* x, int64_t stride, const int* rows, const int* count, int64_t n, const Sizes& s, void* out, bool vec, cudaStream_t st) {
+    pack_rows_kernel<T, kPlanes><<<(unsigned)((n + 7) / 8), 256, 0, st>>>(static_cast<const T*>(x), stride, rows, count, n, s.d, s.pitch,
+                                                                          static_cast<__nv_bfloat16*>(out), vec);
+    return check_launch();
+}
+int pack_any(const void* x, int64_t stride, const int* rows, const int* count, int64_t n, const Sizes& s, void* out, cudaStream_t st) {
+    if (s.f32) return pack<float, 3>(x, stride, rows, count, n, s, out, false, st);
+    return pack<__nv_bfloat16, 1>(x, stride, rows, count, n, s, out, s.d % 8 == 0 && in_place(x, stride, CDSSM_BF16), st);
+}
+
+void fill_saved(Args& a, const Sizes& s, char* saved) {
+    a = Args{};
+    int* header = reinterpret_cast<int*>(saved);
+    a.count = header;
+    a.status = header + 1;
+    a.rows = reinterpret_cast<int*>(saved + s.o_rows);
+    a.target = reinterpret_cast<int*>(saved + s.o_words);
+    a.row_max = reinterpret_cast<float*>(saved + s.o_max);
+    a.row_inv = reinterpret_cast<float*>(saved + s.o_inv);
+    a.hit = reinterpret_cast<float*>(saved + s.o_hit);
+    a.planes = s.planes; a.terms = s.terms; a.Tp = s.Tp; a.d = s.d; a.V = s.V;
+    a.run = s.run; a.n_tiles = s.n_tiles; a.n_runs = s.n_runs; a.d_tiles = s.d_tiles;
+    a.f32 = s.f32;
+    a.vec_dx = a.vec_dw = s.d % (s.f32 ? 4 : 8) == 0;
+    a.wait_ns = wait_limit_ns();
+}
+
+}  // namespace ce
+}  // namespace cdssm
+
+using namespace cdssm;
+
+extern "C" size_t cdssm_b200_linear_ce_saved_bytes(int64_t rows, int d, int vocab, int dtype) {
+    ce::Sizes s;
+    return ce::checked_sizes(rows, d, vocab, dtype, s) == CDSSM_OK ? s.saved : 0;
+}
+extern "C" size_t cdssm_b200_linear_ce_workspace_bytes(int64_t rows, int d, int vocab, int dtype, int backward) {
+    ce::Sizes s;
+    return ce::checked_sizes(rows, d, vocab, dtype, s) == CDSSM_OK ? (backward ? s.bwd : s.fwd) : 0;
+}
+
+extern "C" int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, const void* w, int64_t w_row_stride, const int64_t* target,
+                                        float* loss, void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes, int64_t rows,
+                                        int d, int vocab, int64_t ignore_index, int reduction, int dtype, int flags, void* stream) {
+    if (!x || !w || !target || !loss || !saved || !workspace || reduction < CDSSM_CE_NONE || reduction > CDSSM_CE_SUM) return CDSSM_ERR_BAD_ARG;
+    if (x_row_stride < 0 || w_row_stride < d) return CDSSM_ERR_BAD_ARG;
+    ce::Sizes s;
+    if (int rc = ce::checked_sizes(rows, d, vocab, dtype, s)) return rc;
+    if (saved_bytes < s.saved || workspace_bytes < s.fwd || ((uintptr_t)saved & 255) || ((uintptr_t)workspace & 255)) return CDSSM_ERR_WORKSPACE;
+    const cudaStream_t st = (cudaStream_t)stream;
+    int sms = 0;
+    if (int rc = sm_count(sms)) return rc;
+    char *const sv = static_cast<char*>(saved), *const ws = static_cast<char*>(workspace);
+    ce::Args a;
+    ce::fill_saved(a, s, sv);
+    int* header = reinterpret_cast<int*>(sv);
+    ce::index_rows_kernel<<<(unsigned)((rows + ce::kIndexThreads - 1) / ce::kIndexThreads), ce::kIndexThreads, 0, st>>>(
+        target, ignore_index, rows, s.Tp, vocab, header, const_cast<int*>(a.rows), const_cast<int*>(a.target),
+        reduction == CDSSM_CE_NONE ? loss : nullptr);
+    if (int rc = check_launch()) return rc;
+    if (int rc = ce::pack_any(x, x_row_stride, a.rows, a.count, s.Tp, s, sv + s.o_x, st)) return rc;
+    const bool direct = ce::in_place(w, w_row_stride, dtype);
+    if (!direct)
+        if (int rc = ce::pack_any(w, w_row_stride, nullptr, nullptr, vocab, s, ws, st)) return rc;
+    ce::Maps maps{};
+    if (!ce::make_map(&maps.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, ce::kM) ||
+        !ce::make_map(&maps.b, direct ? w : ws, direct ? d : s.pitch, vocab, s.planes, direct ? w_row_stride : s.pitch, ce::kK, ce::kN))
+        return CDSSM_ERR_CUDA;
+    a.part = reinterpret_cast<float2*>(ws + s.o_part);
+    a.withhold = (flags & CDSSM_SCAN_TEST_WITHHOLD) != 0;
+    const int64_t units = (int64_t)(s.Tp / ce::kM) * s.n_runs;
+    if (int rc = ce::launch_products<ce::kStats>(maps, maps.a, a, (int)std::min<int64_t>(units, sms), st)) return rc;
+    ce::join_runs_kernel<<<s.Tp / 32, 32 * ce::kJoinWarps, 0, st>>>(a.part, 2 * s.n_runs, s.Tp, header, a.rows, a.target, a.row_max, a.row_inv,
+                                                                  a.hit, loss, reduction, reinterpret_cast<double*>(ws + s.o_sums));
+    return check_launch();
+}
+
+extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, int64_t w_row_stride, const int64_t* target, void* saved,
+                                        size_t saved_bytes, void* grad_x, void* grad_w, void* workspace, size_t workspace_bytes, int64_t rows,
+                                        int d, int vocab, int64_t ignore_index, int reduction, int dtype, int flags, void* stream) {
+    if (!grad_loss || !w || !target || !saved || !workspace || (!grad_x && !grad_w) || reduction < CDSSM_CE_NONE || reduction > CDSSM_CE_SUM)
+        return CDSSM_ERR_BAD_ARG;
+    if (w_row_stride < d || ((uintptr_t)grad_x & 15) || ((uintptr_t)grad_w & 15)) return CDSSM_ERR_BAD_ARG;
+    ce::Sizes s;
+    if (int rc = ce::checked_sizes(rows, d, vocab, dtype, s)) return rc;
+    if (saved_bytes < s.saved || workspace_bytes < s.bwd || ((uintptr_t)saved & 255) || ((uintptr_t)workspace & 255)) return CDSSM_ERR_WORKSPACE;
+    const cudaStream_t st = (cudaStream_t)stream;
+    int sms = 0;
+    if (int rc = sm_count(sms)) return rc;
+    char *const sv = static_cast<char*>(saved), *const ws = static_cast<char*>(workspace);
+    const bool direct = ce::in_place(w, w_row_stride, dtype);
+    if (!direct)
+        if (int rc = ce::pack_any(w, w_row_stride, nullptr, nullptr, vocab, s, ws, st)) return rc;
+    const void* const wb = direct ? w : ws;
+    const int64_t w_cols = direct ? d : s.pitch, w_pitch = direct ? w_row_stride : s.pitch;
+    ce::Maps logits{}, grads{};
+    CUtensorMap dz;
+    if (!ce::make_map(&logits.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, ce::kM) ||
+        !ce::make_map(&logits.b, wb, w_cols, vocab, s.planes, w_pitch, ce::kK, ce::kN) ||
+        !ce::make_map(&dz, ws + s.o_dz, s.vn, s.Tp, s.planes, s.vn, 64, 32) ||
+        !ce::make_map(&grads.a, ws + s.o_dz, s.vn, s.Tp, s.planes, s.vn, ce::kK, ce::kM) ||
+        !ce::make_map(&grads.b, wb, w_cols, vocab, s.planes, w_pitch, 64, ce::kK) ||
+        !ce::make_map(&grads.a2, ws + s.o_dz, s.vn, s.Tp, s.planes, s.vn, 64, ce::kK) ||
+        !ce::make_map(&grads.b2, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, 64, ce::kK))
+        return CDSSM_ERR_CUDA;
+    ce::Args a;
+    ce::fill_saved(a, s, sv);
+    a.grad = grad_loss;
+    a.grad_rows = reduction == CDSSM_CE_NONE;
+    a.mean = reduction == CDSSM_CE_MEAN;
+    a.dx = grad_x; a.dw = grad_w;
+    a.acc = reinterpret_cast<float*>(ws + s.o_acc);
+    a.acc_pitch = s.d_tiles * ce::kN;
+    a.slots = reinterpret_cast<float4*>(ws + s.o_slots);
+    a.withhold = (flags & CDSSM_SCAN_TEST_WITHHOLD) != 0;
+    for (int p = 0; p < s.pieces; p++) {
+        a.v0 = p * s.vn;
+        a.vn = std::min(s.vn, vocab - a.v0);
+        a.vn_tiles = (a.vn + ce::kN - 1) / ce::kN;
+        a.first = p == 0;
+        a.last = p + 1 == s.pieces;
+        if (int rc = ce::launch_products<ce::kGradLogits>(logits, dz, a, sms, st)) return rc;
+        if (int rc = ce::launch_products<ce::kGradProducts>(grads, dz, a, sms, st)) return rc;
+        ce::join_split_kernel<<<dim3(sms, 4), 256, 0, st>>>(a, sms);
+        if (int rc = check_launch()) return rc;
+    }
+    if (grad_x) {
+        const unsigned grid = (unsigned)((rows + 7) / 8);
+        if (s.f32) ce::blank_rows_kernel<<<grid, 256, 0, st>>>(target, ignore_index, rows, d, a.count, static_cast<float*>(grad_x));
+        else ce::blank_rows_kernel<<<grid, 256, 0, st>>>(target, ignore_index, rows, d, a.count, static_cast<__nv_bfloat16*>(grad_x));
+        if (int rc = check_launch()) return rc;
+    }
+    return CDSSM_OK;
+}

@@ -206,6 +206,18 @@ class CdssmLM:
         return ops._lib.host().lm_forward(self._native(), self._ids(input_ids), self.per_token_group_norm, scan_flags)
 
     @torch.no_grad()
+    def loss(self, input_ids, targets=None, *, ignore_index=-100, reduction="mean", scan_flags=0):
+        """Cross entropy of the model's predictions, as cdssm/training/trainer.py:219-262 takes it from forward()'s logits, which are
+        not formed here (:func:`ops.linear_cross_entropy`).  input_ids (B,L); targets (B,L), by default the next ids of each row
+        (the last position has none).  "mean" and "sum" give one float32 value, "none" one per position."""
+        ids = self._ids(input_ids)
+        if targets is None:
+            targets = torch.full_like(ids, ignore_index, dtype=torch.int64)
+            targets[:, :-1] = ids[:, 1:]
+        hidden = ops._lib.host().lm_hidden(self._native(), ids, self.per_token_group_norm, scan_flags)
+        return ops.linear_cross_entropy(hidden, self.embedding, self._ids(targets), ignore_index=ignore_index, reduction=reduction)
+
+    @torch.no_grad()
     def prefill(self, input_ids, last_only=True):
         """Prefill that also returns the decode cache: per layer the recurrent state after the last
         token (B,H,N,D) fp32 and the last three conv inputs; plus the position counter."""

@@ -14,6 +14,7 @@ fallback: tensors must be CUDA tensors and the library must be built.
 import torch
 from torch import Tensor
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import CdssmError, check
@@ -21,6 +22,7 @@ from ._lib import CdssmError, check
 __all__ = ["CUDAConv1dSiLUOp", "DynamicsFusedFn", "NormalizeKQFn", "IntraChunkScanFn",
            "InterChunkScanFn", "ExactCorrectionFn", "scan_fused", "decode_step", "decode_step_reference", "reference_decode_state",
            "scan_fused_workspace_bytes", "scan_fused_status", "set_wait_limit_ns", "selftest_bounded_wait", "rms_norm", "groupnorm_gate", "conv1d_silu_step", "scan_summary", "scan_fused_long", "compose_carries",
+           "LinearCrossEntropyFn", "linear_cross_entropy",
            "CdssmError"]
 
 _DT = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
@@ -166,6 +168,50 @@ class ExactCorrectionFn(Function):
         (exact_correction.cu:169-383)."""
         return _lib.host().correction_bwd(grad_corrections, *ctx.saved_tensors, ctx.state_dim,
                                           0 if EXACT_CORRECTION_TRUE_GRADIENT else 1) + (None,)
+
+
+# ------------------------------------------------------------------------------------------
+# The ends of a training step
+# ------------------------------------------------------------------------------------------
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+class LinearCrossEntropyFn(Function):
+    """Softmax cross entropy of hidden rows against a vocabulary, without the logits: see :func:`linear_cross_entropy`."""
+
+    @staticmethod
+    def forward(ctx, hidden: Tensor, weight: Tensor, targets: Tensor, ignore_index: int = -100, reduction: str = "mean",
+                flags: int = 0) -> Tensor:
+        if reduction not in _REDUCTIONS:
+            raise CdssmError(f"reduction must be 'none', 'mean' or 'sum', not {reduction!r}")
+        ctx.args = (int(ignore_index), _REDUCTIONS[reduction])
+        ctx.hidden_shape, ctx.flags = hidden.shape, int(flags)
+        loss, saved = _lib.host().linear_ce_fwd(hidden, weight, targets, *ctx.args, ctx.flags)
+        ctx.save_for_backward(weight, targets, saved)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_loss):
+        """(grad_hidden, grad_weight, None x 4)"""
+        weight, targets, saved = ctx.saved_tensors
+        gx, gw = _lib.host().linear_ce_bwd(grad_loss, weight, targets, saved, *ctx.args, *ctx.needs_input_grad[:2], ctx.flags)
+        return (None if gx is None else gx.view(ctx.hidden_shape), gw) + (None,) * 4
+
+
+def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ignore_index: int = -100,
+                         reduction: str = "mean") -> Tensor:
+    """Cross entropy of ``hidden @ weight.T`` against ``targets``: the LM head and the loss of a training step in one
+    (cdssm/models/model.py:50-51, cdssm/training/trainer.py:219-262), with the (tokens, vocabulary) logits and their gradient never
+    in memory as a whole.
+
+    hidden (..., d) and weight (vocab, d) bfloat16 or float32, of one type (under autocast pass ``weight.to(hidden.dtype)``);
+    targets (...) int64.  Rows whose target is ``ignore_index`` lose 0, take no part in the mean and get zero gradients, whatever
+    they hold (infinities and NaN too).  A target that is neither a word nor ignore_index makes its row's loss NaN.
+    reduction "mean" (NaN when every row is ignored), "sum" or "none" (targets' shape); the loss is float32.
+    Products are bfloat16 ones with float32 sums, for float32 operands exact to 24 bits; the logits' gradient is rounded once to the
+    products' type.  Gradients have the operands' type and are the same from run to run.  Differentiable once."""
+    return LinearCrossEntropyFn.apply(hidden, weight, targets, ignore_index, reduction)
 
 
 # ------------------------------------------------------------------------------------------

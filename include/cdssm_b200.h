@@ -442,6 +442,36 @@ CDSSM_API int cdssm_b200_decode_step_reference(float* local_state, float* correc
                                                float shortcut_scale, int B, int H, int D, int N, int C, int pos,
                                                const int* pos_dev, int dtype, void* stream);
 
+/* ---- the ends of a training step: embedding, loss, gradient norm ------------------------------------- */
+
+/* Softmax cross entropy of hidden rows against a vocabulary, without the logits in memory: with z = x w^T,
+ *   loss_t = log sum_v exp(z_tv) - z_t,target(t);   rows whose target is ignore_index lose 0 and take no part.
+ * x (rows,d) with x_row_stride elements between rows; w (vocab,d) with w_row_stride; target (rows) int64.
+ * reduction: CDSSM_CE_NONE loss (rows), CDSSM_CE_MEAN (over the rows that take part; NaN without any) or CDSSM_CE_SUM one value;
+ * loss is float32.  A row whose target is neither a word nor ignore_index loses NaN.
+ * saved (cdssm_b200_linear_ce_saved_bytes) is what the backward reads: keep it as it is, 256-byte aligned, as the workspace
+ * (cdssm_b200_linear_ce_workspace_bytes), which is free again behind the call.  Both sizes are for the current device, 0 on
+ * bad sizes.  rows <= 2^24, vocab <= 2^24, d <= 65536.  bf16 products with float32 sums; float32 operands enter as three bf16 parts.
+ * flags: 0 or CDSSM_SCAN_TEST_WITHHOLD.  After a bounded wait that ran out the loss is NaN.
+ * Replaces the LM head and the loss of a training step: cdssm/models/model.py:50-51, cdssm/training/trainer.py:219-262. */
+#define CDSSM_CE_NONE 0
+#define CDSSM_CE_MEAN 1
+#define CDSSM_CE_SUM 2
+CDSSM_API size_t cdssm_b200_linear_ce_saved_bytes(int64_t rows, int d, int vocab, int dtype);
+CDSSM_API size_t cdssm_b200_linear_ce_workspace_bytes(int64_t rows, int d, int vocab, int dtype, int backward);
+CDSSM_API int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, const void* w, int64_t w_row_stride,
+                                       const int64_t* target, float* loss, void* saved, size_t saved_bytes, void* workspace,
+                                       size_t workspace_bytes, int64_t rows, int d, int vocab, int64_t ignore_index,
+                                       int reduction, int dtype, int flags, void* stream);
+
+/* Its backward: grad_loss (rows for CDSSM_CE_NONE, else one value) float32 -> grad_x (rows,d) and grad_w (vocab,d), dense, in the
+ * storage type, 16-byte aligned; either may be NULL.  w, target and the other arguments as in the forward that left saved.
+ * dz is formed a piece of the vocabulary at a time (at most 512 MiB of scratch while a row tile allows).  Sums run in a fixed order. */
+CDSSM_API int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, int64_t w_row_stride, const int64_t* target,
+                                       void* saved, size_t saved_bytes, void* grad_x, void* grad_w, void* workspace,
+                                       size_t workspace_bytes, int64_t rows, int d, int vocab, int64_t ignore_index,
+                                       int reduction, int dtype, int flags, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
