@@ -69,6 +69,11 @@ SIGNATURES = {
     "cdssm_b200_linear_ce_workspace_bytes": (_c_size_t, [_c_int64] + [_I] * 4),
     "cdssm_b200_linear_ce_fwd": (_I, [_P, _c_int64, _P, _c_int64, _P, _P, _P, _c_size_t, _P, _c_size_t, _c_int64, _I, _I, _c_int64] + [_I] * 3 + [_P]),
     "cdssm_b200_linear_ce_bwd": (_I, [_P, _P, _c_int64, _P, _P, _c_size_t, _P, _P, _P, _c_size_t, _c_int64, _I, _I, _c_int64] + [_I] * 3 + [_P]),
+    "cdssm_b200_embedding_fwd": (_I, [_P, _P, _c_int64, _P, _c_int64, _I, _I, _F, _I, _P]),
+    "cdssm_b200_embedding_bwd_workspace_bytes": (_c_size_t, [_c_int64] + [_I] * 3),
+    "cdssm_b200_embedding_bwd": (_I, [_P] * 4 + [_c_size_t, _c_int64, _I, _I, _c_int64, _F, _I, _P]),
+    "cdssm_b200_grad_clip_workspace_bytes": (_c_size_t, [_P, _I]),
+    "cdssm_b200_grad_clip": (_I, [_P] * 5 + [_I, _F, _P, _P, _c_size_t, _P]),
     "cdssm_b200_decode_step_at": (_I, [_P] * 8 + [_F] * 6 + [_I] * 4 + [_P, _I, _P]),
 }
 

@@ -1,0 +1,359 @@
+// Rows of a table for token ids, and the table's gradient by sorted tokens.
+//
+// out_t = scale * W[id_t];   dW[v] = scale * sum over t with id_t = v of g_t, in the order of t.
+// The gradient without atomics: (id, t) pairs are sorted, every kTile of them are summed in their order, and an id that goes on over
+// tiles is joined from the tiles' float32 partial sums, again in order: the same bits from run to run.  While one cluster of blocks
+// sorts (a few microseconds of latency for a few KB), the others fill dW with the zeros that most of its rows keep.
+#include "cdssm_common.cuh"
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+
+namespace cdssm {
+namespace emb {
+
+namespace cg = cooperative_groups;
+
+// ---- values of a 16-byte vector, or single ones where rows are no multiple of it ---------------------
+template <typename T, int kE> struct Vec { T v[kE]; };
+template <typename T, int kE> __device__ __forceinline__ void load(const T* p, float (&f)[kE]) {
+    if constexpr (kE == 1) {
+        if constexpr (sizeof(T) == 2) f[0] = __bfloat162float(*p);
+        else f[0] = *p;
+    } else if constexpr (sizeof(T) == 2) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    } else {
+        const float4 u = __ldg(reinterpret_cast<const float4*>(p));
+        f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
+    }
+}
+template <typename T, int kE> __device__ __forceinline__ void store(T* p, const float (&f)[kE]) {
+    if constexpr (kE == 1) {
+        if constexpr (sizeof(T) == 2) *p = __float2bfloat16_rn(f[0]);
+        else *p = f[0];
+    } else if constexpr (sizeof(T) == 2) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = reinterpret_cast<const uint32_t&>(b);
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+        *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+    }
+}
+
+// A thread per vector of the output; an id that is no row of the table gives NaN.
+template <typename T, int kE>
+__global__ void __launch_bounds__(256)
+embed_kernel(const int64_t* __restrict__ ids, const T* __restrict__ w, int64_t w_stride, T* __restrict__ out, int64_t n, int vocab, int d, float scale) {
+    const int per_row = d / kE;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t t = i / per_row;
+    if (t >= n) return;
+    const int c = (int)(i - t * per_row) * kE;
+    const int64_t id = ids[t];
+    float f[kE];
+    if (id >= 0 && id < vocab) {
+        load<T, kE>(w + id * w_stride + c, f);
+#pragma unroll
+        for (int e = 0; e < kE; e++) f[e] *= scale;
+    } else {
+#pragma unroll
+        for (int e = 0; e < kE; e++) f[e] = NAN;
+    }
+    store<T, kE>(out + t * d + c, f);
+}
+
+// ---- sort ------------------------------------------------------------------------------------------
+constexpr int kSortThreads = 1024, kItems = 4, kMostBits = 9, kBins = 1 << kMostBits;
+
+struct SortSmem {
+    int hist[kBins];              // this block's, read by the others of the cluster
+    int base[kBins];              // where this block's next key of a digit goes
+    int warp_total[32];
+    unsigned short count[32][kBins];   // keys of a digit in a warp's part of the sub-tile, then in the warps before
+};
+
+// The cluster of blocks 0 .. clusterDim - 1 sorts (key, token) pairs by key, stable, `bits` bits a pass, each block a contiguous part
+// of the pairs; the other clusters write zeros.  Ids that take no part (no row of the table, `skip`) get the key vocab: behind all others.
+__global__ void __launch_bounds__(kSortThreads)
+sort_and_clear_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t skip, int bits, int passes, uint2* buf0, uint2* buf1,
+                      uint4* __restrict__ zero, size_t zero_vecs, unsigned char* zero_tail, int tail_bytes) {
+    __shared__ SortSmem sm;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), c = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if ((int)blockIdx.x >= C) {
+        const size_t step = (size_t)(gridDim.x - C) * kSortThreads;
+        for (size_t i = (size_t)(blockIdx.x - C) * kSortThreads + tid; i < zero_vecs; i += step) __stcs(zero + i, make_uint4(0, 0, 0, 0));
+        if ((int)blockIdx.x == C && tid < tail_bytes) zero_tail[tid] = 0;
+        return;
+    }
+    const int chunk = (n + C - 1) / C, lo = min(n, c * chunk), hi = min(n, lo + chunk);
+    const int bins = 1 << bits;
+    for (int pass = 0; pass < passes; pass++) {
+        const uint2* const from = pass & 1 ? buf0 : buf1;
+        uint2* const to = pass & 1 ? buf1 : buf0;
+        auto pair_at = [&](int i) -> uint2 {
+            if (pass) return __ldcg(from + i);
+            const int64_t id = ids[i];
+            return make_uint2(id >= 0 && id < vocab && id != skip ? (unsigned)id : (unsigned)vocab, (unsigned)i);
+        };
+        const int shift = pass * bits;
+        auto digit_of = [&](unsigned key) { return (int)(key >> shift) & (bins - 1); };
+        for (int b = tid; b < bins; b += kSortThreads) sm.hist[b] = 0;
+        __syncthreads();
+        for (int i = lo + tid; i < hi; i += kSortThreads) atomicAdd(&sm.hist[digit_of(pair_at(i).x)], 1);
+        cluster.sync();
+        int before = 0, total = 0;
+        if (tid < bins)
+            for (int q = 0; q < C; q++) {
+                const int h = cluster.map_shared_rank(sm.hist, q)[tid];
+                total += h;
+                if (q < c) before += h;
+            }
+        int scan = total;   // over the digits
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(~0u, scan, o);
+            if (lane >= o) scan += x;
+        }
+        if (lane == 31) sm.warp_total[warp] = scan;
+        __syncthreads();
+        int warps_before = lane < warp ? sm.warp_total[lane] : 0;
+        warps_before = __reduce_add_sync(~0u, warps_before);
+        if (tid < bins) sm.base[tid] = warps_before + scan - total + before;
+        for (int s = lo; s < hi; s += kSortThreads * kItems) {
+            for (int i = tid; i < 32 * kBins / 2; i += kSortThreads) reinterpret_cast<unsigned*>(sm.count)[i] = 0;
+            __syncthreads();
+            uint2 pair[kItems];
+            int digit[kItems], rank[kItems];
+#pragma unroll
+            for (int k = 0; k < kItems; k++) {   // a warp's keys lie in a row
+                const int i = s + (warp * kItems + k) * 32 + lane;
+                pair[k] = i < hi ? pair_at(i) : make_uint2(0, 0);
+                digit[k] = i < hi ? digit_of(pair[k].x) : bins;
+            }
+#pragma unroll
+            for (int k = 0; k < kItems; k++) {
+                const unsigned same = __match_any_sync(~0u, digit[k]);
+                const int old = digit[k] < bins ? sm.count[warp][digit[k]] : 0;
+                rank[k] = old + __popc(same & ((1u << lane) - 1));
+                __syncwarp();
+                if (digit[k] < bins && lane == __ffs(same) - 1) sm.count[warp][digit[k]] = (unsigned short)(old + __popc(same));
+                __syncwarp();
+            }
+            __syncthreads();
+            int here = 0;
+            if (tid < bins)
+                for (int q = 0; q < 32; q++) {
+                    const int x = sm.count[q][tid];
+                    sm.count[q][tid] = (unsigned short)here;
+                    here += x;
+                }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kItems; k++)
+                if (digit[k] < bins) to[sm.base[digit[k]] + sm.count[warp][digit[k]] + rank[k]] = pair[k];
+            __syncthreads();
+            if (tid < bins) sm.base[tid] += here;
+            __syncthreads();
+        }
+        __threadfence();
+        cluster.sync();
+    }
+}
+
+// ---- sums --------------------------------------------------------------------------------------------
+// kTile sorted pairs of some columns a block: rows of one id are added up in their order.  An id that lies inside the tile is done; of
+// one that came from the tile before the sum goes to head, of one that goes on into the next (and began here) to tail.
+template <typename T, int kE, int kTile>
+__global__ void sum_tiles_kernel(const uint2* __restrict__ pairs, int n, int vocab, const T* __restrict__ grad, T* __restrict__ dw,
+                                 float* __restrict__ head, float* __restrict__ tail, int d, float scale) {
+    __shared__ uint2 tile[kTile + 2];   // with the neighbours of either side
+    const int tile_id = blockIdx.x, p0 = tile_id * kTile;
+    for (int i = threadIdx.x; i < kTile + 2; i += blockDim.x) {
+        const int p = p0 + i - 1;
+        tile[i] = p >= 0 && p < n ? pairs[p] : make_uint2((unsigned)vocab, 0);
+    }
+    __syncthreads();
+    const int c = (blockIdx.y * blockDim.x + threadIdx.x) * kE;
+    if (c >= d) return;
+    float sum[kE] = {};
+    bool from_before = p0 > 0 && tile[0].x == tile[1].x;
+    constexpr int kAhead = kTile < 8 ? kTile : 8;
+    for (int i0 = 0; i0 < kTile; i0 += kAhead) {
+        if (tile[i0 + 1].x >= (unsigned)vocab) return;
+        float g[kAhead][kE];
+#pragma unroll
+        for (int k = 0; k < kAhead; k++)
+            if (tile[i0 + k + 1].x < (unsigned)vocab) load<T, kE>(grad + (size_t)tile[i0 + k + 1].y * d + c, g[k]);
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const unsigned id = tile[i0 + k + 1].x;
+            if (id >= (unsigned)vocab) return;
+#pragma unroll
+            for (int e = 0; e < kE; e++) sum[e] += g[k][e];
+            const bool ends = tile[i0 + k + 2].x != id, edge = i0 + k + 1 == kTile;
+            if (ends || edge) {
+                if (from_before || !ends) {
+                    float* const to = (from_before ? head : tail) + (size_t)tile_id * d + c;
+#pragma unroll
+                    for (int e = 0; e < kE; e++) to[e] = sum[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kE; e++) sum[e] *= scale;
+                    store<T, kE>(dw + (size_t)id * d + c, sum);
+                }
+#pragma unroll
+                for (int e = 0; e < kE; e++) sum[e] = 0.f;
+                from_before = false;
+            }
+        }
+    }
+}
+
+// An id that begins in this tile and goes on: its tail and the heads of the tiles behind, eight contiguous parts beside each other.
+constexpr int kJoinParts = 8;
+template <typename T, int kTile>
+__global__ void __launch_bounds__(32 * kJoinParts)
+join_tiles_kernel(const uint2* __restrict__ pairs, int n, int vocab, const float* __restrict__ head, const float* __restrict__ tail, T* __restrict__ dw,
+                  int d, float scale) {
+    __shared__ float part[kJoinParts][32];
+    const int tile_id = blockIdx.x, last = tile_id * kTile + kTile - 1;
+    if (last + 1 >= n) return;
+    const unsigned id = pairs[last].x;
+    if (id >= (unsigned)vocab || pairs[last + 1].x != id) return;
+    if (tile_id > 0 && pairs[last - kTile].x == id) return;   // it came from the tile before
+    int lo = last + 1, hi = n;                                 // first pair of another id
+    while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (pairs[mid].x == id) lo = mid + 1;
+        else hi = mid;
+    }
+    const int tiles = (lo - 1) / kTile - tile_id + 1, lane = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int share = (tiles + kJoinParts - 1) / kJoinParts, q0 = y * share, q1 = min(tiles, q0 + share);
+    const int c = blockIdx.y * 32 + lane;
+    float sum = 0.f;
+    if (c < d)
+#pragma unroll 8
+        for (int q = q0; q < q1; q++) sum += (q ? head : tail)[(size_t)(tile_id + q) * d + c];
+    part[y][lane] = sum;
+    __syncthreads();
+    if (y == 0 && c < d) {
+        for (int i = 1; i < kJoinParts; i++) sum += part[i][lane];
+        float f[1] = {sum * scale};
+        store<T, 1>(dw + (size_t)id * d + c, f);
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------
+inline size_t up(size_t n, size_t to) { return (n + to - 1) / to * to; }
+constexpr int kTilePairs = 32;
+
+struct Layout {
+    size_t buf0, buf1, head, tail, bytes;
+    int tiles;
+};
+Layout layout(int64_t n, int d) {
+    Layout l;
+    l.tiles = (int)((n + kTilePairs - 1) / kTilePairs);
+    size_t o = 0;
+    auto take = [&](size_t b) { const size_t at = o; o += up(b, 256); return at; };
+    l.buf0 = take(8 * (size_t)n); l.buf1 = take(8 * (size_t)n);
+    l.head = take(4 * (size_t)l.tiles * d); l.tail = take(4 * (size_t)l.tiles * d);
+    l.bytes = o;
+    return l;
+}
+int check_sizes(int64_t n, int vocab, int d, int dtype) {
+    if (n < 1 || vocab < 1 || d < 1 || (dtype != CDSSM_BF16 && dtype != CDSSM_F32)) return CDSSM_ERR_BAD_ARG;
+    if (n > (1 << 28) || d > (1 << 16) || vocab > (1 << 26)) return CDSSM_ERR_UNSUPPORTED;
+    return CDSSM_OK;
+}
+
+template <typename T, int kE>
+int forward(const int64_t* ids, const void* w, int64_t w_stride, void* out, int64_t n, int vocab, int d, float scale, cudaStream_t st) {
+    const int64_t blocks = (n * (d / kE) + 255) / 256;
+    if (blocks > 0x7fffffff) return CDSSM_ERR_UNSUPPORTED;
+    embed_kernel<T, kE><<<(unsigned)blocks, 256, 0, st>>>(ids, static_cast<const T*>(w), w_stride, static_cast<T*>(out), n, vocab, d, scale);
+    return check_launch();
+}
+
+template <typename T, int kE>
+int sums(const uint2* pairs, int n, int vocab, const void* grad, void* dw, float* head, float* tail, int tiles, int d, float scale, cudaStream_t st) {
+    const int vecs = d / kE, threads = std::min(256, (vecs + 31) / 32 * 32);
+    sum_tiles_kernel<T, kE, kTilePairs><<<dim3(tiles, (vecs + threads - 1) / threads), threads, 0, st>>>(
+        pairs, n, vocab, static_cast<const T*>(grad), static_cast<T*>(dw), head, tail, d, scale);
+    if (int rc = check_launch()) return rc;
+    join_tiles_kernel<T, kTilePairs><<<dim3(tiles, (d + 31) / 32), 32 * kJoinParts, 0, st>>>(pairs, n, vocab, head, tail, static_cast<T*>(dw), d, scale);
+    return check_launch();
+}
+
+}  // namespace emb
+}  // namespace cdssm
+
+using namespace cdssm;
+
+extern "C" int cdssm_b200_embedding_fwd(const int64_t* ids, const void* w, int64_t w_row_stride, void* out, int64_t n, int vocab, int d, float scale,
+                                        int dtype, void* stream) {
+    if (!ids || !w || !out || w_row_stride < 0) return CDSSM_ERR_BAD_ARG;
+    if (int rc = emb::check_sizes(n, vocab, d, dtype)) return rc;
+    const cudaStream_t st = (cudaStream_t)stream;
+    const int e = dtype == CDSSM_BF16 ? 8 : 4;
+    const bool vec = d % e == 0 && w_row_stride % e == 0 && (((uintptr_t)w | (uintptr_t)out) & 15) == 0;
+    if (dtype == CDSSM_BF16)
+        return vec ? emb::forward<__nv_bfloat16, 8>(ids, w, w_row_stride, out, n, vocab, d, scale, st)
+                   : emb::forward<__nv_bfloat16, 1>(ids, w, w_row_stride, out, n, vocab, d, scale, st);
+    return vec ? emb::forward<float, 4>(ids, w, w_row_stride, out, n, vocab, d, scale, st)
+               : emb::forward<float, 1>(ids, w, w_row_stride, out, n, vocab, d, scale, st);
+}
+
+extern "C" size_t cdssm_b200_embedding_bwd_workspace_bytes(int64_t n, int vocab, int d, int dtype) {
+    return emb::check_sizes(n, vocab, d, dtype) == CDSSM_OK ? emb::layout(n, d).bytes : 0;
+}
+
+extern "C" int cdssm_b200_embedding_bwd(const int64_t* ids, const void* grad, void* grad_w, void* workspace, size_t workspace_bytes, int64_t n,
+                                        int vocab, int d, int64_t padding_idx, float scale, int dtype, void* stream) {
+    if (!ids || !grad || !grad_w || !workspace) return CDSSM_ERR_BAD_ARG;
+    if (int rc = emb::check_sizes(n, vocab, d, dtype)) return rc;
+    if (((uintptr_t)grad | (uintptr_t)grad_w) & 15) return CDSSM_ERR_BAD_ARG;
+    const emb::Layout l = emb::layout(n, d);
+    if (workspace_bytes < l.bytes || ((uintptr_t)workspace & 255)) return CDSSM_ERR_WORKSPACE;
+    const cudaStream_t st = (cudaStream_t)stream;
+    int sms = 0;
+    if (int rc = sm_count(sms)) return rc;
+    char* const ws = static_cast<char*>(workspace);
+    uint2 *const b0 = reinterpret_cast<uint2*>(ws + l.buf0), *const b1 = reinterpret_cast<uint2*>(ws + l.buf1);
+    int bits = 1;
+    while ((int64_t)1 << bits <= vocab) bits++;   // keys 0 .. vocab
+    const int passes = (bits + emb::kMostBits - 1) / emb::kMostBits, per_pass = (bits + passes - 1) / passes;
+    const size_t bytes = (size_t)vocab * d * (dtype == CDSSM_BF16 ? 2 : 4);
+    // one sub-tile of a block needs no cluster; eight blocks are the most that every launch may ask for
+    const int cluster = n > emb::kSortThreads * emb::kItems ? 8 : 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(cluster * std::max(2, sms / cluster)));
+    cfg.blockDim = dim3(emb::kSortThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (int rc = counted(check_cuda(cudaLaunchKernelEx(&cfg, emb::sort_and_clear_kernel, ids, (int)n, vocab, padding_idx, per_pass, passes, b0, b1,
+                                                       static_cast<uint4*>(grad_w), bytes / 16, static_cast<unsigned char*>(grad_w) + bytes / 16 * 16,
+                                                       (int)(bytes % 16)))))
+        return rc;
+    const uint2* const sorted = passes & 1 ? b0 : b1;
+    float *const head = reinterpret_cast<float*>(ws + l.head), *const tail = reinterpret_cast<float*>(ws + l.tail);
+    if (dtype == CDSSM_BF16)
+        return d % 8 == 0 ? emb::sums<__nv_bfloat16, 8>(sorted, (int)n, vocab, grad, grad_w, head, tail, l.tiles, d, scale, st)
+                          : emb::sums<__nv_bfloat16, 1>(sorted, (int)n, vocab, grad, grad_w, head, tail, l.tiles, d, scale, st);
+    return d % 4 == 0 ? emb::sums<float, 4>(sorted, (int)n, vocab, grad, grad_w, head, tail, l.tiles, d, scale, st)
+                      : emb::sums<float, 1>(sorted, (int)n, vocab, grad, grad_w, head, tail, l.tiles, d, scale, st);
+}

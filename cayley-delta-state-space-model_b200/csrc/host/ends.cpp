@@ -1,7 +1,10 @@
-// The ends of a training step: the loss of hidden rows against a vocabulary, forward and backward, one native call each.
+// The ends of a training step, one native call each: rows of a table for token ids, the loss of hidden rows against a vocabulary, both
+// with their gradients, and the norm and clipping of all gradients.
 #include "host.h"
 
+#include <algorithm>
 #include <cmath>
+#include <vector>
 
 namespace cdssm_host {
 namespace {
@@ -100,10 +103,155 @@ PyObject* py_linear_ce_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// embedding_fwd(ids (..) int64, weight (vocab, d), scale) -> out (.., d)
+PyObject* py_embedding_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&] {
+        Args in{a, n};
+        const Tensor ids_ = in.tensor("ids"), weight = in.tensor("weight");
+        const float scale = (float)in.number();
+        need_cuda(ids_, "ids");
+        need_cuda(weight, "weight");
+        need_same_device(ids_, weight, "ids");
+        if (ids_.scalar_type() != at::kLong) throw Error("ids must be int64");
+        need_dims(weight, 2, "weight");
+        const int64_t d = weight.size(1), vocab = weight.size(0), count = ids_.numel();
+        if (d < 1 || vocab < 1) throw Error("weight is empty");
+        const int dt = dtype_code(weight);
+        return wrap(without_gil([&] {
+            const c10::cuda::CUDAGuard guard(weight.device());
+            auto sizes = ids_.sizes().vec();
+            sizes.push_back(d);
+            const Tensor out = empty_like_dims(sizes, weight);
+            if (count == 0) return out;
+            if (d > INT32_MAX || vocab > INT32_MAX) check(CDSSM_ERR_UNSUPPORTED, "embedding_fwd");
+            const Tensor ids = ids_.contiguous(), w = ce_weight(weight);
+            check(cdssm_b200_embedding_fwd(ids.const_data_ptr<int64_t>(), cptr(w), row_stride(w), mptr(out), count, (int)vocab, (int)d, scale, dt,
+                                           stream_of(w)),
+                  "embedding_fwd");
+            return out;
+        }));
+    });
+}
+
+// embedding_bwd(grad (.., d), ids, vocab, padding_idx (-1: none), scale) -> grad_weight (vocab, d)
+PyObject* py_embedding_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&] {
+        Args in{a, n};
+        const Tensor grad_ = in.tensor("grad"), ids_ = in.tensor("ids");
+        const int64_t vocab = in.integer(), padding = in.integer();
+        const float scale = (float)in.number();
+        const int64_t d = grad_.size(-1), count = ids_.numel();
+        return wrap(without_gil([&] {
+            const c10::cuda::CUDAGuard guard(grad_.device());
+            if (count == 0) return at::zeros({vocab, d}, grad_.options());
+            const Tensor out = empty_like_dims({vocab, d}, grad_);
+            const int dt = dtype_code(grad_);
+            const size_t bytes = cdssm_b200_embedding_bwd_workspace_bytes(count, (int)vocab, (int)d, dt);
+            if (bytes == 0) check(CDSSM_ERR_UNSUPPORTED, "embedding_bwd");
+            Tensor grad = grad_.contiguous();
+            if (reinterpret_cast<uintptr_t>(grad.const_data_ptr()) & 15) grad = grad.clone();
+            const Tensor ids = ids_.contiguous(), ws = scratch(bytes, grad_);
+            check(cdssm_b200_embedding_bwd(ids.const_data_ptr<int64_t>(), cptr(grad), mptr(out), mptr(ws), bytes, count, (int)vocab, (int)d, padding,
+                                           scale, dt, stream_of(grad)),
+                  "embedding_bwd");
+            return out;
+        }));
+    });
+}
+
+// Tensors as the kernels walk them: every value once, in the order of memory.
+void need_dense(const Tensor& t, const char* name) {
+    need_cuda(t, name);
+    if (t.layout() != at::kStrided) throw Error(std::string(name) + ": a sparse tensor");
+    dtype_code(t);
+    if (!t.is_non_overlapping_and_dense()) throw Error(std::string(name) + ": a tensor with holes or overlaps in memory");
+}
+
+// No output may lie over another tensor of the call (its own input apart): blocks would read what others have written.
+void need_apart(const std::vector<Tensor>& ins, const std::vector<Tensor>& outs) {
+    struct Range {
+        uintptr_t at, end;
+        size_t i;
+        bool out;
+    };
+    std::vector<Range> r;
+    r.reserve(ins.size() + outs.size());
+    auto add = [&](const Tensor& t, size_t i, bool out) {
+        const uintptr_t p = reinterpret_cast<uintptr_t>(t.const_data_ptr());
+        if (t.numel()) r.push_back({p, p + t.numel() * t.element_size(), i, out});
+    };
+    for (size_t i = 0; i < outs.size(); i++) {
+        add(outs[i], i, true);
+        if (outs[i].const_data_ptr() != ins[i].const_data_ptr() || outs[i].scalar_type() != ins[i].scalar_type()) add(ins[i], i, false);
+    }
+    std::sort(r.begin(), r.end(), [](const Range& x, const Range& y) { return x.at < y.at; });
+    uintptr_t end = 0, end_out = 0;   // of all before, of the outputs before
+    for (const Range& x : r) {
+        if (x.at < (x.out ? end : end_out)) throw Error("clip_grads_: an output overlaps another tensor of the call");
+        end = std::max(end, x.end);
+        if (x.out) end_out = std::max(end_out, x.end);
+    }
+}
+
+// grad_clip(list of tensors, list of outputs or None, max_norm) -> norm; outputs may be the tensors themselves; None: the norm alone
+PyObject* py_grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&] {
+        Args in{a, n};
+        auto list = [&](PyObject* o, const char* name) {
+            std::vector<Tensor> v;
+            if (!PyList_Check(o)) throw Error(std::string(name) + " must be a list");
+            Args items{PySequence_Fast_ITEMS(o), PyList_GET_SIZE(o)};
+            for (Py_ssize_t i = 0; i < items.n; i++) v.push_back(items.tensor(name));
+            return v;
+        };
+        const std::vector<Tensor> ins = list(in.next(), "gradients");
+        PyObject* o = in.next();
+        const bool scale = o != Py_None;
+        const std::vector<Tensor> outs = scale ? (o == a[0] ? ins : list(o, "out")) : std::vector<Tensor>();
+        const float max_norm = (float)in.number();
+        if (ins.empty()) throw Error("no gradients");
+        if (scale && outs.size() != ins.size()) throw Error("out must have as many tensors as the gradients");
+        std::vector<const void*> pi;
+        std::vector<void*> po;
+        std::vector<int64_t> sizes;
+        std::vector<int> di, dout;
+        for (size_t i = 0; i < ins.size(); i++) {
+            need_dense(ins[i], "gradients");
+            need_same_device(ins[i], ins[0], "gradients");
+            pi.push_back(cptr(ins[i]));
+            sizes.push_back(ins[i].numel());
+            di.push_back(dtype_code(ins[i]));
+            if (!scale) continue;
+            need_dense(outs[i], "out");
+            need_same_device(outs[i], ins[0], "out");
+            if (outs[i].sizes() != ins[i].sizes() || outs[i].strides() != ins[i].strides()) throw Error("out must have the gradients' shapes and strides");
+            if (outs[i].scalar_type() != ins[i].scalar_type() && outs[i].scalar_type() != at::kFloat) throw Error("out must have the gradients' types or float32");
+            po.push_back(mptr(outs[i]));
+            dout.push_back(dtype_code(outs[i]));
+        }
+        if (scale) need_apart(ins, outs);
+        return wrap(without_gil([&] {
+            const c10::cuda::CUDAGuard guard(ins[0].device());
+            const Tensor norm = empty_f32({}, ins[0]);
+            const size_t bytes = cdssm_b200_grad_clip_workspace_bytes(sizes.data(), (int)sizes.size());
+            const Tensor ws = scratch(bytes, ins[0]);
+            check(cdssm_b200_grad_clip(pi.data(), scale ? po.data() : nullptr, sizes.data(), di.data(), dout.data(), (int)sizes.size(), max_norm,
+                                       fmut(norm), mptr(ws), bytes, stream_of(ins[0])),
+                  "grad_clip");
+            for (const Tensor& t : outs)
+                if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();   // written in place, as autograd counts it
+            return norm;
+        }));
+    });
+}
+
 #define FAST(fn) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fn)), METH_FASTCALL, nullptr
 PyMethodDef g_ends_methods[] = {
     {"linear_ce_fwd", FAST(py_linear_ce_fwd)},
     {"linear_ce_bwd", FAST(py_linear_ce_bwd)},
+    {"embedding_fwd", FAST(py_embedding_fwd)},
+    {"embedding_bwd", FAST(py_embedding_bwd)},
+    {"grad_clip", FAST(py_grad_clip)},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -22,7 +22,7 @@ from ._lib import CdssmError, check
 __all__ = ["CUDAConv1dSiLUOp", "DynamicsFusedFn", "NormalizeKQFn", "IntraChunkScanFn",
            "InterChunkScanFn", "ExactCorrectionFn", "scan_fused", "decode_step", "decode_step_reference", "reference_decode_state",
            "scan_fused_workspace_bytes", "scan_fused_status", "set_wait_limit_ns", "selftest_bounded_wait", "rms_norm", "groupnorm_gate", "conv1d_silu_step", "scan_summary", "scan_fused_long", "compose_carries",
-           "LinearCrossEntropyFn", "linear_cross_entropy",
+           "EmbeddingFn", "embedding", "LinearCrossEntropyFn", "linear_cross_entropy", "grad_norm", "clip_grads_", "clip_grad_norm_",
            "CdssmError"]
 
 _DT = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
@@ -173,6 +173,36 @@ class ExactCorrectionFn(Function):
 # ------------------------------------------------------------------------------------------
 # The ends of a training step
 # ------------------------------------------------------------------------------------------
+class EmbeddingFn(Function):
+    """Rows of a table for token ids, scaled: see :func:`embedding`."""
+
+    @staticmethod
+    def forward(ctx, ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: int = None) -> Tensor:
+        padding = -1 if padding_idx is None else int(padding_idx)
+        if padding_idx is not None and not 0 <= padding < weight.shape[0]:
+            raise CdssmError(f"padding_idx {padding_idx} is no row of the table")
+        ctx.args = (weight.shape[0], padding, float(scale))
+        out = _lib.host().embedding_fwd(ids, weight, scale)
+        ctx.save_for_backward(ids)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        """(None, grad_weight, None, None)"""
+        ids, = ctx.saved_tensors
+        return None, _lib.host().embedding_bwd(grad_out, ids, *ctx.args), None, None
+
+
+def embedding(ids: Tensor, weight: Tensor, *, scale: float = 1.0, padding_idx: int = None) -> Tensor:
+    """scale * weight[ids] (cdssm/models/model.py:46): ids (...) int64, weight (vocab, d) bfloat16 or float32 -> (..., d).
+
+    The gradient (vocab, d) is dense, in the weight's type; the rows of one id are added up in float32 in the order of the tokens and
+    rounded once, the same bits from run to run; ``padding_idx``'s row gets none.  An id that is no row of the table (negative ones too)
+    gives a row of NaN and takes no part in the gradient.  Differentiable once."""
+    return EmbeddingFn.apply(ids, weight, scale, padding_idx)
+
+
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
@@ -212,6 +242,31 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
     Products are bfloat16 ones with float32 sums, for float32 operands exact to 24 bits; the logits' gradient is rounded once to the
     products' type.  Gradients have the operands' type and are the same from run to run.  Differentiable once."""
     return LinearCrossEntropyFn.apply(hidden, weight, targets, ignore_index, reduction)
+
+
+def grad_norm(grads) -> Tensor:
+    """The 2-norm of all tensors together, one float32 value on their device; squares are summed in 64 bits in a fixed order.
+    bfloat16 and float32 CUDA tensors, dense in memory, at least one."""
+    return _lib.host().grad_clip(list(grads), None, 0.0)
+
+
+def clip_grads_(grads, max_norm: float, *, out=None) -> Tensor:
+    """Scales gradients by min(1, max_norm / (norm + 1e-6)), in place or into ``out`` (tensors of the same shapes and strides, of the
+    same types or float32, e.g. an optimizer's buffers), and returns the norm before.  Nothing waits for the GPU.  In place, gradients
+    within the bound are not written.  A norm that is NaN makes all of them NaN, an infinite one makes finite values zero."""
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise CdssmError(f"max_norm must be a number of at least 0, not {max_norm}")
+    grads = list(grads)
+    return _lib.host().grad_clip(grads, grads if out is None else list(out), max_norm)
+
+
+def clip_grad_norm_(parameters, max_norm: float) -> Tensor:
+    """:func:`clip_grads_` of the parameters' gradients, as a trainer calls it between backward and step
+    (cdssm/training/trainer.py:219-262); parameters without a gradient are passed over, without any the norm is 0."""
+    parameters = [parameters] if isinstance(parameters, Tensor) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    return clip_grads_(grads, max_norm) if grads else torch.zeros(())
 
 
 # ------------------------------------------------------------------------------------------

@@ -472,6 +472,30 @@ CDSSM_API int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, in
                                        size_t workspace_bytes, int64_t rows, int d, int vocab, int64_t ignore_index,
                                        int reduction, int dtype, int flags, void* stream);
 
+/* Rows of a table for token ids: out (n,d) = scale * w[ids], each value rounded once; w (vocab,d) with w_row_stride elements between
+ * rows.  An id that is no row of the table gives a row of NaN.  vocab <= 2^26, n <= 2^28, d <= 65536.
+ * Replaces the embedding, cdssm/models/model.py:46. */
+CDSSM_API int cdssm_b200_embedding_fwd(const int64_t* ids, const void* w, int64_t w_row_stride, void* out, int64_t n, int vocab,
+                                       int d, float scale, int dtype, void* stream);
+/* Its backward: grad_w (vocab,d) = scale * the sum of grad (n,d) over the tokens of each id, in their order, in float32 and rounded
+ * once; ids that are no row of the table and padding_idx (-1: none) take no part.  grad and grad_w 16-byte aligned, dense; the
+ * workspace of cdssm_b200_embedding_bwd_workspace_bytes 256-byte aligned. */
+CDSSM_API size_t cdssm_b200_embedding_bwd_workspace_bytes(int64_t n, int vocab, int d, int dtype);
+CDSSM_API int cdssm_b200_embedding_bwd(const int64_t* ids, const void* grad, void* grad_w, void* workspace,
+                                       size_t workspace_bytes, int64_t n, int vocab, int d, int64_t padding_idx, float scale,
+                                       int dtype, void* stream);
+
+/* The 2-norm of n tensors together and, where out is not NULL, their values times min(1, max_norm / (norm + 1e-6)).
+ * in, out, sizes (values) and the types (CDSSM_BF16 or CDSSM_F32) are HOST arrays of n; out[i] may be in[i], or another buffer of
+ * the same type or of float32, and no out may overlap another tensor of the call.  norm: one float32 in device memory.  Squares are
+ * summed in float64 in a fixed order.  Where the factor is 1 tensors in place are not written.  A norm that is no number makes every
+ * output NaN, an infinite one zeros of what is finite.  workspace: cdssm_b200_grad_clip_workspace_bytes, 256-byte aligned.
+ * Replaces clip_grad_norm_ of a training step, cdssm/training/trainer.py:219-262. */
+CDSSM_API size_t cdssm_b200_grad_clip_workspace_bytes(const int64_t* sizes, int n);
+CDSSM_API int cdssm_b200_grad_clip(const void* const* in, void* const* out, const int64_t* sizes, const int* in_dtypes,
+                                   const int* out_dtypes, int n, float max_norm, float* norm, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
