@@ -8,9 +8,13 @@
 // joined by a small kernel.  Backward, a piece of the vocabulary at a time: z of the piece anew, dz of it rounded to the products'
 // type into scratch, then both products that read it in one launch.  Rows without a target are left out before the first product.
 //
+// Where all rows have one upstream gradient (mean, sum) it is a factor of dx and dW, not of dz: dz holds p - [v = y] then, and a factor's
+// own rounding to bf16 does not shift all of a gradient the same way.
+//
 // All products are tcgen05 ones of TMA tiles: 128 x 256 outputs a block, fp32 accumulators, two of them in tensor memory so that the
 // epilogue of a tile runs beside the products of the next.  float32 operands enter as three bf16 parts (exact to 24 bits) and six of
-// the nine part products, the small ones first.
+// the nine part products, the small ones first.  The tensor cores' float32 sums are cut off, not rounded, so that the error of a long sum
+// grows with its length: sums that must be good to float32 are folded into registers every so many steps (fold_blocks()).
 #include "cdssm_common.cuh"
 #include "sm100_ptx.cuh"
 #include "tile_map.cuh"
@@ -32,6 +36,10 @@ constexpr int kTmemCols = 2 * kN;
 
 enum Mode { kStats, kGradLogits, kGradProducts };
 
+// Depth blocks after which a sum is folded.  Loss, width 768 / 2048 in one piece: off by 7.5e-7 / 1.4e-6 of itself (float32 sums in
+// registers 2.9e-7).  Sums of bf16 gradients run on: they are rounded to 2^-8 in the end.
+constexpr int kFoldLogits = 12, kFold3 = 4;
+
 // Part products of float32 operands in the order in which they are added up: the small ones first, so that they are not lost beside
 // the large one's rounding.  (2,1), (1,2), (2,2) are below 2^-24 of the whole.
 constexpr int kTerms3 = 6;
@@ -52,7 +60,7 @@ struct Args {
     float2* part;                // (runs x 2, Tp) maximum and sum of a run of tiles
     const float* grad;           // upstream gradient: one value, or one a row of the caller
     int grad_rows, mean;
-    int planes, terms;
+    int planes, terms, fold;
     int Tp, d, V;
     int run, n_tiles, n_runs;    // forward: tiles of a run, tiles and runs of a row
     int v0, vn, vn_tiles;        // backward: first word and words of the piece
@@ -82,7 +90,7 @@ __device__ __forceinline__ float ex2(float x) {
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- the blocks' shares of the work ---------------------------------------------------------
-// A segment: depth blocks [k0, k1) of one tile.
+// A segment: depth blocks [k0, k1) of one tile.  `fold` of the depth's blocks at a time go through all part products.
 struct Segment {
     int dw;          // kGradProducts: 0 a tile of dx, 1 of dW
     int m, n;        // row and column tile
@@ -199,6 +207,17 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, const void* s
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
+// Where block k of a tile's kt stands: its place in the depth, its part product, and whether the fold ends with it.
+struct Place {
+    int kc, term;
+    bool ends;
+};
+__device__ __forceinline__ Place place(const Args& a, int k, int kt) {
+    if (a.terms == 1) return {k, 0, (k + 1) % a.fold == 0};
+    const int depth = kt / a.terms, per = a.fold * a.terms, c = k / per, r = k - c * per, n = min(a.fold, depth - c * a.fold), t = r / n;
+    return {c * a.fold + r - t * n, t, r + 1 == n * a.terms};
+}
+
 struct Maps {   // kStats, kGradLogits: a x, b W, out dz; kGradProducts: (a dz, b W) for dx, (a2 dz, b2 x) for dW
     CUtensorMap a, b, a2, b2;
 };
@@ -211,15 +230,15 @@ __device__ __forceinline__ bool produce(Smem& sm, const Maps& maps, const Args& 
     Segment s;
     uint32_t it = 0;
     while (walk.next(s)) {
-        const int depth = s.kt / a.terms;
 #pragma unroll 1
         for (int k = s.k0; k < s.k1; k++, it++) {
             const int st = it % kStages;
             if (!mbar_wait_suspend(&sm.empty[st], (it / kStages & 1) ^ 1, ab, a.wait_ns)) return false;
             mbar_arrive_expect_tx(&sm.full[st], (kM + kN) * kK * 2);
+            const Place at = place(a, k, s.kt);
             int pa, pb;
-            term_planes(a.planes, k / depth, pa, pb);
-            const int kc = (k % depth) * kK;
+            term_planes(a.planes, at.term, pa, pb);
+            const int kc = at.kc * kK;
             if (kMode != kGradProducts) {
                 tma_load_3d(sm.a[st], &maps.a, &sm.full[st], kc, s.m * kM, pa);
                 tma_load_3d(sm.b[st], &maps.b, &sm.full[st], kc, a.v0 + s.n * kN, pb);
@@ -250,28 +269,30 @@ __device__ __forceinline__ bool multiply(Smem& sm, const Args& a, int count) {
     uint32_t it = 0, tile = 0;
     const uint32_t tm = sm.tmem_base;
     while (walk.next(s)) {
-        const int acc = tile & 1;
-        if (!mbar_wait_suspend(&sm.acc_empty[acc], (tile >> 1 & 1) ^ 1, ab, a.wait_ns)) return false;
-        tc_fence_after();
         // (a K-major row of a tile is 128 bytes: 16 columns are 32 bytes on; an MN-major one holds 64 rows of the operand: 16 of the
         // depth are 16 rows of 128 bytes on, the next 64 rows of the operand 8192 bytes)
         const bool a_mn = kMode == kGradProducts && s.dw, b_mn = kMode == kGradProducts;
         const uint32_t idesc = umma_idesc_bf16(kM, kN, false, false) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
         const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;
         const uint32_t a_lbo = a_mn ? 8192 : 16, b_lbo = b_mn ? 8192 : 16;
+        bool begins = true;
 #pragma unroll 1
         for (int k = s.k0; k < s.k1; k++, it++) {
-            const int st = it % kStages;
+            const int st = it % kStages, acc = tile & 1;
+            if (begins && !mbar_wait_suspend(&sm.acc_empty[acc], (tile >> 1 & 1) ^ 1, ab, a.wait_ns)) return false;
             if (!mbar_wait_suspend(&sm.full[st], it / kStages & 1, ab, a.wait_ns)) return false;
             tc_fence_after();
             const uint32_t da = desc_lo_sw128(smem_u32(sm.a[st]), a_lbo), db = desc_lo_sw128(smem_u32(sm.b[st]), b_lbo);
 #pragma unroll
             for (int j = 0; j < kK / 16; j++)
-                umma_bf16_elect(tm + acc * kN, da + j * a_step, db + j * b_step, idesc, k > s.k0 || j > 0);
+                umma_bf16_elect(tm + acc * kN, da + j * a_step, db + j * b_step, idesc, !begins || j > 0);
             umma_commit_elect(&sm.empty[st]);
+            begins = k + 1 == s.k1 || place(a, k, s.kt).ends;
+            if (begins) {
+                umma_commit_elect(&sm.acc_full[acc]);
+                tile++;
+            }
         }
-        umma_commit_elect(&sm.acc_full[acc]);
-        tile++;
     }
     return true;
 }
@@ -308,11 +329,18 @@ __device__ __forceinline__ void store_row(T* row, int col, int cols, const float
     }
 }
 
+// What all of dz has been left without.
+__device__ __forceinline__ float gradient_factor(const Args& a, int count) {
+    return a.grad_rows ? 1.f : a.mean ? a.grad[0] / (float)count : a.grad[0];
+}
+
 // 32 columns of a row of a finished tile of dx or dW.  dx of several pieces is summed in float32 and rounded once, by the last.
-__device__ __forceinline__ void emit(const Args& a, int count, int dw, int row, int col, float (&v)[32]) {
+__device__ __forceinline__ void emit(const Args& a, int count, float factor, int dw, int row, int col, float (&v)[32]) {
     if (col >= a.d) return;
     if (dw) {
         if (row >= a.vn) return;
+#pragma unroll
+        for (int j = 0; j < 32; j++) v[j] *= factor;
         const size_t at = (size_t)(a.v0 + row) * a.d;
         if (a.f32) store_row(static_cast<float*>(a.dw) + at, col, a.d, v, a.vec_dw);
         else store_row(static_cast<__nv_bfloat16*>(a.dw) + at, col, a.d, v, a.vec_dw);
@@ -332,6 +360,8 @@ __device__ __forceinline__ void emit(const Args& a, int count, int dw, int row, 
         for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(acc + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
         return;
     }
+#pragma unroll
+    for (int j = 0; j < 32; j++) v[j] *= factor;
     const size_t at = (size_t)a.rows[row] * a.d;
     if (a.f32) store_row(static_cast<float*>(a.dx) + at, col, a.d, v, a.vec_dx);
     else store_row(static_cast<__nv_bfloat16*>(a.dx) + at, col, a.d, v, a.vec_dx);
@@ -343,7 +373,8 @@ __device__ __forceinline__ size_t slot_at(int slot, int warp, int chunk, int j4,
     return (size_t)slot * kSlotFloat4 + ((warp * 4 + chunk) * 8 + j4) * 32 + lane;
 }
 
-template <int kMode>
+// kFold: the tile's sums come in folds and are added up here, in 128 registers a thread; else they are read from tensor memory as used.
+template <int kMode, bool kFold>
 __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, const Args& a, int count) {
     volatile int* ab = &sm.abort_flag;
     auto walk = make_walk<kMode>(a, count);
@@ -354,9 +385,10 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
     float top = -INFINITY, sum = 0.f;
     int run_rows = -1, target = -1;                      // of the present row tile
     float mx = 0.f, inv = 0.f, g = 0.f;
+    const float factor = kMode == kGradProducts ? gradient_factor(a, count) : 0.f;
     uint32_t tile = 0;
     while (walk.next(s)) {
-        const int acc = tile & 1, row = s.m * kM + lrow;
+        const int row = s.m * kM + lrow;
         if (kMode != kGradProducts && run_rows != s.m) {
             run_rows = s.m;
             target = a.target[row];
@@ -364,22 +396,49 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
                 mx = a.row_max[row];
                 inv = a.row_inv[row];
                 g = 0.f;
-                if (row < count) {
-                    g = a.grad_rows ? a.grad[a.rows[row]] : a.grad[0];
-                    if (a.mean) g /= (float)count;
-                    if (target == -2) g = NAN;           // (a target that is no word)
-                }
+                if (row < count) g = target == -2 ? NAN : a.grad_rows ? a.grad[a.rows[row]] : 1.f;   // (-2: a target that is no word)
             }
         }
-        if (!mbar_wait_suspend(&sm.acc_full[acc], tile >> 1 & 1, ab, a.wait_ns)) return false;
-        tc_fence_after();
-        if (kMode == kStats) {
+        float folded[kFold ? 128 : 1] = {};
+        int acc = tile & 1;
+        if constexpr (kFold) {
 #pragma unroll 1
+            for (int k = s.k0; k < s.k1; k++) {
+                if (!(k + 1 == s.k1 || place(a, k, s.kt).ends)) continue;
+                acc = tile & 1;
+                if (!mbar_wait_suspend(&sm.acc_full[acc], tile >> 1 & 1, ab, a.wait_ns)) return false;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    float z[32];
+                    tmem_ld32(tm + acc * kN + c * 32, z);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) folded[c * 32 + j] += z[j];
+                }
+                tc_fence_before();
+                mbar_arrive(&sm.acc_empty[acc]);
+                tile++;
+            }
+        } else {
+            if (!mbar_wait_suspend(&sm.acc_full[acc], tile >> 1 & 1, ab, a.wait_ns)) return false;
+            tc_fence_after();
+        }
+        auto columns = [&](int c, float* z) {            // 32 of them
+            if constexpr (kFold) {
+#pragma unroll
+                for (int j = 0; j < 32; j++) z[j] = folded[c * 32 + j];
+            } else {
+                tmem_ld32(tm + acc * kN + c * 32, z);
+            }
+        };
+        constexpr int kUnroll = kFold ? 4 : 1;
+        if (kMode == kStats) {
+#pragma unroll kUnroll
             for (int c = 0; c < 4; c++) {
                 const int v0 = s.n * kN + half * 128 + c * 32;
                 if (v0 >= a.V) break;
                 float z[32];
-                tmem_ld32(tm + acc * kN + c * 32, z);
+                columns(c, z);
                 if (v0 + 32 > a.V) {
 #pragma unroll
                     for (int j = 0; j < 32; j++)
@@ -405,14 +464,19 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
             }
         } else if (kMode == kGradLogits) {
             const float scale = g * inv;
-#pragma unroll 1
+#pragma unroll kUnroll
             for (int c = 0; c < 2; c++) {
                 const int col = s.n * kN + half * 128 + c * 64, v0 = a.v0 + col;
                 float z[64];
-                tmem_ld32x2(tm + acc * kN + c * 64, z, tm + acc * kN + c * 64 + 32, z + 32);
+                if constexpr (kFold) {
+                    columns(2 * c, z);
+                    columns(2 * c + 1, z + 32);
+                } else {
+                    tmem_ld32x2(tm + acc * kN + c * 64, z, tm + acc * kN + c * 64 + 32, z + 32);
+                }
 #pragma unroll
                 for (int j = 0; j < 64; j++) z[j] = ex2((z[j] - mx) * kLog2e) * scale;
-                // (in the last step of the target's entry 1 - p is taken from p in float32: nothing is lost where p is near one)
+                // (1 is taken from the target's p in float32: nothing is lost where p is near one)
                 const unsigned rel = (unsigned)(target - v0);
                 if (__any_sync(~0u, rel < 64u)) {
 #pragma unroll
@@ -425,6 +489,7 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
                 }
                 const bool live = row < count;
                 uint8_t* const mine = sm.out[warp];
+#pragma unroll 1
                 for (int p = 0; p < a.planes; p++) {
                     if (lane == 0) tma_store_wait_read();
                     __syncwarp();
@@ -451,12 +516,12 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
         } else {
             const bool whole = s.k0 == 0 && s.k1 == s.kt;
             const int slot = 2 * blockIdx.x + (s.k0 == 0 ? 1 : 0);
-#pragma unroll 1
+#pragma unroll kUnroll
             for (int c = 0; c < 4; c++) {
                 float v[32];
-                tmem_ld32(tm + acc * kN + c * 32, v);
+                columns(c, v);
                 if (whole) {
-                    emit(a, count, s.dw, row, s.n * kN + half * 128 + c * 32, v);
+                    emit(a, count, factor, s.dw, row, s.n * kN + half * 128 + c * 32, v);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; j++)
@@ -464,9 +529,11 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
                 }
             }
         }
-        tc_fence_before();
-        mbar_arrive(&sm.acc_empty[acc]);
-        tile++;
+        if constexpr (!kFold) {
+            tc_fence_before();
+            mbar_arrive(&sm.acc_empty[acc]);
+            tile++;
+        }
         if (kMode == kStats && s.last) {
             a.part[(size_t)(2 * s.run + half) * a.Tp + row] = make_float2(top, sum);
             top = -INFINITY;
@@ -477,7 +544,7 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
     return true;
 }
 
-template <int kMode>
+template <int kMode, bool kFold>
 __global__ void __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtensorMap map_out, const Args a) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -500,12 +567,17 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
     tc_fence_after();
     const int count = *a.count;
     bool ok = true;
-    if (warp == 0) {
-        if ((threadIdx.x & 31) == 0 && !a.withhold) ok = produce<kMode>(sm, maps, a, count);
-    } else if (warp == 1) {
-        ok = multiply<kMode>(sm, a, count);
-    } else if (warp >= 4) {
-        ok = finish<kMode>(sm, &map_out, a, count);
+    // (a warpgroup's registers: 128 x 40 + 256 x 232 are the 384 x 168 of the launch)
+    if (warp < 4) {
+        if constexpr (kFold) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 0) {
+            if ((threadIdx.x & 31) == 0 && !a.withhold) ok = produce<kMode>(sm, maps, a, count);
+        } else if (warp == 1) {
+            ok = multiply<kMode>(sm, a, count);
+        }
+    } else {
+        if constexpr (kFold) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        ok = finish<kMode, kFold>(sm, &map_out, a, count);
     }
     if (!ok) atomicCAS(a.status, 0, 400 + warp);
     __syncwarp();
@@ -550,7 +622,7 @@ __global__ void __launch_bounds__(256) join_split_kernel(const Args a, int grid)
         }
         any = true;
     }
-    emit(a, count, dw, tile / t.d_tiles * kM + (warp & 3) * 32 + lane, tile % t.d_tiles * kN + (warp >> 2) * 128 + chunk * 32, v);
+    emit(a, count, gradient_factor(a, count), dw, tile / t.d_tiles * kM + (warp & 3) * 32 + lane, tile % t.d_tiles * kN + (warp >> 2) * 128 + chunk * 32, v);
 }
 
 // ---- rows in, losses out -------------------------------------------------------------------------
@@ -782,12 +854,19 @@ bool make_map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int 
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int kMode> struct Tag {};
-template <int kMode>
-int launch_products(const Maps& maps, const CUtensorMap& out, const Args& a, int grid, cudaStream_t st) {
-    if (int rc = allow_smem<Tag<kMode>>((const void*)product_kernel<kMode>, sizeof(Smem))) return rc;
-    product_kernel<kMode><<<grid, kThreads, sizeof(Smem), st>>>(maps, out, a);
+template <int kMode, bool kFold> struct Tag {};
+template <int kMode, bool kFold>
+int launch_as(const Maps& maps, const CUtensorMap& out, const Args& a, int grid, cudaStream_t st) {
+    if (int rc = allow_smem<Tag<kMode, kFold>>((const void*)product_kernel<kMode, kFold>, sizeof(Smem))) return rc;
+    product_kernel<kMode, kFold><<<grid, kThreads, sizeof(Smem), st>>>(maps, out, a);
     return check_launch();
+}
+constexpr int kNoFold = 1 << 30;
+template <int kMode>
+int launch_products(const Maps& maps, const CUtensorMap& out, Args a, int grid, cudaStream_t st) {
+    a.fold = a.planes == 3 ? kFold3 : kMode == kGradProducts ? kNoFold : kFoldLogits;
+    const bool one = kMode == kGradProducts ? a.fold == kNoFold : a.fold * kK >= a.d;
+    return one ? launch_as<kMode, false>(maps, out, a, grid, st) : launch_as<kMode, true>(maps, out, a, grid, st);
 }
 
 bool in_place(const void* w, int64_t stride, int dtype) {   // a matrix that TMA reads as it lies
