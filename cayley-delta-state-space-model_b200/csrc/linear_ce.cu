@@ -11,10 +11,10 @@
 // Where all rows have one upstream gradient (mean, sum) it is a factor of dx and dW, not of dz: dz holds p - [v = y] then, and a factor's
 // own rounding to bf16 does not shift all of a gradient the same way.
 //
-// All products are tcgen05 ones of TMA tiles: 128 x 256 outputs a block, fp32 accumulators, two of them in tensor memory so that the
-// epilogue of a tile runs beside the products of the next.  float32 operands enter as three bf16 parts (exact to 24 bits) and six of
+// All products are tcgen05 ones of TMA tiles by pairs of blocks: 256 x 256 outputs, each block loads half of both operands and keeps 128
+// rows of the result, fp32 accumulators, two of them in tensor memory so that the epilogue of a tile runs beside the products of the next.  float32 operands enter as three bf16 parts (exact to 24 bits) and six of
 // the nine part products, the small ones first.  The tensor cores' float32 sums are cut off, not rounded, so that the error of a long sum
-// grows with its length: sums that must be good to float32 are folded into registers every so many steps (fold_blocks()).
+// grows with its length: sums that must be good to float32 are folded into registers every so many steps (kFoldLogits, kFold3).
 #include "cdssm_common.cuh"
 #include "sm100_ptx.cuh"
 #include "tile_map.cuh"
@@ -28,10 +28,10 @@ namespace ce {
 
 using namespace sm100;
 
-constexpr int kM = 128, kN = 256, kK = 64;              // rows and columns of a block's tile, depth of a stage
-constexpr int kStages = 4;
+constexpr int kM = 256, kN = 256, kK = 64;              // rows and columns of a pair's tile, depth of a stage
+constexpr int kHalf = 128;                              // of either, a block's
+constexpr int kStages = 6;
 constexpr int kEpilogueWarps = 8, kThreads = 128 + 32 * kEpilogueWarps;
-constexpr int kRowTile = 256;                           // packed rows come in multiples of this
 constexpr int kTmemCols = 2 * kN;
 
 enum Mode { kStats, kGradLogits, kGradProducts };
@@ -40,18 +40,12 @@ enum Mode { kStats, kGradLogits, kGradProducts };
 // registers 2.9e-7).  Sums of bf16 gradients run on: they are rounded to 2^-8 in the end.
 constexpr int kFoldLogits = 12, kFold3 = 4;
 
-// Part products of float32 operands in the order in which they are added up: the small ones first, so that they are not lost beside
-// the large one's rounding.  (2,1), (1,2), (2,2) are below 2^-24 of the whole.
+// Part products in the order in which they are added up: the small ones first, so that they are not lost beside the large one's rounding.
+// float32 operands: (2,1), (1,2), (2,2) are below 2^-24 of the whole.  dz of a few rows of bf16 (kFewRows): its two parts.
 constexpr int kTerms3 = 6;
-__device__ __forceinline__ void term_planes(int planes, int term, int& pa, int& pb) {
-    if (planes == 1) { pa = pb = 0; return; }
-    constexpr uint32_t a = 2u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 0u << 10, b = 0u | 2u << 2 | 1u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
-    pa = (a >> (2 * term)) & 3;
-    pb = (b >> (2 * term)) & 3;
-}
 
 struct Args {
-    // what the forward leaves for the backward; Tp: rows padded to kRowTile
+    // what the forward leaves for the backward; Tp: rows padded to kM
     const int* count;            // rows that have a target
     const int* rows;             // (Tp) compact row -> row of the caller, -1 behind the last
     const int* target;           // (Tp) its word, -2: outside of the vocabulary
@@ -60,7 +54,8 @@ struct Args {
     float2* part;                // (runs x 2, Tp) maximum and sum of a run of tiles
     const float* grad;           // upstream gradient: one value, or one a row of the caller
     int grad_rows, mean;
-    int planes, terms, fold;
+    int planes, dz_planes;
+    int terms, group, folds;     // part products; depth blocks that go through all of them together; whether a group's sum is folded
     int Tp, d, V;
     int run, n_tiles, n_runs;    // forward: tiles of a run, tiles and runs of a row
     int v0, vn, vn_tiles;        // backward: first word and words of the piece
@@ -74,13 +69,20 @@ struct Args {
 };
 
 struct __align__(1024) Smem {
-    uint8_t a[kStages][kM * kK * 2];
-    uint8_t b[kStages][kN * kK * 2];
+    uint8_t a[kStages][kHalf * kK * 2];
+    uint8_t b[kStages][kHalf * kK * 2];
     uint8_t out[kEpilogueWarps][4096];
+    // full and acc_empty: of both blocks, the first one's; empty and acc_full: arrived at in both by the first one's products
     uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
     uint32_t tmem_base;
     int abort_flag;
 };
+
+__device__ __forceinline__ void term_planes(const Args& a, bool of_dz, int term, int& pa, int& pb) {
+    constexpr uint32_t ta = 2u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 0u << 10, tb = 0u | 2u << 2 | 1u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
+    pa = a.planes == 3 ? (ta >> (2 * term)) & 3 : of_dz ? a.dz_planes - 1 - term : 0;
+    pb = a.planes == 3 ? (tb >> (2 * term)) & 3 : 0;
+}
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -90,7 +92,7 @@ __device__ __forceinline__ float ex2(float x) {
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- the blocks' shares of the work ---------------------------------------------------------
-// A segment: depth blocks [k0, k1) of one tile.  `fold` of the depth's blocks at a time go through all part products.
+// A segment: depth blocks [k0, k1) of one tile.
 struct Segment {
     int dw;          // kGradProducts: 0 a tile of dx, 1 of dW
     int m, n;        // row and column tile
@@ -99,22 +101,25 @@ struct Segment {
     int run;
 };
 
-__device__ __forceinline__ int row_tiles(int count) { return max(1, (count + kRowTile - 1) / kRowTile) * (kRowTile / kM); }
+__device__ __forceinline__ int row_tiles(int count) { return max(1, (count + kM - 1) / kM); }
 
-// Forward and dz: a run of vocabulary tiles of one row tile is a block's unit.  Row tiles change fastest, so the blocks that run
+// Forward and dz: a run of vocabulary tiles of one row tile is a pair's unit.  Row tiles change fastest, so the pairs that run
 // beside each other read the same rows of W and every row of W leaves DRAM about once.
+__device__ __forceinline__ int pair_id() { return blockIdx.x >> 1; }
+__device__ __forceinline__ int pairs() { return gridDim.x >> 1; }
+
 struct RunWalk {
     int unit, units, mt, run_len, n_tiles, kt, n, n_end, m, run;
     __device__ RunWalk(const Args& a, int count, int n_tiles_, int run_len_) : run_len(run_len_), n_tiles(n_tiles_) {
         mt = row_tiles(count);
         units = mt * ((n_tiles + run_len - 1) / run_len);
         kt = (a.d + kK - 1) / kK * a.terms;
-        unit = (int)blockIdx.x - (int)gridDim.x;
+        unit = (int)pair_id() - (int)pairs();
         n = n_end = 0;
     }
     __device__ bool next(Segment& s) {
         if (n >= n_end) {
-            unit += gridDim.x;
+            unit += pairs();
             if (unit >= units) return false;
             run = unit / mt;
             m = unit - run * mt;
@@ -127,8 +132,8 @@ struct RunWalk {
     }
 };
 
-// dx and dW: as many whole tiles as fill the grid evenly, column tiles fastest (the blocks beside each other read the same rows of
-// dz); the depth blocks of the tiles that are left, dx before dW, are cut into as many equal shares as there are blocks.
+// dx and dW: as many whole tiles as fill the grid evenly, column tiles fastest (the pairs beside each other read the same rows of
+// dz); the depth blocks of the tiles that are left, dx before dW, are cut into as many equal shares as there are pairs.
 struct SplitTiles {
     int nx, nw, fx, fw, kx, kw, G, d_tiles;
     long long rest;
@@ -139,7 +144,7 @@ struct SplitTiles {
         fw = nw / G * G;
         rest = (long long)(nx - fx) * kx + (long long)(nw - fw) * kw;
     }
-    __device__ long long begin(int block) const { return rest * block / G; }
+    __device__ long long begin(int pair) const { return rest * pair / G; }
     // the tile that depth block i of the rest belongs to, and where it begins
     __device__ void at(long long i, int& dw, int& tile, long long& start) const {
         const long long x = (long long)(nx - fx) * kx;
@@ -157,10 +162,10 @@ struct SplitWalk {
     SplitTiles t;
     int phase = 0, i;
     long long at, end;
-    __device__ SplitWalk(const Args& a, int count) : t(split_tiles(a, count, gridDim.x)) {
-        i = blockIdx.x;
-        at = t.begin(blockIdx.x);
-        end = t.begin(blockIdx.x + 1);
+    __device__ SplitWalk(const Args& a, int count) : t(split_tiles(a, count, pairs())) {
+        i = pair_id();
+        at = t.begin(i);
+        end = t.begin(i + 1);
     }
     __device__ bool next(Segment& s) {
         while (phase < 2) {
@@ -171,7 +176,7 @@ struct SplitWalk {
                 return true;
             }
             phase++;
-            i = blockIdx.x;
+            i = pair_id();
         }
         if (at >= end) return false;
         int dw, tile;
@@ -192,10 +197,59 @@ __device__ __forceinline__ typename WalkOf<kMode>::type make_walk(const Args& a,
     else return RunWalk(a, count, kMode == kStats ? a.n_tiles : a.vn_tiles, a.run);
 }
 
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2) {
+// ---- pairs of blocks ---------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t block_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The first block's copy of a barrier, as both blocks address it.
+__device__ __forceinline__ uint32_t in_first(const void* bar) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
+    return r;
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t* dst) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(kTmemCols) : "memory");
+}
+// D (+)= A B over both blocks' shared memory (the same offsets in both) and tensor memory.
+__device__ __forceinline__ void pair_umma_elect(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 ad, bd;\n\t"
+        "mov.b64 ad, {%1, %5};\n\t"
+        "mov.b64 bd, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], ad, bd, %3, p;\n\t}" ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc),
+        "r"(kDescHiSw128)
+        : "memory");
+}
+// Both blocks' copies of the barrier are arrived at when the products issued so far are done.
+__device__ __forceinline__ void pair_commit_elect(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(smem_u32(bar)),
+        "h"((unsigned short)3)
+        : "memory");
+}
+
+// A tile into this block's shared memory; its bytes are counted at the first block's barrier.
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
         : "memory");
 }
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, const void* src, int c0, int c1, int c2) {
@@ -207,60 +261,65 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, const void* s
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
-// Where block k of a tile's kt stands: its place in the depth, its part product, and whether the fold ends with it.
+// Where block k of a tile's kt stands: its place in the depth, its part product, and whether a fold ends with it.
 struct Place {
     int kc, term;
     bool ends;
 };
 __device__ __forceinline__ Place place(const Args& a, int k, int kt) {
-    if (a.terms == 1) return {k, 0, (k + 1) % a.fold == 0};
-    const int depth = kt / a.terms, per = a.fold * a.terms, c = k / per, r = k - c * per, n = min(a.fold, depth - c * a.fold), t = r / n;
-    return {c * a.fold + r - t * n, t, r + 1 == n * a.terms};
+    if (a.terms == 1) return {k, 0, a.folds && (k + 1) % a.group == 0};
+    const int depth = kt / a.terms, per = a.group * a.terms, c = k / per, r = k - c * per, n = min(a.group, depth - c * a.group), t = r / n;
+    return {c * a.group + r - t * n, t, a.folds && r + 1 == n * a.terms};
 }
 
 struct Maps {   // kStats, kGradLogits: a x, b W, out dz; kGradProducts: (a dz, b W) for dx, (a2 dz, b2 x) for dW
     CUtensorMap a, b, a2, b2;
 };
 
-// ---- producer: one thread ------------------------------------------------------------------
+// ---- producer: one thread of either block ------------------------------------------------------
 template <int kMode>
 __device__ __forceinline__ bool produce(Smem& sm, const Maps& maps, const Args& a, int count) {
     volatile int* ab = &sm.abort_flag;
     auto walk = make_walk<kMode>(a, count);
     Segment s;
     uint32_t it = 0;
+    const int rank = block_rank(), am = rank * kHalf, bn = rank * kHalf;
+    const uint32_t full0 = in_first(&sm.full[0]);
     while (walk.next(s)) {
 #pragma unroll 1
         for (int k = s.k0; k < s.k1; k++, it++) {
             const int st = it % kStages;
             if (!mbar_wait_suspend(&sm.empty[st], (it / kStages & 1) ^ 1, ab, a.wait_ns)) return false;
-            mbar_arrive_expect_tx(&sm.full[st], (kM + kN) * kK * 2);
+            if (rank == 0) mbar_arrive_expect_tx(&sm.full[st], 2 * 2 * kHalf * kK * 2);
+            const uint32_t full = full0 + st * 8;
             const Place at = place(a, k, s.kt);
             int pa, pb;
-            term_planes(a.planes, at.term, pa, pb);
+            term_planes(a, kMode == kGradProducts, at.term, pa, pb);
             const int kc = at.kc * kK;
             if (kMode != kGradProducts) {
-                tma_load_3d(sm.a[st], &maps.a, &sm.full[st], kc, s.m * kM, pa);
-                tma_load_3d(sm.b[st], &maps.b, &sm.full[st], kc, a.v0 + s.n * kN, pb);
+                tma_load_3d(sm.a[st], &maps.a, full, kc, s.m * kM + am, pa);
+                tma_load_3d(sm.b[st], &maps.b, full, kc, a.v0 + s.n * kN + bn, pb);
             } else if (!s.dw) {
-                tma_load_3d(sm.a[st], &maps.a, &sm.full[st], kc, s.m * kM, pa);
+                tma_load_3d(sm.a[st], &maps.a, full, kc, s.m * kM + am, pa);
 #pragma unroll
-                for (int j = 0; j < kN / 64; j++)
-                    tma_load_3d(sm.b[st] + j * 64 * kK * 2, &maps.b, &sm.full[st], s.n * kN + j * 64, a.v0 + kc, pb);
+                for (int j = 0; j < kHalf / 64; j++)
+                    tma_load_3d(sm.b[st] + j * 64 * kK * 2, &maps.b, full, s.n * kN + bn + j * 64, a.v0 + kc, pb);
             } else {
 #pragma unroll
-                for (int j = 0; j < kM / 64; j++)
-                    tma_load_3d(sm.a[st] + j * 64 * kK * 2, &maps.a2, &sm.full[st], s.m * kM + j * 64, kc, pa);
-#pragma unroll
-                for (int j = 0; j < kN / 64; j++)
-                    tma_load_3d(sm.b[st] + j * 64 * kK * 2, &maps.b2, &sm.full[st], s.n * kN + j * 64, kc, pb);
+                for (int j = 0; j < kHalf / 64; j++) {
+                    tma_load_3d(sm.a[st] + j * 64 * kK * 2, &maps.a2, full, s.m * kM + am + j * 64, kc, pa);
+                    tma_load_3d(sm.b[st] + j * 64 * kK * 2, &maps.b2, full, s.n * kN + bn + j * 64, kc, pb);
+                }
             }
         }
     }
+    // the last products have let go of every stage: nothing arrives here once the block is gone
+    for (uint32_t i = it > kStages ? it - kStages : 0; i < it; i++)
+        if (!mbar_wait_suspend(&sm.empty[i % kStages], i / kStages & 1, ab, a.wait_ns)) return false;
     return true;
 }
 
-// ---- products: one warp ----------------------------------------------------------------------
+// ---- products: one warp of the first block -------------------------------------------------------
 template <int kMode>
 __device__ __forceinline__ bool multiply(Smem& sm, const Args& a, int count) {
     volatile int* ab = &sm.abort_flag;
@@ -285,11 +344,11 @@ __device__ __forceinline__ bool multiply(Smem& sm, const Args& a, int count) {
             const uint32_t da = desc_lo_sw128(smem_u32(sm.a[st]), a_lbo), db = desc_lo_sw128(smem_u32(sm.b[st]), b_lbo);
 #pragma unroll
             for (int j = 0; j < kK / 16; j++)
-                umma_bf16_elect(tm + acc * kN, da + j * a_step, db + j * b_step, idesc, !begins || j > 0);
-            umma_commit_elect(&sm.empty[st]);
+                pair_umma_elect(tm + acc * kN, da + j * a_step, db + j * b_step, idesc, !begins || j > 0);
+            pair_commit_elect(&sm.empty[st]);
             begins = k + 1 == s.k1 || place(a, k, s.kt).ends;
             if (begins) {
-                umma_commit_elect(&sm.acc_full[acc]);
+                pair_commit_elect(&sm.acc_full[acc]);
                 tile++;
             }
         }
@@ -297,7 +356,7 @@ __device__ __forceinline__ bool multiply(Smem& sm, const Args& a, int count) {
     return true;
 }
 
-// ---- epilogues: eight warps, a row a thread, 128 columns ---------------------------------------
+// ---- epilogues: eight warps of either block, a row a thread, 128 columns --------------------------
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
     return reinterpret_cast<const uint32_t&>(p);
@@ -368,7 +427,7 @@ __device__ __forceinline__ void emit(const Args& a, int count, float factor, int
 }
 
 constexpr int kSlotFloat4 = kM * kN / 4;
-// where lane `lane` of a warp keeps four columns of a partial tile: a warp's store is 512 bytes in a row
+// where lane `lane` of warp `warp` (of the pair's sixteen) keeps four columns of a partial tile: a warp's store is 512 bytes in a row
 __device__ __forceinline__ size_t slot_at(int slot, int warp, int chunk, int j4, int lane) {
     return (size_t)slot * kSlotFloat4 + ((warp * 4 + chunk) * 8 + j4) * 32 + lane;
 }
@@ -380,7 +439,13 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
     auto walk = make_walk<kMode>(a, count);
     Segment s;
     const int warp = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31, quarter = warp & 3, half = warp >> 2;
-    const int lrow = quarter * 32 + lane;                // row of the tile
+    const int rank = block_rank(), lrow = rank * kHalf + quarter * 32 + lane;   // row of the tile
+    const uint32_t acc_empty = in_first(&sm.acc_empty[0]);
+    auto release = [&](int acc) {                        // of the accumulator: a lane of every warp
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_at(acc_empty + acc * 8);
+    };
     const uint32_t tm = sm.tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
     float top = -INFINITY, sum = 0.f;
     int run_rows = -1, target = -1;                      // of the present row tile
@@ -415,8 +480,7 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
 #pragma unroll
                     for (int j = 0; j < 32; j++) folded[c * 32 + j] += z[j];
                 }
-                tc_fence_before();
-                mbar_arrive(&sm.acc_empty[acc]);
+                release(acc);
                 tile++;
             }
         } else {
@@ -490,7 +554,7 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
                 const bool live = row < count;
                 uint8_t* const mine = sm.out[warp];
 #pragma unroll 1
-                for (int p = 0; p < a.planes; p++) {
+                for (int p = 0; p < a.dz_planes; p++) {
                     if (lane == 0) tma_store_wait_read();
                     __syncwarp();
 #pragma unroll
@@ -499,7 +563,7 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
                                    pack2(z[8 * j + 6], z[8 * j + 7])};
                         if (!live) u = {0, 0, 0, 0};
                         *reinterpret_cast<uint4*>(mine + lane * 128 + ((j ^ (lane & 7)) << 4)) = u;
-                        if (p + 1 < a.planes) {          // what the rounding has left
+                        if (p + 1 < a.dz_planes) {          // what the rounding has left
                             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
@@ -510,12 +574,12 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
                     }
                     fence_proxy_async();
                     __syncwarp();
-                    if (lane == 0) tma_store_3d(map_out, mine, col, s.m * kM + quarter * 32, p);
+                    if (lane == 0) tma_store_3d(map_out, mine, col, s.m * kM + rank * kHalf + quarter * 32, p);
                 }
             }
         } else {
             const bool whole = s.k0 == 0 && s.k1 == s.kt;
-            const int slot = 2 * blockIdx.x + (s.k0 == 0 ? 1 : 0);
+            const int slot = 2 * pair_id() + (s.k0 == 0 ? 1 : 0);
 #pragma unroll kUnroll
             for (int c = 0; c < 4; c++) {
                 float v[32];
@@ -525,13 +589,12 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; j++)
-                        a.slots[slot_at(slot, warp, c, j, lane)] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                        a.slots[slot_at(slot, rank * 8 + warp, c, j, lane)] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
                 }
             }
         }
         if constexpr (!kFold) {
-            tc_fence_before();
-            mbar_arrive(&sm.acc_empty[acc]);
+            release(acc);
             tile++;
         }
         if (kMode == kStats && s.last) {
@@ -545,7 +608,7 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
 }
 
 template <int kMode, bool kFold>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtensorMap map_out, const Args a) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
@@ -556,14 +619,15 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
     }
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; i++) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
-        for (int i = 0; i < 2; i++) { mbar_init(&sm.acc_full[i], 1); mbar_init(&sm.acc_empty[i], 32 * kEpilogueWarps); }
+        for (int i = 0; i < 2; i++) { mbar_init(&sm.acc_full[i], 1); mbar_init(&sm.acc_empty[i], 2 * kEpilogueWarps); }
         sm.abort_flag = 0;
         fence_barrier_init();
     }
-    if (warp == 1) tmem_alloc(&sm.tmem_base, kTmemCols);
+    if (warp == 1) pair_tmem_alloc(&sm.tmem_base);
     fence_proxy_async();
     tc_fence_before();
     __syncthreads();
+    cluster_sync();
     tc_fence_after();
     const int count = *a.count;
     bool ok = true;
@@ -572,7 +636,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
         if constexpr (kFold) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0) {
             if ((threadIdx.x & 31) == 0 && !a.withhold) ok = produce<kMode>(sm, maps, a, count);
-        } else if (warp == 1) {
+        } else if (warp == 1 && block_rank() == 0) {
             ok = multiply<kMode>(sm, a, count);
         }
     } else {
@@ -583,16 +647,17 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (sm.abort_flag) {   // copies and products that are under way end within microseconds: none outlives the block's memory
+    if (sm.abort_flag) {   // copies and products that are under way end within microseconds: none outlives the pair's memory
         const uint64_t t0 = global_ns();
         while (global_ns() - t0 < 2'000'000ull) __nanosleep(1000);
-        __syncthreads();
     }
-    if (warp == 1) tmem_dealloc(sm.tmem_base, kTmemCols);
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1) pair_tmem_dealloc(sm.tmem_base);
 }
 
 // Sums the shares of the tiles that were split, in the order of their depth, and hands them out.  Block (boundary, group of
-// eight warps' chunks); the first boundary inside a tile does it.
+// eight warps' chunks); the first boundary inside a tile does it.  grid: pairs of the launch before.
 __global__ void __launch_bounds__(256) join_split_kernel(const Args a, int grid) {
     const int count = *a.count, p = (int)blockIdx.x + 1, lane = threadIdx.x & 31, id = blockIdx.y * 8 + (threadIdx.x >> 5);
     const int warp = id >> 2, chunk = id & 3;
@@ -622,7 +687,8 @@ __global__ void __launch_bounds__(256) join_split_kernel(const Args a, int grid)
         }
         any = true;
     }
-    emit(a, count, gradient_factor(a, count), dw, tile / t.d_tiles * kM + (warp & 3) * 32 + lane, tile % t.d_tiles * kN + (warp >> 2) * 128 + chunk * 32, v);
+    emit(a, count, gradient_factor(a, count), dw, tile / t.d_tiles * kM + (warp >> 3) * kHalf + (warp & 3) * 32 + lane,
+         tile % t.d_tiles * kN + (warp >> 2 & 1) * 128 + chunk * 32, v);
 }
 
 // ---- rows in, losses out -------------------------------------------------------------------------
@@ -791,13 +857,16 @@ inline size_t up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
 struct Sizes {
     int64_t rows;
-    int d, V, planes, terms, Tp, pitch, n_tiles, run, n_runs, pieces, vn, d_tiles;
+    int d, V, planes, dz_planes, Tp, pitch, n_tiles, run, n_runs, pieces, vn, d_tiles;
     bool f32;
     // saved
     size_t o_rows, o_words, o_max, o_inv, o_hit, o_x, saved;
     // scratch of the forward (W's planes if it is not read in place) and of the backward
     size_t w_planes, o_part, o_sums, fwd, o_dz, o_acc, o_slots, bwd;
 };
+// Up to this many rows of bf16, dz keeps 16 bits: where a row has one large entry (its target's), that entry's rounding to 8 bits is all of the
+// row's error.  Beyond, the rows' roundings average out and the product's time shows.
+constexpr int kFewRows = 256;
 constexpr size_t kPieceBytes = 512ull << 20;   // of dz, beyond which the vocabulary is cut
 constexpr int kMostRun = 8;                    // vocabulary tiles of a run: a tenth of a per cent of the row sums' traffic, still even shares
 
@@ -806,14 +875,14 @@ bool sizes_of(int64_t rows, int d, int vocab, int dtype, int sms, Sizes& s) {
     s.rows = rows; s.d = d; s.V = vocab;
     s.f32 = dtype == CDSSM_F32;
     s.planes = s.f32 ? 3 : 1;
-    s.terms = s.f32 ? kTerms3 : 1;
-    s.Tp = (int)up(rows, kRowTile);
+    s.dz_planes = s.f32 ? 3 : rows <= kFewRows ? 2 : 1;
+    s.Tp = (int)up(rows, kM);
     s.pitch = (int)up(d, 8);
     s.n_tiles = (vocab + kN - 1) / kN;
     const int64_t tiles = (int64_t)(s.Tp / kM) * s.n_tiles;
-    s.run = (int)std::min<int64_t>(kMostRun, std::max<int64_t>(1, tiles / (8 * (int64_t)sms)));
+    s.run = (int)std::min<int64_t>(kMostRun, std::max<int64_t>(1, tiles / (4 * (int64_t)sms)));
     s.n_runs = (s.n_tiles + s.run - 1) / s.run;
-    const size_t column = (size_t)s.Tp * 2 * s.planes;
+    const size_t column = (size_t)s.Tp * 2 * s.dz_planes;
     const size_t most = std::max<size_t>(kN, kPieceBytes / column / kN * kN);
     s.pieces = (int)((up(vocab, kN) + most - 1) / most);
     s.vn = (int)up((vocab + s.pieces - 1) / s.pieces, kN);
@@ -830,7 +899,7 @@ bool sizes_of(int64_t rows, int d, int vocab, int dtype, int sms, Sizes& s) {
     s.fwd = o;
     o = s.w_planes;
     s.o_dz = take(column * s.vn); s.o_acc = take(s.pieces > 1 ? 4ull * s.Tp * s.d_tiles * kN : 0);
-    s.o_slots = take(2ull * sms * kM * kN * 4);
+    s.o_slots = take(2ull * (sms / 2) * kM * kN * 4);
     s.bwd = o;
     return true;
 }
@@ -861,12 +930,13 @@ int launch_as(const Maps& maps, const CUtensorMap& out, const Args& a, int grid,
     product_kernel<kMode, kFold><<<grid, kThreads, sizeof(Smem), st>>>(maps, out, a);
     return check_launch();
 }
-constexpr int kNoFold = 1 << 30;
 template <int kMode>
 int launch_products(const Maps& maps, const CUtensorMap& out, Args a, int grid, cudaStream_t st) {
-    a.fold = a.planes == 3 ? kFold3 : kMode == kGradProducts ? kNoFold : kFoldLogits;
-    const bool one = kMode == kGradProducts ? a.fold == kNoFold : a.fold * kK >= a.d;
-    return one ? launch_as<kMode, false>(maps, out, a, grid, st) : launch_as<kMode, true>(maps, out, a, grid, st);
+    a.terms = a.planes == 3 ? kTerms3 : kMode == kGradProducts ? a.dz_planes : 1;
+    // (two parts of dz: block by block, so that the other operand's comes from L2 the second time)
+    a.group = a.planes == 3 ? kFold3 : kMode == kGradProducts ? 1 : kFoldLogits;
+    a.folds = a.planes == 3 || (kMode != kGradProducts && a.group * kK < a.d);
+    return a.folds ? launch_as<kMode, true>(maps, out, a, grid, st) : launch_as<kMode, false>(maps, out, a, grid, st);
 }
 
 bool in_place(const void* w, int64_t stride, int dtype) {   // a matrix that TMA reads as it lies
@@ -894,7 +964,7 @@ void fill_saved(Args& a, const Sizes& s, char* saved) {
     a.row_max = reinterpret_cast<float*>(saved + s.o_max);
     a.row_inv = reinterpret_cast<float*>(saved + s.o_inv);
     a.hit = reinterpret_cast<float*>(saved + s.o_hit);
-    a.planes = s.planes; a.terms = s.terms; a.Tp = s.Tp; a.d = s.d; a.V = s.V;
+    a.planes = s.planes; a.dz_planes = s.dz_planes; a.Tp = s.Tp; a.d = s.d; a.V = s.V;
     a.run = s.run; a.n_tiles = s.n_tiles; a.n_runs = s.n_runs; a.d_tiles = s.d_tiles;
     a.f32 = s.f32;
     a.vec_dx = a.vec_dw = s.d % (s.f32 ? 4 : 8) == 0;
@@ -939,13 +1009,13 @@ extern "C" int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, con
     if (!direct)
         if (int rc = ce::pack_any(w, w_row_stride, nullptr, nullptr, vocab, s, ws, st)) return rc;
     ce::Maps maps{};
-    if (!ce::make_map(&maps.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, ce::kM) ||
-        !ce::make_map(&maps.b, direct ? w : ws, direct ? d : s.pitch, vocab, s.planes, direct ? w_row_stride : s.pitch, ce::kK, ce::kN))
+    if (!ce::make_map(&maps.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, ce::kHalf) ||
+        !ce::make_map(&maps.b, direct ? w : ws, direct ? d : s.pitch, vocab, s.planes, direct ? w_row_stride : s.pitch, ce::kK, ce::kHalf))
         return CDSSM_ERR_CUDA;
     a.part = reinterpret_cast<float2*>(ws + s.o_part);
     a.withhold = (flags & CDSSM_SCAN_TEST_WITHHOLD) != 0;
     const int64_t units = (int64_t)(s.Tp / ce::kM) * s.n_runs;
-    if (int rc = ce::launch_products<ce::kStats>(maps, maps.a, a, (int)std::min<int64_t>(units, sms), st)) return rc;
+    if (int rc = ce::launch_products<ce::kStats>(maps, maps.a, a, 2 * (int)std::min<int64_t>(units, sms / 2), st)) return rc;
     ce::join_runs_kernel<<<s.Tp / 32, 32 * ce::kJoinWarps, 0, st>>>(a.part, 2 * s.n_runs, s.Tp, header, a.rows, a.target, a.row_max, a.row_inv,
                                                                   a.hit, loss, reduction, reinterpret_cast<double*>(ws + s.o_sums));
     return check_launch();
@@ -971,12 +1041,12 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
     const int64_t w_cols = direct ? d : s.pitch, w_pitch = direct ? w_row_stride : s.pitch;
     ce::Maps logits{}, grads{};
     CUtensorMap dz;
-    if (!ce::make_map(&logits.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, ce::kM) ||
-        !ce::make_map(&logits.b, wb, w_cols, vocab, s.planes, w_pitch, ce::kK, ce::kN) ||
-        !ce::make_map(&dz, ws + s.o_dz, s.vn, s.Tp, s.planes, s.vn, 64, 32) ||
-        !ce::make_map(&grads.a, ws + s.o_dz, s.vn, s.Tp, s.planes, s.vn, ce::kK, ce::kM) ||
+    if (!ce::make_map(&logits.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, ce::kHalf) ||
+        !ce::make_map(&logits.b, wb, w_cols, vocab, s.planes, w_pitch, ce::kK, ce::kHalf) ||
+        !ce::make_map(&dz, ws + s.o_dz, s.vn, s.Tp, s.dz_planes, s.vn, 64, 32) ||
+        !ce::make_map(&grads.a, ws + s.o_dz, s.vn, s.Tp, s.dz_planes, s.vn, ce::kK, ce::kHalf) ||
         !ce::make_map(&grads.b, wb, w_cols, vocab, s.planes, w_pitch, 64, ce::kK) ||
-        !ce::make_map(&grads.a2, ws + s.o_dz, s.vn, s.Tp, s.planes, s.vn, 64, ce::kK) ||
+        !ce::make_map(&grads.a2, ws + s.o_dz, s.vn, s.Tp, s.dz_planes, s.vn, 64, ce::kK) ||
         !ce::make_map(&grads.b2, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, 64, ce::kK))
         return CDSSM_ERR_CUDA;
     ce::Args a;
@@ -995,9 +1065,10 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
         a.vn_tiles = (a.vn + ce::kN - 1) / ce::kN;
         a.first = p == 0;
         a.last = p + 1 == s.pieces;
-        if (int rc = ce::launch_products<ce::kGradLogits>(logits, dz, a, sms, st)) return rc;
-        if (int rc = ce::launch_products<ce::kGradProducts>(grads, dz, a, sms, st)) return rc;
-        ce::join_split_kernel<<<dim3(sms, 4), 256, 0, st>>>(a, sms);
+        if (int rc = ce::launch_products<ce::kGradLogits>(logits, dz, a, sms / 2 * 2, st)) return rc;
+        if (int rc = ce::launch_products<ce::kGradProducts>(grads, dz, a, sms / 2 * 2, st)) return rc;
+        a.terms = s.f32 ? ce::kTerms3 : s.dz_planes;
+        ce::join_split_kernel<<<dim3(sms / 2, 8), 256, 0, st>>>(a, sms / 2);
         if (int rc = check_launch()) return rc;
     }
     if (grad_x) {
