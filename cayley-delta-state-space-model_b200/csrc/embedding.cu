@@ -14,7 +14,6 @@ namespace emb {
 namespace cg = cooperative_groups;
 
 // ---- values of a 16-byte vector, or single ones where rows are no multiple of it ---------------------
-template <typename T, int kE> struct Vec { T v[kE]; };
 template <typename T, int kE> __device__ __forceinline__ void load(const T* p, float (&f)[kE]) {
     if constexpr (kE == 1) {
         if constexpr (sizeof(T) == 2) f[0] = __bfloat162float(*p);
@@ -36,6 +35,9 @@ template <typename T, int kE> __device__ __forceinline__ void store(T* p, const 
     if constexpr (kE == 1) {
         if constexpr (sizeof(T) == 2) *p = __float2bfloat16_rn(f[0]);
         else *p = f[0];
+    } else if constexpr (sizeof(T) == 2 && kE == 4) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+        *reinterpret_cast<uint2*>(p) = make_uint2(reinterpret_cast<const uint32_t&>(a), reinterpret_cast<const uint32_t&>(b));
     } else if constexpr (sizeof(T) == 2) {
         uint32_t w[4];
 #pragma unroll
@@ -49,26 +51,32 @@ template <typename T, int kE> __device__ __forceinline__ void store(T* p, const 
     }
 }
 
-// A thread per vector of the output; an id that is no row of the table gives NaN.
+// A warp per row; an id that is no row of the table gives NaN.
 template <typename T, int kE>
 __global__ void __launch_bounds__(256)
 embed_kernel(const int64_t* __restrict__ ids, const T* __restrict__ w, int64_t w_stride, T* __restrict__ out, int64_t n, int vocab, int d, float scale) {
-    const int per_row = d / kE;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t t = i / per_row;
+    const int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    grid_launch_dependents();
+    grid_dependency_wait();
     if (t >= n) return;
-    const int c = (int)(i - t * per_row) * kE;
     const int64_t id = ids[t];
-    float f[kE];
-    if (id >= 0 && id < vocab) {
-        load<T, kE>(w + id * w_stride + c, f);
+    const bool known = id >= 0 && id < vocab;
+    const T* const from = w + (known ? id : 0) * w_stride;
+    T* const to = out + t * d;
+    constexpr int kAhead = 4;
+    for (int c0 = (threadIdx.x & 31) * kE; c0 < d; c0 += 32 * kE * kAhead) {
+        float f[kAhead][kE];
 #pragma unroll
-        for (int e = 0; e < kE; e++) f[e] *= scale;
-    } else {
+        for (int k = 0; k < kAhead; k++)
+            if (c0 + k * 32 * kE < d) load<T, kE>(from + c0 + k * 32 * kE, f[k]);
 #pragma unroll
-        for (int e = 0; e < kE; e++) f[e] = NAN;
+        for (int k = 0; k < kAhead; k++)
+            if (c0 + k * 32 * kE < d) {
+#pragma unroll
+                for (int e = 0; e < kE; e++) f[k][e] = known ? f[k][e] * scale : NAN;
+                store<T, kE>(to + c0 + k * 32 * kE, f[k]);
+            }
     }
-    store<T, kE>(out + t * d + c, f);
 }
 
 // ---- sort ------------------------------------------------------------------------------------------
@@ -85,13 +93,17 @@ struct SortSmem {
 // of the pairs; the other clusters write zeros.  Ids that take no part (no row of the table, `skip`) get the key vocab: behind all others.
 __global__ void __launch_bounds__(kSortThreads)
 sort_and_clear_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t skip, int bits, int passes, uint2* buf0, uint2* buf1,
-                      uint4* __restrict__ zero, size_t zero_vecs, unsigned char* zero_tail, int tail_bytes) {
+                      uint4* __restrict__ zero, size_t zero_vecs, unsigned char* zero_tail, int tail_bytes, int* spans) {
     __shared__ SortSmem sm;
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), c = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    if (blockIdx.x == 0 && tid == 0) spans[0] = 0;
     if ((int)blockIdx.x >= C) {
         const size_t step = (size_t)(gridDim.x - C) * kSortThreads;
-        for (size_t i = (size_t)(blockIdx.x - C) * kSortThreads + tid; i < zero_vecs; i += step) __stcs(zero + i, make_uint4(0, 0, 0, 0));
+#pragma unroll 4
+        for (size_t i = (size_t)(blockIdx.x - C) * kSortThreads + tid; i < zero_vecs; i += step) zero[i] = make_uint4(0, 0, 0, 0);
         if ((int)blockIdx.x == C && tid < tail_bytes) zero_tail[tid] = 0;
         return;
     }
@@ -171,12 +183,15 @@ sort_and_clear_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t
 
 // ---- sums --------------------------------------------------------------------------------------------
 // kTile sorted pairs of some columns a block: rows of one id are added up in their order.  An id that lies inside the tile is done; of
-// one that came from the tile before the sum goes to head, of one that goes on into the next (and began here) to tail.
+// one that came from the tile before the sum goes to head, of one that goes on into the next (and began here) to tail, and the tile is listed
+// in spans (their number first).
 template <typename T, int kE, int kTile>
 __global__ void sum_tiles_kernel(const uint2* __restrict__ pairs, int n, int vocab, const T* __restrict__ grad, T* __restrict__ dw,
-                                 float* __restrict__ head, float* __restrict__ tail, int d, float scale) {
+                                 float* __restrict__ head, float* __restrict__ tail, int* __restrict__ spans, int d, float scale) {
     __shared__ uint2 tile[kTile + 2];   // with the neighbours of either side
     const int tile_id = blockIdx.x, p0 = tile_id * kTile;
+    grid_launch_dependents();
+    grid_dependency_wait();
     for (int i = threadIdx.x; i < kTile + 2; i += blockDim.x) {
         const int p = p0 + i - 1;
         tile[i] = p >= 0 && p < n ? pairs[p] : make_uint2((unsigned)vocab, 0);
@@ -205,6 +220,7 @@ __global__ void sum_tiles_kernel(const uint2* __restrict__ pairs, int n, int voc
                     float* const to = (from_before ? head : tail) + (size_t)tile_id * d + c;
 #pragma unroll
                     for (int e = 0; e < kE; e++) to[e] = sum[e];
+                    if (!ends && !from_before && c == 0) spans[1 + atomicAdd(spans, 1)] = tile_id;   // (their order changes nothing)
                 } else {
 #pragma unroll
                     for (int e = 0; e < kE; e++) sum[e] *= scale;
@@ -218,55 +234,71 @@ __global__ void sum_tiles_kernel(const uint2* __restrict__ pairs, int n, int voc
     }
 }
 
-// An id that begins in this tile and goes on: its tail and the heads of the tiles behind, eight contiguous parts beside each other.
+// An id that begins in a listed tile and goes on: its tail and the heads of the tiles behind, eight contiguous parts beside each other and
+// then those in order; 32 x kE columns at a time.  (A block per tile instead of the list: 29 us for 512 tiles, nearly all of them without one.)
 constexpr int kJoinParts = 8;
-template <typename T, int kTile>
+template <typename T, int kE, int kTile>
 __global__ void __launch_bounds__(32 * kJoinParts)
-join_tiles_kernel(const uint2* __restrict__ pairs, int n, int vocab, const float* __restrict__ head, const float* __restrict__ tail, T* __restrict__ dw,
-                  int d, float scale) {
-    __shared__ float part[kJoinParts][32];
-    const int tile_id = blockIdx.x, last = tile_id * kTile + kTile - 1;
-    if (last + 1 >= n) return;
-    const unsigned id = pairs[last].x;
-    if (id >= (unsigned)vocab || pairs[last + 1].x != id) return;
-    if (tile_id > 0 && pairs[last - kTile].x == id) return;   // it came from the tile before
-    int lo = last + 1, hi = n;                                 // first pair of another id
-    while (lo < hi) {
-        const int mid = lo + (hi - lo) / 2;
-        if (pairs[mid].x == id) lo = mid + 1;
-        else hi = mid;
-    }
-    const int tiles = (lo - 1) / kTile - tile_id + 1, lane = threadIdx.x & 31, y = threadIdx.x >> 5;
-    const int share = (tiles + kJoinParts - 1) / kJoinParts, q0 = y * share, q1 = min(tiles, q0 + share);
-    const int c = blockIdx.y * 32 + lane;
-    float sum = 0.f;
-    if (c < d)
+join_tiles_kernel(const uint2* __restrict__ pairs, int n, const float* __restrict__ head, const float* __restrict__ tail, const int* __restrict__ spans,
+                  T* __restrict__ dw, int d, float scale) {
+    __shared__ float part[kJoinParts][32][kE];
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31, y = threadIdx.x >> 5, chunks = (d + 32 * kE - 1) / (32 * kE);
+    const long long items = (long long)spans[0] * chunks;
+    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+        const int tile_id = spans[1 + item / chunks], c = ((int)(item % chunks) * 32 + lane) * kE;
+        const unsigned id = pairs[(size_t)tile_id * kTile + kTile - 1].x;
+        int lo = (tile_id + 1) * kTile, hi = n;              // first pair of another id
+        while (lo < hi) {
+            const int mid = lo + (hi - lo) / 2;
+            if (pairs[mid].x == id) lo = mid + 1;
+            else hi = mid;
+        }
+        const int tiles = (lo - 1) / kTile - tile_id + 1, share = (tiles + kJoinParts - 1) / kJoinParts, q0 = y * share, q1 = min(tiles, q0 + share);
+        float sum[kE] = {};
+        if (c < d) {
 #pragma unroll 8
-        for (int q = q0; q < q1; q++) sum += (q ? head : tail)[(size_t)(tile_id + q) * d + c];
-    part[y][lane] = sum;
-    __syncthreads();
-    if (y == 0 && c < d) {
-        for (int i = 1; i < kJoinParts; i++) sum += part[i][lane];
-        float f[1] = {sum * scale};
-        store<T, 1>(dw + (size_t)id * d + c, f);
+            for (int q = q0; q < q1; q++) {
+                float f[kE];
+                load<float, kE>((q ? head : tail) + (size_t)(tile_id + q) * d + c, f);
+#pragma unroll
+                for (int e = 0; e < kE; e++) sum[e] += f[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kE; e++) part[y][lane][e] = sum[e];
+        __syncthreads();
+        if (y == 0 && c < d) {
+            for (int i = 1; i < kJoinParts; i++)
+#pragma unroll
+                for (int e = 0; e < kE; e++) sum[e] += part[i][lane][e];
+#pragma unroll
+            for (int e = 0; e < kE; e++) sum[e] *= scale;
+            store<T, kE>(dw + (size_t)id * d + c, sum);
+        }
+        __syncthreads();
     }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------
 inline size_t up(size_t n, size_t to) { return (n + to - 1) / to * to; }
-constexpr int kTilePairs = 32;
+// Pairs of a tile: few where there are few of them (523 tokens by 32: 10 us for 17 blocks of four rounds of loads).
+constexpr int kFewPairs = 8192, kTileFew = 8, kTileMany = 32;
 
 struct Layout {
-    size_t buf0, buf1, head, tail, bytes;
+    size_t buf0, buf1, head, tail, spans, bytes;
     int tiles;
 };
 Layout layout(int64_t n, int d) {
     Layout l;
-    l.tiles = (int)((n + kTilePairs - 1) / kTilePairs);
+    const int tile = n <= kFewPairs ? kTileFew : kTileMany;
+    l.tiles = (int)((n + tile - 1) / tile);
     size_t o = 0;
     auto take = [&](size_t b) { const size_t at = o; o += up(b, 256); return at; };
     l.buf0 = take(8 * (size_t)n); l.buf1 = take(8 * (size_t)n);
     l.head = take(4 * (size_t)l.tiles * d); l.tail = take(4 * (size_t)l.tiles * d);
+    l.spans = take(4 * ((size_t)l.tiles + 1));
     l.bytes = o;
     return l;
 }
@@ -278,20 +310,26 @@ int check_sizes(int64_t n, int vocab, int d, int dtype) {
 
 template <typename T, int kE>
 int forward(const int64_t* ids, const void* w, int64_t w_stride, void* out, int64_t n, int vocab, int d, float scale, cudaStream_t st) {
-    const int64_t blocks = (n * (d / kE) + 255) / 256;
-    if (blocks > 0x7fffffff) return CDSSM_ERR_UNSUPPORTED;
-    embed_kernel<T, kE><<<(unsigned)blocks, 256, 0, st>>>(ids, static_cast<const T*>(w), w_stride, static_cast<T*>(out), n, vocab, d, scale);
-    return check_launch();
+    return launch_overlapped(embed_kernel<T, kE>, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, ids, static_cast<const T*>(w), w_stride,
+                             static_cast<T*>(out), n, vocab, d, scale);
 }
 
-template <typename T, int kE>
-int sums(const uint2* pairs, int n, int vocab, const void* grad, void* dw, float* head, float* tail, int tiles, int d, float scale, cudaStream_t st) {
+template <typename T, int kE, int kTile>
+int sums_by(const uint2* pairs, int n, int vocab, const void* grad, void* dw, char* ws, const Layout& l, int d, float scale, int sms, cudaStream_t st) {
     const int vecs = d / kE, threads = std::min(256, (vecs + 31) / 32 * 32);
-    sum_tiles_kernel<T, kE, kTilePairs><<<dim3(tiles, (vecs + threads - 1) / threads), threads, 0, st>>>(
-        pairs, n, vocab, static_cast<const T*>(grad), static_cast<T*>(dw), head, tail, d, scale);
-    if (int rc = check_launch()) return rc;
-    join_tiles_kernel<T, kTilePairs><<<dim3(tiles, (d + 31) / 32), 32 * kJoinParts, 0, st>>>(pairs, n, vocab, head, tail, static_cast<T*>(dw), d, scale);
-    return check_launch();
+    float *const head = reinterpret_cast<float*>(ws + l.head), *const tail = reinterpret_cast<float*>(ws + l.tail);
+    int* const spans = reinterpret_cast<int*>(ws + l.spans);
+    if (int rc = launch_overlapped(sum_tiles_kernel<T, kE, kTile>, dim3(l.tiles, (vecs + threads - 1) / threads), dim3(threads), 0, st, pairs, n, vocab,
+                                   static_cast<const T*>(grad), static_cast<T*>(dw), head, tail, spans, d, scale))
+        return rc;
+    constexpr int kJoinE = kE == 1 ? 1 : 4;
+    return launch_overlapped(join_tiles_kernel<T, kJoinE, kTile>, dim3(std::min(l.tiles * ((d + 127) / 128), 4 * sms)), dim3(32 * kJoinParts), 0, st,
+                             pairs, n, head, tail, spans, static_cast<T*>(dw), d, scale);
+}
+template <typename T, int kE>
+int sums(const uint2* pairs, int n, int vocab, const void* grad, void* dw, char* ws, const Layout& l, int d, float scale, int sms, cudaStream_t st) {
+    return n <= kFewPairs ? sums_by<T, kE, kTileFew>(pairs, n, vocab, grad, dw, ws, l, d, scale, sms, st)
+                          : sums_by<T, kE, kTileMany>(pairs, n, vocab, grad, dw, ws, l, d, scale, sms, st);
 }
 
 }  // namespace emb
@@ -339,21 +377,22 @@ extern "C" int cdssm_b200_embedding_bwd(const int64_t* ids, const void* grad, vo
     cfg.gridDim = dim3((unsigned)(cluster * std::max(2, sms / cluster)));
     cfg.blockDim = dim3(emb::kSortThreads);
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     if (int rc = counted(check_cuda(cudaLaunchKernelEx(&cfg, emb::sort_and_clear_kernel, ids, (int)n, vocab, padding_idx, per_pass, passes, b0, b1,
                                                        static_cast<uint4*>(grad_w), bytes / 16, static_cast<unsigned char*>(grad_w) + bytes / 16 * 16,
-                                                       (int)(bytes % 16)))))
+                                                       (int)(bytes % 16), reinterpret_cast<int*>(ws + l.spans)))))
         return rc;
     const uint2* const sorted = passes & 1 ? b0 : b1;
-    float *const head = reinterpret_cast<float*>(ws + l.head), *const tail = reinterpret_cast<float*>(ws + l.tail);
     if (dtype == CDSSM_BF16)
-        return d % 8 == 0 ? emb::sums<__nv_bfloat16, 8>(sorted, (int)n, vocab, grad, grad_w, head, tail, l.tiles, d, scale, st)
-                          : emb::sums<__nv_bfloat16, 1>(sorted, (int)n, vocab, grad, grad_w, head, tail, l.tiles, d, scale, st);
-    return d % 4 == 0 ? emb::sums<float, 4>(sorted, (int)n, vocab, grad, grad_w, head, tail, l.tiles, d, scale, st)
-                      : emb::sums<float, 1>(sorted, (int)n, vocab, grad, grad_w, head, tail, l.tiles, d, scale, st);
+        return d % 8 == 0 ? emb::sums<__nv_bfloat16, 8>(sorted, (int)n, vocab, grad, grad_w, ws, l, d, scale, sms, st)
+                          : emb::sums<__nv_bfloat16, 1>(sorted, (int)n, vocab, grad, grad_w, ws, l, d, scale, sms, st);
+    return d % 4 == 0 ? emb::sums<float, 4>(sorted, (int)n, vocab, grad, grad_w, ws, l, d, scale, sms, st)
+                      : emb::sums<float, 1>(sorted, (int)n, vocab, grad, grad_w, ws, l, d, scale, sms, st);
 }

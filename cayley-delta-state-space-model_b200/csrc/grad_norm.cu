@@ -6,6 +6,8 @@
 // the blocks in a fixed order: the same bits from run to run, and no length at which small gradients are lost.
 #include "cdssm_common.cuh"
 #include <cuda_bf16.h>
+#include <algorithm>
+#include <type_traits>
 
 namespace cdssm {
 namespace gn {
@@ -128,6 +130,8 @@ __device__ __forceinline__ double block_sum(double x) {   // valid in thread 0
 template <int kMost>
 __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ Table<kMost> t, double* __restrict__ sums) {
     const Piece p = piece(t, blockIdx.x);
+    grid_launch_dependents();
+    grid_dependency_wait();
     const double s = block_sum(p.in_f32 ? chunk_squares(static_cast<const float*>(p.in) + p.at, p.n)
                                         : chunk_squares(static_cast<const __nv_bfloat16*>(p.in) + p.at, p.n));
     if (threadIdx.x == 0) sums[blockIdx.x] = s;
@@ -135,8 +139,17 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
 
 // norm and the factor (1 where the norm is within the bound; NaN where it is none)
 __global__ void __launch_bounds__(1024) norm_kernel(const double* __restrict__ sums, int64_t n, float max_norm, float* norm, float* factor) {
+    grid_launch_dependents();
+    grid_dependency_wait();
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) s += sums[i];
+    constexpr int kAhead = 8;
+    for (int64_t i = threadIdx.x; i < n; i += 1024 * kAhead) {
+        double x[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) x[k] = i + 1024 * k < n ? __ldg(sums + i + 1024 * k) : 0.0;
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) s += x[k];
+    }
     s = block_sum(s);
     if (threadIdx.x == 0) {
         const float x = (float)sqrt(s), c = max_norm / (x + 1e-6f);
@@ -147,7 +160,6 @@ __global__ void __launch_bounds__(1024) norm_kernel(const double* __restrict__ s
 
 template <typename T, typename O>
 __device__ __forceinline__ void chunk_scale(const T* p, O* o, int n, float c) {
-    constexpr int kE = PerVec<T>::k;
     const bool bits = c == 1.f && sizeof(T) == sizeof(O);
     auto one = [&](int i) {
         if constexpr (sizeof(T) == sizeof(O)) {
@@ -156,18 +168,22 @@ __device__ __forceinline__ void chunk_scale(const T* p, O* o, int n, float c) {
         if constexpr (sizeof(O) == 2) o[i] = __float2bfloat16_rn(value(p[i]) * c);
         else o[i] = value(p[i]) * c;
     };
-    const int lead = min(n, (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T));
-    if (((uintptr_t)(o + lead) & 15) != 0) {   // the two lie at different offsets
+    // values up to the first 16-byte boundary of the output and behind the last one singly
+    constexpr int kE = 16 / sizeof(O);
+    const int lead = min(n, (int)((16 - ((uintptr_t)o & 15)) & 15) / (int)sizeof(O));
+    if (((uintptr_t)(p + lead) & (kE * sizeof(T) - 1)) != 0) {   // the two lie at different offsets
         for (int i = threadIdx.x; i < n; i += kThreads) one(i);
         return;
     }
     const int vecs = (n - lead) / kE, rest = n - lead - vecs * kE;
     if (threadIdx.x < lead) one(threadIdx.x);
     if (threadIdx.x < rest) one(n - rest + threadIdx.x);
-    const uint4* const v = reinterpret_cast<const uint4*>(p + lead);
+    using In = std::conditional_t<sizeof(T) == sizeof(O), uint4, uint2>;
+    const In* const v = reinterpret_cast<const In*>(p + lead);
+    uint4* const to = reinterpret_cast<uint4*>(o + lead);
     constexpr int kAhead = 4;
     for (int i0 = threadIdx.x; i0 < vecs; i0 += kThreads * kAhead) {
-        uint4 u[kAhead];
+        In u[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; k++)
             if (i0 + k * kThreads < vecs) u[k] = v[i0 + k * kThreads];
@@ -175,38 +191,47 @@ __device__ __forceinline__ void chunk_scale(const T* p, O* o, int n, float c) {
         for (int k = 0; k < kAhead; k++) {
             const int i = i0 + k * kThreads;
             if (i >= vecs) continue;
-            float f[kE];
-            unpack<T>(u[k], f);
-#pragma unroll
-            for (int e = 0; e < kE; e++) f[e] *= c;
-            if constexpr (sizeof(O) == 2) {
-                uint32_t w[4];
+            if constexpr (sizeof(T) == sizeof(O)) {
+                if (bits) { to[i] = u[k]; continue; }
+                const uint32_t w[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+                uint32_t r[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * e], f[2 * e + 1]);
-                    w[e] = reinterpret_cast<const uint32_t&>(b);
+                    if constexpr (sizeof(T) == 2) {
+                        const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(w[e] << 16) * c, __uint_as_float(w[e] & 0xffff0000u) * c);
+                        r[e] = reinterpret_cast<const uint32_t&>(b);
+                    } else {
+                        r[e] = __float_as_uint(__uint_as_float(w[e]) * c);
+                    }
                 }
-                reinterpret_cast<uint4*>(o + lead)[i] = bits ? u[k] : make_uint4(w[0], w[1], w[2], w[3]);
+                to[i] = make_uint4(r[0], r[1], r[2], r[3]);
             } else {
-#pragma unroll
-                for (int e = 0; e < kE; e += 4)
-                    reinterpret_cast<float4*>(o + lead)[i * (kE / 4) + e / 4] = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+                const uint32_t w[2] = {u[k].x, u[k].y};
+                to[i] = make_uint4(__float_as_uint(__uint_as_float(w[0] << 16) * c), __float_as_uint(__uint_as_float(w[0] & 0xffff0000u) * c),
+                                   __float_as_uint(__uint_as_float(w[1] << 16) * c), __float_as_uint(__uint_as_float(w[1] & 0xffff0000u) * c));
             }
         }
     }
 }
 
-// The chunks backwards: what the norm has read last is in L2 still.
+// The chunks backwards: what the norm has read last is in L2 still.  In place and within the bound there is nothing to do, and the grid is
+// small enough to find that out quickly (26 000 blocks: 31 us).
 template <int kMost>
-__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table<kMost> t, const float* __restrict__ factor) {
+__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table<kMost> t, const float* __restrict__ factor, int chunks, int in_place) {
+    grid_launch_dependents();
+    grid_dependency_wait();
     const float c = *factor;
-    const Piece p = piece(t, (int)(gridDim.x - 1 - blockIdx.x));
-    if (c == 1.f && p.in == p.out) return;
-    if (p.in_f32) chunk_scale(static_cast<const float*>(p.in) + p.at, static_cast<float*>(p.out) + p.at, p.n, c);
-    else if (p.out_f32) chunk_scale(static_cast<const __nv_bfloat16*>(p.in) + p.at, static_cast<float*>(p.out) + p.at, p.n, c);
-    else chunk_scale(static_cast<const __nv_bfloat16*>(p.in) + p.at, static_cast<__nv_bfloat16*>(p.out) + p.at, p.n, c);
+    if (c == 1.f && in_place) return;
+    for (int chunk = chunks - 1 - (int)blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
+        const Piece p = piece(t, chunk);
+        if (c == 1.f && p.in == p.out) continue;
+        if (p.in_f32) chunk_scale(static_cast<const float*>(p.in) + p.at, static_cast<float*>(p.out) + p.at, p.n, c);
+        else if (p.out_f32) chunk_scale(static_cast<const __nv_bfloat16*>(p.in) + p.at, static_cast<float*>(p.out) + p.at, p.n, c);
+        else chunk_scale(static_cast<const __nv_bfloat16*>(p.in) + p.at, static_cast<__nv_bfloat16*>(p.out) + p.at, p.n, c);
+    }
 }
 
+constexpr int kScaleBlocks = 8;              // of an SM
 constexpr int kSmall = 48, kLarge = 900;   // tensors of a launch: a table of 2 KB, or of as much as kernel arguments may hold
 
 inline int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
@@ -245,18 +270,20 @@ int run(const void* const* in, void* const* out, const int64_t* sizes, const int
     Table<kMost> t;
     int rc = each_launch(sizes, n, [&](int first, int m, int64_t chunks) {
         fill(t, in, nullptr, sizes, in_dt, nullptr, first, m);
-        squares_kernel<kMost><<<(unsigned)chunks, kThreads, 0, st>>>(t, sums + at);
+        const int64_t to = at;
         at += chunks;
-        return check_launch();
+        return launch_overlapped(squares_kernel<kMost>, dim3((unsigned)chunks), dim3(kThreads), 0, st, t, sums + to);
     });
     if (rc) return rc;
-    norm_kernel<<<1, 1024, 0, st>>>(sums, at, max_norm, norm, factor);
-    if (int e = check_launch()) return e;
+    if (int e = launch_overlapped(norm_kernel, dim3(1), dim3(1024), 0, st, sums, at, max_norm, norm, factor)) return e;
     if (!out) return CDSSM_OK;
+    int sms = 0, in_place = 1;
+    if (int e = sm_count(sms)) return e;
+    for (int i = 0; i < n; i++) in_place &= in[i] == out[i];
     return each_launch(sizes, n, [&](int first, int m, int64_t chunks) {
         fill(t, in, out, sizes, in_dt, out_dt, first, m);
-        scale_kernel<kMost><<<(unsigned)chunks, kThreads, 0, st>>>(t, factor);
-        return check_launch();
+        return launch_overlapped(scale_kernel<kMost>, dim3((unsigned)std::min<int64_t>(chunks, kScaleBlocks * sms)), dim3(kThreads), 0, st, t, factor,
+                                 (int)chunks, in_place);
     });
 }
 

@@ -2,6 +2,8 @@
 // with their gradients, and the norm and clipping of all gradients.
 #include "host.h"
 
+#include <torch/csrc/autograd/custom_function.h>
+
 #include <algorithm>
 #include <cmath>
 #include <vector>
@@ -23,142 +25,169 @@ Tensor row_matrix(const Tensor& t, int64_t d) {
 }
 int64_t row_stride(const Tensor& m) { return m.size(0) > 1 ? m.stride(0) : m.size(1); }
 
-struct CeArgs {
-    Tensor weight;   // (vocab, d), rows dense
-    int64_t rows, d, vocab, ignore;
-    int reduction, dtype;
-};
-Tensor ce_weight(const Tensor& weight) {
-    return (weight.size(1) == 1 || weight.stride(1) == 1) && (weight.size(0) == 1 || weight.stride(0) >= weight.size(1)) ? weight : weight.contiguous();
+// (vocab, d), rows dense and apart: as it lies, or a copy
+Tensor table(const Tensor& w) {
+    return (w.size(1) == 1 || w.stride(1) == 1) && (w.size(0) == 1 || w.stride(0) >= w.size(1)) ? w : w.contiguous();
+}
+void need_table(const Tensor& w, const char* name) {
+    need_cuda(w, name);
+    need_dims(w, 2, name);
+    if (w.size(0) < 1 || w.size(1) < 1) throw Error(std::string(name) + " is empty");
+    if (w.size(0) > INT32_MAX || w.size(1) > INT32_MAX) check(CDSSM_ERR_UNSUPPORTED, name);
+    dtype_code(w);
+}
+bool wants_grad(const Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+// The gradients come from kernels that autograd does not see into: a graph of them would leave out what they depend on.
+void once_only(const char* what) {
+    if (c10::GradMode::is_enabled()) throw Error(std::string(what) + " is differentiable once: no create_graph=True");
 }
 
-// linear_ce_fwd(hidden (.., d), weight (vocab, d), targets (..) int64, ignore_index, reduction, flags) -> (loss, saved bytes)
-PyObject* py_linear_ce_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// ---- loss ------------------------------------------------------------------------------------------
+struct CeOut {
+    Tensor loss, saved;
+};
+CeOut ce_forward(const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignore, int64_t reduction, int64_t flags) {
+    const c10::cuda::CUDAGuard guard(hidden.device());
+    const int64_t d = weight.size(1), vocab = weight.size(0), rows = targets.numel();
+    const int dt = dtype_code(hidden);
+    const Tensor loss = reduction == CDSSM_CE_NONE ? empty_f32(targets.sizes(), hidden) : empty_f32({}, hidden);
+    if (rows == 0) {   // mean of nothing: NaN, as everywhere
+        if (reduction != CDSSM_CE_NONE) loss.fill_(reduction == CDSSM_CE_MEAN ? NAN : 0.0);
+        return {loss, scratch(0, hidden)};
+    }
+    const size_t sb = cdssm_b200_linear_ce_saved_bytes(rows, (int)d, (int)vocab, dt);
+    if (sb == 0) check(CDSSM_ERR_UNSUPPORTED, "linear_cross_entropy");
+    const size_t wb = cdssm_b200_linear_ce_workspace_bytes(rows, (int)d, (int)vocab, dt, 0);
+    const Tensor x = row_matrix(hidden, d), w = table(weight), y = targets.contiguous(), ws = scratch(wb, hidden), saved = scratch(sb, hidden);
+    check(cdssm_b200_linear_ce_fwd(cptr(x), row_stride(x), cptr(w), row_stride(w), y.const_data_ptr<int64_t>(), fmut(loss), mptr(saved), sb, mptr(ws),
+                                   wb, rows, (int)d, (int)vocab, ignore, (int)reduction, dt, (int)flags, stream_of(x)),
+          "linear_cross_entropy");
+    return {loss, saved};
+}
+struct CeGrads {
+    Tensor x, w;
+};
+CeGrads ce_backward(const Tensor& grad, const Tensor& weight, const Tensor& targets, const Tensor& saved, int64_t ignore, int64_t reduction,
+                    bool want_x, bool want_w, at::IntArrayRef hidden_sizes, int64_t flags) {
+    const c10::cuda::CUDAGuard guard(weight.device());
+    const int64_t d = weight.size(1), vocab = weight.size(0), rows = targets.numel();
+    const int dt = dtype_code(weight);
+    CeGrads r;
+    if (want_x) r.x = empty_like_dims(hidden_sizes, weight);
+    if (want_w) r.w = rows ? empty_like_dims({vocab, d}, weight) : at::zeros({vocab, d}, weight.options());
+    if (rows == 0 || (!want_x && !want_w)) return r;
+    const size_t wb = cdssm_b200_linear_ce_workspace_bytes(rows, (int)d, (int)vocab, dt, 1);
+    const Tensor g = (grad.scalar_type() == at::kFloat ? grad : grad.to(at::kFloat)).contiguous(), w = table(weight), y = targets.contiguous(),
+                 ws = scratch(wb, weight);
+    check(cdssm_b200_linear_ce_bwd(fptr(g), cptr(w), row_stride(w), y.const_data_ptr<int64_t>(), mptr(saved), (size_t)saved.numel(), mptr(r.x), mptr(r.w),
+                                   mptr(ws), wb, rows, (int)d, (int)vocab, ignore, (int)reduction, dt, (int)flags, stream_of(w)),
+          "linear_cross_entropy backward");
+    return r;
+}
+struct CeNode : torch::autograd::Function<CeNode> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignore,
+                          int64_t reduction, int64_t flags) {
+        CeOut o = ce_forward(hidden, weight, targets, ignore, reduction, flags);
+        ctx->save_for_backward({weight, targets, o.saved});
+        ctx->saved_data["args"] = std::vector<int64_t>{ignore, reduction, flags};
+        ctx->saved_data["sizes"] = hidden.sizes().vec();
+        return o.loss;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        once_only("linear_cross_entropy");
+        const auto saved = ctx->get_saved_variables();
+        const auto args = ctx->saved_data["args"].toIntVector(), sizes = ctx->saved_data["sizes"].toIntVector();
+        CeGrads g = ce_backward(grads[0], saved[0], saved[1], saved[2], args[0], args[1], ctx->needs_input_grad(0), ctx->needs_input_grad(1), sizes, args[2]);
+        return {g.x, g.w, Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// linear_cross_entropy(hidden (.., d), weight (vocab, d), targets (..) int64, ignore_index, reduction, flags) -> loss
+PyObject* py_linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&] {
         Args in{a, n};
-        const Tensor hidden = in.tensor("hidden"), weight_ = in.tensor("weight"), targets = in.tensor("targets");
+        const Tensor hidden = in.tensor("hidden"), weight = in.tensor("weight"), targets = in.tensor("targets");
         const int64_t ignore = in.integer(), reduction = in.integer(), flags = in.integer();
         need_cuda(hidden, "hidden");
-        need_cuda(weight_, "weight");
+        need_table(weight, "weight");
         need_cuda(targets, "targets");
-        need_same_device(weight_, hidden, "weight");
+        need_same_device(weight, hidden, "weight");
         need_same_device(targets, hidden, "targets");
-        const int dt = dtype_code(hidden);
-        if (weight_.scalar_type() != hidden.scalar_type())
-            throw Error(std::string("weight has dtype ") + c10::toString(weight_.scalar_type()) + ", hidden " + c10::toString(hidden.scalar_type()));
+        dtype_code(hidden);
+        if (weight.scalar_type() != hidden.scalar_type())
+            throw Error(std::string("weight has dtype ") + c10::toString(weight.scalar_type()) + ", hidden " + c10::toString(hidden.scalar_type()));
         if (targets.scalar_type() != at::kLong) throw Error("targets must be int64");
-        need_dims(weight_, 2, "weight");
-        if (hidden.dim() < 1 || hidden.size(-1) != weight_.size(1)) throw Error("hidden and weight must agree in their last dimension");
-        const int64_t d = weight_.size(1), vocab = weight_.size(0);
-        if (d < 1 || vocab < 1) throw Error("weight is empty");
+        if (hidden.dim() < 1 || hidden.size(-1) != weight.size(1)) throw Error("hidden and weight must agree in their last dimension");
         if (targets.sizes() != hidden.sizes().slice(0, hidden.dim() - 1)) throw Error("targets must have hidden's shape without its last dimension");
-        const int64_t rows = targets.numel();
-        Tensor loss, saved;
-        without_gil([&] {
-            const c10::cuda::CUDAGuard guard(hidden.device());
-            loss = reduction == CDSSM_CE_NONE ? empty_f32(targets.sizes(), hidden) : empty_f32({}, hidden);
-            if (rows == 0) {   // mean of nothing: NaN, as everywhere
-                if (reduction != CDSSM_CE_NONE) loss.fill_(reduction == CDSSM_CE_MEAN ? NAN : 0.0);
-                saved = scratch(0, hidden);
-                return;
-            }
-            const size_t sb = cdssm_b200_linear_ce_saved_bytes(rows, (int)std::min<int64_t>(d, INT32_MAX), (int)std::min<int64_t>(vocab, INT32_MAX), dt);
-            const size_t wb = cdssm_b200_linear_ce_workspace_bytes(rows, (int)std::min<int64_t>(d, INT32_MAX), (int)std::min<int64_t>(vocab, INT32_MAX), dt, 0);
-            if (sb == 0) check(CDSSM_ERR_UNSUPPORTED, "linear_ce_fwd");
-            const Tensor x = row_matrix(hidden, d), w = ce_weight(weight_), y = targets.contiguous(), ws = scratch(wb, hidden);
-            saved = scratch(sb, hidden);
-            check(cdssm_b200_linear_ce_fwd(cptr(x), row_stride(x), cptr(w), row_stride(w), y.const_data_ptr<int64_t>(), fmut(loss), mptr(saved), sb,
-                                           mptr(ws), wb, rows, (int)d, (int)vocab, ignore, (int)reduction, dt, (int)flags, stream_of(x)),
-                  "linear_ce_fwd");
-        });
-        return Py_BuildValue("(NN)", wrap(std::move(loss)), wrap(std::move(saved)));
-    });
-}
-
-// linear_ce_bwd(grad_loss, weight, targets, saved, ignore_index, reduction, want_x, want_w, flags) -> (grad_x (rows, d) or None, grad_w or None)
-PyObject* py_linear_ce_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded([&] {
-        Args in{a, n};
-        const Tensor grad_ = in.tensor("grad_loss"), weight_ = in.tensor("weight"), targets = in.tensor("targets"), saved = in.tensor("saved");
-        const int64_t ignore = in.integer(), reduction = in.integer();
-        const bool want_x = in.flag(), want_w = in.flag();
-        const int64_t flags = in.integer();
-        const int64_t rows = targets.numel(), d = weight_.size(1), vocab = weight_.size(0);
-        const int dt = dtype_code(weight_);
-        Tensor gx, gw;
-        without_gil([&] {
-            const c10::cuda::CUDAGuard guard(weight_.device());
-            if (want_x) gx = empty_like_dims({rows, d}, weight_);
-            if (want_w) gw = rows ? empty_like_dims({vocab, d}, weight_) : at::zeros({vocab, d}, weight_.options());
-            if (rows == 0 || (!want_x && !want_w)) return;
-            const size_t wb = cdssm_b200_linear_ce_workspace_bytes(rows, (int)d, (int)vocab, dt, 1);
-            const Tensor g = grad_.to(at::kFloat).contiguous(), w = ce_weight(weight_), y = targets.contiguous(), ws = scratch(wb, weight_);
-            check(cdssm_b200_linear_ce_bwd(fptr(g), cptr(w), row_stride(w), y.const_data_ptr<int64_t>(), mptr(saved), (size_t)saved.numel(), mptr(gx),
-                                           mptr(gw), mptr(ws), wb, rows, (int)d, (int)vocab, ignore, (int)reduction, dt, (int)flags, stream_of(w)),
-                  "linear_ce_bwd");
-        });
-        auto give = [](Tensor& t) { return t.defined() ? wrap(std::move(t)) : (Py_INCREF(Py_None), Py_None); };
-        PyObject* x = give(gx);
-        return Py_BuildValue("(NN)", x, give(gw));
-    });
-}
-
-// embedding_fwd(ids (..) int64, weight (vocab, d), scale) -> out (.., d)
-PyObject* py_embedding_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    return guarded([&] {
-        Args in{a, n};
-        const Tensor ids_ = in.tensor("ids"), weight = in.tensor("weight");
-        const float scale = (float)in.number();
-        need_cuda(ids_, "ids");
-        need_cuda(weight, "weight");
-        need_same_device(ids_, weight, "ids");
-        if (ids_.scalar_type() != at::kLong) throw Error("ids must be int64");
-        need_dims(weight, 2, "weight");
-        const int64_t d = weight.size(1), vocab = weight.size(0), count = ids_.numel();
-        if (d < 1 || vocab < 1) throw Error("weight is empty");
-        const int dt = dtype_code(weight);
         return wrap(without_gil([&] {
-            const c10::cuda::CUDAGuard guard(weight.device());
-            auto sizes = ids_.sizes().vec();
-            sizes.push_back(d);
-            const Tensor out = empty_like_dims(sizes, weight);
-            if (count == 0) return out;
-            if (d > INT32_MAX || vocab > INT32_MAX) check(CDSSM_ERR_UNSUPPORTED, "embedding_fwd");
-            const Tensor ids = ids_.contiguous(), w = ce_weight(weight);
-            check(cdssm_b200_embedding_fwd(ids.const_data_ptr<int64_t>(), cptr(w), row_stride(w), mptr(out), count, (int)vocab, (int)d, scale, dt,
-                                           stream_of(w)),
-                  "embedding_fwd");
-            return out;
+            return wants_grad(hidden) || wants_grad(weight) ? CeNode::apply(hidden, weight, targets, ignore, reduction, flags)
+                                                            : ce_forward(hidden, weight, targets, ignore, reduction, flags).loss;
         }));
     });
 }
 
-// embedding_bwd(grad (.., d), ids, vocab, padding_idx (-1: none), scale) -> grad_weight (vocab, d)
-PyObject* py_embedding_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// ---- embedding -----------------------------------------------------------------------------------------
+Tensor embed_forward(const Tensor& ids_, const Tensor& weight, double scale) {
+    const c10::cuda::CUDAGuard guard(weight.device());
+    const int64_t d = weight.size(1), count = ids_.numel();
+    auto sizes = ids_.sizes().vec();
+    sizes.push_back(d);
+    const Tensor out = empty_like_dims(sizes, weight);
+    if (count == 0) return out;
+    const Tensor ids = ids_.contiguous(), w = table(weight);
+    check(cdssm_b200_embedding_fwd(ids.const_data_ptr<int64_t>(), cptr(w), row_stride(w), mptr(out), count, (int)weight.size(0), (int)d, (float)scale,
+                                   dtype_code(weight), stream_of(w)),
+          "embedding");
+    return out;
+}
+Tensor embed_backward(const Tensor& grad_, const Tensor& ids_, int64_t vocab, int64_t d, int64_t padding, double scale) {
+    const c10::cuda::CUDAGuard guard(grad_.device());
+    const int64_t count = ids_.numel();
+    if (count == 0) return at::zeros({vocab, d}, grad_.options());
+    const Tensor out = empty_like_dims({vocab, d}, grad_);
+    const int dt = dtype_code(grad_);
+    const size_t bytes = cdssm_b200_embedding_bwd_workspace_bytes(count, (int)vocab, (int)d, dt);
+    if (bytes == 0) check(CDSSM_ERR_UNSUPPORTED, "embedding backward");
+    Tensor grad = grad_.contiguous();
+    if (reinterpret_cast<uintptr_t>(grad.const_data_ptr()) & 15) grad = grad.clone();
+    const Tensor ids = ids_.contiguous(), ws = scratch(bytes, grad_);
+    check(cdssm_b200_embedding_bwd(ids.const_data_ptr<int64_t>(), cptr(grad), mptr(out), mptr(ws), bytes, count, (int)vocab, (int)d, padding,
+                                   (float)scale, dt, stream_of(grad)),
+          "embedding backward");
+    return out;
+}
+struct EmbedNode : torch::autograd::Function<EmbedNode> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& weight, const Tensor& ids, double scale, int64_t padding) {
+        ctx->save_for_backward({ids});
+        ctx->saved_data["args"] = std::vector<int64_t>{weight.size(0), weight.size(1), padding};
+        ctx->saved_data["scale"] = scale;
+        return embed_forward(ids, weight, scale);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        once_only("embedding");
+        const auto args = ctx->saved_data["args"].toIntVector();
+        return {embed_backward(grads[0], ctx->get_saved_variables()[0], args[0], args[1], args[2], ctx->saved_data["scale"].toDouble()), Tensor(),
+                Tensor(), Tensor()};
+    }
+};
+
+// embedding(ids (..) int64, weight (vocab, d), scale, padding_idx (-1: none)) -> (.., d)
+PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&] {
         Args in{a, n};
-        const Tensor grad_ = in.tensor("grad"), ids_ = in.tensor("ids");
-        const int64_t vocab = in.integer(), padding = in.integer();
-        const float scale = (float)in.number();
-        const int64_t d = grad_.size(-1), count = ids_.numel();
-        return wrap(without_gil([&] {
-            const c10::cuda::CUDAGuard guard(grad_.device());
-            if (count == 0) return at::zeros({vocab, d}, grad_.options());
-            const Tensor out = empty_like_dims({vocab, d}, grad_);
-            const int dt = dtype_code(grad_);
-            const size_t bytes = cdssm_b200_embedding_bwd_workspace_bytes(count, (int)vocab, (int)d, dt);
-            if (bytes == 0) check(CDSSM_ERR_UNSUPPORTED, "embedding_bwd");
-            Tensor grad = grad_.contiguous();
-            if (reinterpret_cast<uintptr_t>(grad.const_data_ptr()) & 15) grad = grad.clone();
-            const Tensor ids = ids_.contiguous(), ws = scratch(bytes, grad_);
-            check(cdssm_b200_embedding_bwd(ids.const_data_ptr<int64_t>(), cptr(grad), mptr(out), mptr(ws), bytes, count, (int)vocab, (int)d, padding,
-                                           scale, dt, stream_of(grad)),
-                  "embedding_bwd");
-            return out;
-        }));
+        const Tensor ids = in.tensor("ids"), weight = in.tensor("weight");
+        const double scale = in.number();
+        const int64_t padding = in.integer();
+        need_cuda(ids, "ids");
+        need_table(weight, "weight");
+        need_same_device(ids, weight, "ids");
+        if (ids.scalar_type() != at::kLong) throw Error("ids must be int64");
+        if (padding < -1 || padding >= weight.size(0)) throw Error("padding_idx " + std::to_string(padding) + " is no row of the table");
+        return wrap(without_gil([&] { return wants_grad(weight) ? EmbedNode::apply(weight, ids, scale, padding) : embed_forward(ids, weight, scale); }));
     });
 }
 
+// ---- gradient norm ---------------------------------------------------------------------------------------
 // Tensors as the kernels walk them: every value once, in the order of memory.
 void need_dense(const Tensor& t, const char* name) {
     need_cuda(t, name);
@@ -247,10 +276,8 @@ PyObject* py_grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FAST(fn) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fn)), METH_FASTCALL, nullptr
 PyMethodDef g_ends_methods[] = {
-    {"linear_ce_fwd", FAST(py_linear_ce_fwd)},
-    {"linear_ce_bwd", FAST(py_linear_ce_bwd)},
-    {"embedding_fwd", FAST(py_embedding_fwd)},
-    {"embedding_bwd", FAST(py_embedding_bwd)},
+    {"linear_cross_entropy", FAST(py_linear_cross_entropy)},
+    {"embedding", FAST(py_embedding)},
     {"grad_clip", FAST(py_grad_clip)},
     {nullptr, nullptr, 0, nullptr},
 };

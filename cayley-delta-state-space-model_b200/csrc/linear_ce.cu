@@ -30,7 +30,7 @@ using namespace sm100;
 
 constexpr int kM = 256, kN = 256, kK = 64;              // rows and columns of a pair's tile, depth of a stage
 constexpr int kHalf = 128;                              // of either, a block's
-constexpr int kStages = 6;
+constexpr int kStages = 7;
 constexpr int kEpilogueWarps = 8, kThreads = 128 + 32 * kEpilogueWarps;
 constexpr int kTmemCols = 2 * kN;
 
@@ -59,6 +59,8 @@ struct Args {
     int Tp, d, V;
     int run, n_tiles, n_runs;    // forward: tiles of a run, tiles and runs of a row
     int v0, vn, vn_tiles;        // backward: first word and words of the piece
+    __nv_bfloat16* dz;           // (dz_planes, Tp, dz_pitch)
+    int dz_pitch;
     void *dx, *dw;
     float* acc;                  // (Tp, acc_pitch) dx of the pieces before, summed
     int acc_pitch, d_tiles, f32, first, last, vec_dx, vec_dw;
@@ -71,7 +73,6 @@ struct Args {
 struct __align__(1024) Smem {
     uint8_t a[kStages][kHalf * kK * 2];
     uint8_t b[kStages][kHalf * kK * 2];
-    uint8_t out[kEpilogueWarps][4096];
     // full and acc_empty: of both blocks, the first one's; empty and acc_full: arrived at in both by the first one's products
     uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
     uint32_t tmem_base;
@@ -252,14 +253,13 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, uin
         "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
         : "memory");
 }
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, const void* src, int c0, int c1, int c2) {
-    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(reinterpret_cast<uint64_t>(m)),
-                 "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2)
+// 32 bytes of one row: a whole sector of DRAM.  dz goes out of registers straight: shared memory is what the products' operands fill (its
+// way in and out there cost a tenth of the kernel).
+__device__ __forceinline__ void store_sector(void* p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
                  : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // Where block k of a tile's kt stands: its place in the depth, its part product, and whether a fold ends with it.
 struct Place {
@@ -272,7 +272,7 @@ __device__ __forceinline__ Place place(const Args& a, int k, int kt) {
     return {c * a.group + r - t * n, t, a.folds && r + 1 == n * a.terms};
 }
 
-struct Maps {   // kStats, kGradLogits: a x, b W, out dz; kGradProducts: (a dz, b W) for dx, (a2 dz, b2 x) for dW
+struct Maps {   // kStats, kGradLogits: a x, b W; kGradProducts: (a dz, b W) for dx, (a2 dz, b2 x) for dW
     CUtensorMap a, b, a2, b2;
 };
 
@@ -434,7 +434,7 @@ __device__ __forceinline__ size_t slot_at(int slot, int warp, int chunk, int j4,
 
 // kFold: the tile's sums come in folds and are added up here, in 128 registers a thread; else they are read from tensor memory as used.
 template <int kMode, bool kFold>
-__device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, const Args& a, int count) {
+__device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
     volatile int* ab = &sm.abort_flag;
     auto walk = make_walk<kMode>(a, count);
     Segment s;
@@ -552,29 +552,23 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
                         if (v0 + j >= a.V) z[j] = 0.f;
                 }
                 const bool live = row < count;
-                uint8_t* const mine = sm.out[warp];
 #pragma unroll 1
                 for (int p = 0; p < a.dz_planes; p++) {
-                    if (lane == 0) tma_store_wait_read();
-                    __syncwarp();
+                    __nv_bfloat16* const to = a.dz + ((size_t)p * a.Tp + row) * a.dz_pitch + col;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        uint4 u = {pack2(z[8 * j], z[8 * j + 1]), pack2(z[8 * j + 2], z[8 * j + 3]), pack2(z[8 * j + 4], z[8 * j + 5]),
-                                   pack2(z[8 * j + 6], z[8 * j + 7])};
-                        if (!live) u = {0, 0, 0, 0};
-                        *reinterpret_cast<uint4*>(mine + lane * 128 + ((j ^ (lane & 7)) << 4)) = u;
-                        if (p + 1 < a.dz_planes) {          // what the rounding has left
-                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                    for (int j = 0; j < 64; j += 16) {
+                        uint32_t w[8];
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                z[8 * j + 2 * e] -= __uint_as_float(w[e] << 16);
-                                z[8 * j + 2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
+                        for (int e = 0; e < 8; e++) w[e] = live ? pack2(z[j + 2 * e], z[j + 2 * e + 1]) : 0u;
+                        store_sector(to + j, w);
+                        if (p + 1 < a.dz_planes) {       // what the rounding has left
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                z[j + 2 * e] -= __uint_as_float(w[e] << 16);
+                                z[j + 2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
                             }
                         }
                     }
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) tma_store_3d(map_out, mine, col, s.m * kM + rank * kHalf + quarter * 32, p);
                 }
             }
         } else {
@@ -603,13 +597,12 @@ __device__ __forceinline__ bool finish(Smem& sm, const CUtensorMap* map_out, con
             sum = 0.f;
         }
     }
-    if (kMode == kGradLogits && lane == 0) tma_store_wait();
     return true;
 }
 
 template <int kMode, bool kFold>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtensorMap map_out, const Args a) {
+product_kernel(const __grid_constant__ Maps maps, const Args a) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
     const int warp = threadIdx.x >> 5;
@@ -629,19 +622,22 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
     __syncthreads();
     cluster_sync();
     tc_fence_after();
+    grid_launch_dependents();
+    grid_dependency_wait();
     const int count = *a.count;
     bool ok = true;
     // (a warpgroup's registers: 128 x 40 + 256 x 232 are the 384 x 168 of the launch)
     if (warp < 4) {
         if constexpr (kFold) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0) {
+            asm volatile("fence.proxy.async.global;" ::: "memory");   // packed rows and dz were plain stores; TMA reads them
             if ((threadIdx.x & 31) == 0 && !a.withhold) ok = produce<kMode>(sm, maps, a, count);
         } else if (warp == 1 && block_rank() == 0) {
             ok = multiply<kMode>(sm, a, count);
         }
     } else {
         if constexpr (kFold) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-        ok = finish<kMode, kFold>(sm, &map_out, a, count);
+        ok = finish<kMode, kFold>(sm, a, count);
     }
     if (!ok) atomicCAS(a.status, 0, 400 + warp);
     __syncwarp();
@@ -659,6 +655,8 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ CUtens
 // Sums the shares of the tiles that were split, in the order of their depth, and hands them out.  Block (boundary, group of
 // eight warps' chunks); the first boundary inside a tile does it.  grid: pairs of the launch before.
 __global__ void __launch_bounds__(256) join_split_kernel(const Args a, int grid) {
+    grid_launch_dependents();
+    grid_dependency_wait();
     const int count = *a.count, p = (int)blockIdx.x + 1, lane = threadIdx.x & 31, id = blockIdx.y * 8 + (threadIdx.x >> 5);
     const int warp = id >> 2, chunk = id & 3;
     const SplitTiles t = split_tiles(a, count, grid);
@@ -703,6 +701,8 @@ index_rows_kernel(const int64_t* __restrict__ target, int64_t ignore, int64_t n_
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t base = (int64_t)blockIdx.x * kIndexThreads;
     int n = 0;
+    grid_launch_dependents();
+    grid_dependency_wait();
     for (int64_t i = tid; i < base; i += kIndexThreads) n += target[i] != ignore;
     n = __reduce_add_sync(~0u, n);
     const int64_t t = base + tid;
@@ -757,6 +757,8 @@ pack_rows_kernel(const T* __restrict__ x, int64_t stride, const int* __restrict_
                  int pitch, __nv_bfloat16* __restrict__ out, int vec) {
     const int lane = threadIdx.x & 31;
     const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    grid_launch_dependents();
+    grid_dependency_wait();
     if (r >= n_rows || (count && r >= (int64_t)row_tiles(*count) * kM)) return;
     const int64_t from = rows ? rows[r] : r;
     const T* const src = x + (from < 0 ? 0 : from) * stride;
@@ -783,17 +785,21 @@ pack_rows_kernel(const T* __restrict__ x, int64_t stride, const int* __restrict_
     }
 }
 
-// Joins the runs of a row: m, 1 / s and the loss, and (not kRows) the losses' sum or mean: every block leaves its sum, the last one to
-// come adds them up in their order.  A lane per row, a warp per eighth of the runs.
-constexpr int kJoinWarps = 8;
-__global__ void __launch_bounds__(32 * kJoinWarps)
+// Joins the runs of a row: m, 1 / s and the loss, and (mean, sum) the losses' sum: every block leaves its own, the last one to come adds
+// them up in their order.  Eight rows a block, 32 threads a row: a call of few rows has few of them and hundreds of runs each (400 runs of
+// 61 rows with a thread per row and eighth of the runs: 28 us).
+constexpr int kJoinRows = 8;
+__global__ void __launch_bounds__(256)
 join_runs_kernel(const float2* __restrict__ part, int n_parts, int Tp, int* header, const int* __restrict__ rows, const int* __restrict__ words,
                  float* __restrict__ row_max, float* __restrict__ row_inv, const float* __restrict__ hit, float* __restrict__ loss, int reduction,
                  double* __restrict__ sums) {
-    __shared__ float2 join[kJoinWarps][32];
-    __shared__ double warp_sum[kJoinWarps];
+    __shared__ float2 join[8][kJoinRows];
+    __shared__ double warp_sum[8];
     __shared__ bool is_last;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.x * 32 + lane, count = header[0];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.x * kJoinRows + (tid & 7);
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int count = header[0];
     const bool failed = header[1] != 0;
     float top = -INFINITY, sum = 0.f;
     auto add = [&](float2 p) {
@@ -801,27 +807,40 @@ join_runs_kernel(const float2* __restrict__ part, int n_parts, int Tp, int* head
         sum = sum * ex2((top - ref) * kLog2e) + p.y * ex2((p.x - ref) * kLog2e);
         top = best;
     };
-    if (r < count)
-        for (int i = warp; i < n_parts; i += kJoinWarps) add(part[(size_t)i * Tp + r]);
-    join[warp][lane] = make_float2(top, sum);
+    if (r < count) {
+        constexpr int kAhead = 4;
+        for (int i = tid >> 3; i < n_parts; i += 32 * kAhead) {
+            float2 p[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) p[k] = i + 32 * k < n_parts ? __ldg(part + (size_t)(i + 32 * k) * Tp + r) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) add(p[k]);
+        }
+    }
+#pragma unroll
+    for (int o = 8; o < 32; o <<= 1) {
+        const float2 p = {__shfl_down_sync(~0u, top, o), __shfl_down_sync(~0u, sum, o)};
+        add(p);
+    }
+    if (lane < kJoinRows) join[warp][lane] = make_float2(top, sum);
     __syncthreads();
     double mine = 0.0;
     if (warp == 0) {
-        if (r < count) {
+        if (lane < kJoinRows && r < count) {
             top = -INFINITY;
             sum = 0.f;
-            for (int i = 0; i < kJoinWarps; i++) add(join[i][lane]);
+            for (int i = 0; i < 8; i++) add(join[i][lane]);
             row_max[r] = top;
             row_inv[r] = 1.f / sum;
             // (a row without any logit that is a number: NaN, as exp(-inf - -inf))
-            float l = words[r] == -2 || failed || top == -INFINITY ? NAN : (top - hit[r]) + logf(sum);
+            const float l = words[r] == -2 || failed || top == -INFINITY ? NAN : (top - hit[r]) + logf(sum);
             if (reduction == CDSSM_CE_NONE) loss[rows[r]] = l;
             mine = (double)l;
         }
-        for (int o = 16; o; o >>= 1) mine += __shfl_down_sync(~0u, mine, o);
+        for (int o = 4; o; o >>= 1) mine += __shfl_down_sync(~0u, mine, o);
     }
     if (reduction == CDSSM_CE_NONE) return;
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         sums[blockIdx.x] = mine;
         __threadfence();
         is_last = atomicAdd(&header[2], 1) + 1 == (int)gridDim.x;
@@ -830,13 +849,13 @@ join_runs_kernel(const float2* __restrict__ part, int n_parts, int Tp, int* head
     if (!is_last) return;
     __threadfence();
     double total = 0.0;
-    for (int i = threadIdx.x; i < (int)gridDim.x; i += 32 * kJoinWarps) total += __ldcg(&sums[i]);
+    for (int i = tid; i < (int)gridDim.x; i += 256) total += __ldcg(&sums[i]);
     for (int o = 16; o; o >>= 1) total += __shfl_down_sync(~0u, total, o);
     if (lane == 0) warp_sum[warp] = total;
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
         total = 0.0;
-        for (int i = 0; i < kJoinWarps; i++) total += warp_sum[i];
+        for (int i = 0; i < 8; i++) total += warp_sum[i];
         *loss = (float)(reduction == CDSSM_CE_MEAN ? total / (double)count : total);   // (mean of no rows: NaN)
     }
 }
@@ -846,6 +865,8 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 blank_rows_kernel(const int64_t* __restrict__ target, int64_t ignore, int64_t n_rows, int d, const int* __restrict__ header, T* __restrict__ dx) {
     const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    grid_launch_dependents();
+    grid_dependency_wait();
     if (r >= n_rows) return;
     const bool failed = header[1] != 0;
     if (!failed && target[r] != ignore) return;
@@ -895,7 +916,7 @@ bool sizes_of(int64_t rows, int d, int vocab, int dtype, int sms, Sizes& s) {
     s.saved = o;
     s.w_planes = up(2ull * s.planes * (size_t)vocab * s.pitch, 256);
     o = s.w_planes;
-    s.o_part = take(8ull * 2 * s.n_runs * s.Tp); s.o_sums = take(8ull * (s.Tp / 32));
+    s.o_part = take(8ull * 2 * s.n_runs * s.Tp); s.o_sums = take(8ull * (s.Tp / kJoinRows));
     s.fwd = o;
     o = s.w_planes;
     s.o_dz = take(column * s.vn); s.o_acc = take(s.pieces > 1 ? 4ull * s.Tp * s.d_tiles * kN : 0);
@@ -925,18 +946,17 @@ bool make_map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int 
 
 template <int kMode, bool kFold> struct Tag {};
 template <int kMode, bool kFold>
-int launch_as(const Maps& maps, const CUtensorMap& out, const Args& a, int grid, cudaStream_t st) {
+int launch_as(const Maps& maps, const Args& a, int grid, cudaStream_t st) {
     if (int rc = allow_smem<Tag<kMode, kFold>>((const void*)product_kernel<kMode, kFold>, sizeof(Smem))) return rc;
-    product_kernel<kMode, kFold><<<grid, kThreads, sizeof(Smem), st>>>(maps, out, a);
-    return check_launch();
+    return launch_overlapped(product_kernel<kMode, kFold>, dim3(grid), dim3(kThreads), sizeof(Smem), st, maps, a);
 }
 template <int kMode>
-int launch_products(const Maps& maps, const CUtensorMap& out, Args a, int grid, cudaStream_t st) {
+int launch_products(const Maps& maps, Args a, int grid, cudaStream_t st) {
     a.terms = a.planes == 3 ? kTerms3 : kMode == kGradProducts ? a.dz_planes : 1;
     // (two parts of dz: block by block, so that the other operand's comes from L2 the second time)
     a.group = a.planes == 3 ? kFold3 : kMode == kGradProducts ? 1 : kFoldLogits;
     a.folds = a.planes == 3 || (kMode != kGradProducts && a.group * kK < a.d);
-    return a.folds ? launch_as<kMode, true>(maps, out, a, grid, st) : launch_as<kMode, false>(maps, out, a, grid, st);
+    return a.folds ? launch_as<kMode, true>(maps, a, grid, st) : launch_as<kMode, false>(maps, a, grid, st);
 }
 
 bool in_place(const void* w, int64_t stride, int dtype) {   // a matrix that TMA reads as it lies
@@ -945,9 +965,8 @@ bool in_place(const void* w, int64_t stride, int dtype) {   // a matrix that TMA
 
 template <typename T, int kPlanes>
 int pack(const void* x, int64_t stride, const int* rows, const int* count, int64_t n, const Sizes& s, void* out, bool vec, cudaStream_t st) {
-    pack_rows_kernel<T, kPlanes><<<(unsigned)((n + 7) / 8), 256, 0, st>>>(static_cast<const T*>(x), stride, rows, count, n, s.d, s.pitch,
-                                                                          static_cast<__nv_bfloat16*>(out), vec);
-    return check_launch();
+    return launch_overlapped(pack_rows_kernel<T, kPlanes>, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, static_cast<const T*>(x), stride, rows,
+                             count, n, s.d, s.pitch, static_cast<__nv_bfloat16*>(out), vec);
 }
 int pack_any(const void* x, int64_t stride, const int* rows, const int* count, int64_t n, const Sizes& s, void* out, cudaStream_t st) {
     if (s.f32) return pack<float, 3>(x, stride, rows, count, n, s, out, false, st);
@@ -1000,10 +1019,10 @@ extern "C" int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, con
     ce::Args a;
     ce::fill_saved(a, s, sv);
     int* header = reinterpret_cast<int*>(sv);
-    ce::index_rows_kernel<<<(unsigned)((rows + ce::kIndexThreads - 1) / ce::kIndexThreads), ce::kIndexThreads, 0, st>>>(
-        target, ignore_index, rows, s.Tp, vocab, header, const_cast<int*>(a.rows), const_cast<int*>(a.target),
-        reduction == CDSSM_CE_NONE ? loss : nullptr);
-    if (int rc = check_launch()) return rc;
+    if (int rc = launch_overlapped(ce::index_rows_kernel, dim3((unsigned)((rows + ce::kIndexThreads - 1) / ce::kIndexThreads)),
+                                   dim3(ce::kIndexThreads), 0, st, target, ignore_index, rows, s.Tp, vocab, header, const_cast<int*>(a.rows),
+                                   const_cast<int*>(a.target), reduction == CDSSM_CE_NONE ? loss : nullptr))
+        return rc;
     if (int rc = ce::pack_any(x, x_row_stride, a.rows, a.count, s.Tp, s, sv + s.o_x, st)) return rc;
     const bool direct = ce::in_place(w, w_row_stride, dtype);
     if (!direct)
@@ -1015,10 +1034,9 @@ extern "C" int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, con
     a.part = reinterpret_cast<float2*>(ws + s.o_part);
     a.withhold = (flags & CDSSM_SCAN_TEST_WITHHOLD) != 0;
     const int64_t units = (int64_t)(s.Tp / ce::kM) * s.n_runs;
-    if (int rc = ce::launch_products<ce::kStats>(maps, maps.a, a, 2 * (int)std::min<int64_t>(units, sms / 2), st)) return rc;
-    ce::join_runs_kernel<<<s.Tp / 32, 32 * ce::kJoinWarps, 0, st>>>(a.part, 2 * s.n_runs, s.Tp, header, a.rows, a.target, a.row_max, a.row_inv,
-                                                                  a.hit, loss, reduction, reinterpret_cast<double*>(ws + s.o_sums));
-    return check_launch();
+    if (int rc = ce::launch_products<ce::kStats>(maps, a, 2 * (int)std::min<int64_t>(units, sms / 2), st)) return rc;
+    return launch_overlapped(ce::join_runs_kernel, dim3(s.Tp / ce::kJoinRows), dim3(256), 0, st, a.part, 2 * s.n_runs, s.Tp, header, a.rows, a.target,
+                             a.row_max, a.row_inv, a.hit, loss, reduction, reinterpret_cast<double*>(ws + s.o_sums));
 }
 
 extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, int64_t w_row_stride, const int64_t* target, void* saved,
@@ -1040,10 +1058,8 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
     const void* const wb = direct ? w : ws;
     const int64_t w_cols = direct ? d : s.pitch, w_pitch = direct ? w_row_stride : s.pitch;
     ce::Maps logits{}, grads{};
-    CUtensorMap dz;
     if (!ce::make_map(&logits.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, ce::kHalf) ||
         !ce::make_map(&logits.b, wb, w_cols, vocab, s.planes, w_pitch, ce::kK, ce::kHalf) ||
-        !ce::make_map(&dz, ws + s.o_dz, s.vn, s.Tp, s.dz_planes, s.vn, 64, 32) ||
         !ce::make_map(&grads.a, ws + s.o_dz, s.vn, s.Tp, s.dz_planes, s.vn, ce::kK, ce::kHalf) ||
         !ce::make_map(&grads.b, wb, w_cols, vocab, s.planes, w_pitch, 64, ce::kK) ||
         !ce::make_map(&grads.a2, ws + s.o_dz, s.vn, s.Tp, s.dz_planes, s.vn, 64, ce::kK) ||
@@ -1055,6 +1071,8 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
     a.grad_rows = reduction == CDSSM_CE_NONE;
     a.mean = reduction == CDSSM_CE_MEAN;
     a.dx = grad_x; a.dw = grad_w;
+    a.dz = reinterpret_cast<__nv_bfloat16*>(ws + s.o_dz);
+    a.dz_pitch = s.vn;
     a.acc = reinterpret_cast<float*>(ws + s.o_acc);
     a.acc_pitch = s.d_tiles * ce::kN;
     a.slots = reinterpret_cast<float4*>(ws + s.o_slots);
@@ -1065,17 +1083,18 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
         a.vn_tiles = (a.vn + ce::kN - 1) / ce::kN;
         a.first = p == 0;
         a.last = p + 1 == s.pieces;
-        if (int rc = ce::launch_products<ce::kGradLogits>(logits, dz, a, sms / 2 * 2, st)) return rc;
-        if (int rc = ce::launch_products<ce::kGradProducts>(grads, dz, a, sms / 2 * 2, st)) return rc;
+        if (int rc = ce::launch_products<ce::kGradLogits>(logits, a, sms / 2 * 2, st)) return rc;
+        if (int rc = ce::launch_products<ce::kGradProducts>(grads, a, sms / 2 * 2, st)) return rc;
         a.terms = s.f32 ? ce::kTerms3 : s.dz_planes;
-        ce::join_split_kernel<<<dim3(sms / 2, 8), 256, 0, st>>>(a, sms / 2);
-        if (int rc = check_launch()) return rc;
+        if (int rc = launch_overlapped(ce::join_split_kernel, dim3(sms / 2, 8), dim3(256), 0, st, a, sms / 2)) return rc;
     }
     if (grad_x) {
         const unsigned grid = (unsigned)((rows + 7) / 8);
-        if (s.f32) ce::blank_rows_kernel<<<grid, 256, 0, st>>>(target, ignore_index, rows, d, a.count, static_cast<float*>(grad_x));
-        else ce::blank_rows_kernel<<<grid, 256, 0, st>>>(target, ignore_index, rows, d, a.count, static_cast<__nv_bfloat16*>(grad_x));
-        if (int rc = check_launch()) return rc;
+        if (int rc = s.f32 ? launch_overlapped(ce::blank_rows_kernel<float>, dim3(grid), dim3(256), 0, st, target, ignore_index, rows, d, a.count,
+                                               static_cast<float*>(grad_x))
+                           : launch_overlapped(ce::blank_rows_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, st, target, ignore_index, rows, d, a.count,
+                                               static_cast<__nv_bfloat16*>(grad_x)))
+            return rc;
     }
     return CDSSM_OK;
 }

@@ -14,7 +14,6 @@ fallback: tensors must be CUDA tensors and the library must be built.
 import torch
 from torch import Tensor
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import CdssmError, check
@@ -22,7 +21,7 @@ from ._lib import CdssmError, check
 __all__ = ["CUDAConv1dSiLUOp", "DynamicsFusedFn", "NormalizeKQFn", "IntraChunkScanFn",
            "InterChunkScanFn", "ExactCorrectionFn", "scan_fused", "decode_step", "decode_step_reference", "reference_decode_state",
            "scan_fused_workspace_bytes", "scan_fused_status", "set_wait_limit_ns", "selftest_bounded_wait", "rms_norm", "groupnorm_gate", "conv1d_silu_step", "scan_summary", "scan_fused_long", "compose_carries",
-           "EmbeddingFn", "embedding", "LinearCrossEntropyFn", "linear_cross_entropy", "grad_norm", "clip_grads_", "clip_grad_norm_",
+           "embedding", "linear_cross_entropy", "grad_norm", "clip_grads_", "clip_grad_norm_",
            "CdssmError"]
 
 _DT = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
@@ -173,64 +172,20 @@ class ExactCorrectionFn(Function):
 # ------------------------------------------------------------------------------------------
 # The ends of a training step
 # ------------------------------------------------------------------------------------------
-class EmbeddingFn(Function):
-    """Rows of a table for token ids, scaled: see :func:`embedding`."""
-
-    @staticmethod
-    def forward(ctx, ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: int = None) -> Tensor:
-        padding = -1 if padding_idx is None else int(padding_idx)
-        if padding_idx is not None and not 0 <= padding < weight.shape[0]:
-            raise CdssmError(f"padding_idx {padding_idx} is no row of the table")
-        ctx.args = (weight.shape[0], padding, float(scale))
-        out = _lib.host().embedding_fwd(ids, weight, scale)
-        ctx.save_for_backward(ids)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out):
-        """(None, grad_weight, None, None)"""
-        ids, = ctx.saved_tensors
-        return None, _lib.host().embedding_bwd(grad_out, ids, *ctx.args), None, None
-
-
 def embedding(ids: Tensor, weight: Tensor, *, scale: float = 1.0, padding_idx: int = None) -> Tensor:
     """scale * weight[ids] (cdssm/models/model.py:46): ids (...) int64, weight (vocab, d) bfloat16 or float32 -> (..., d).
 
     The gradient (vocab, d) is dense, in the weight's type; the rows of one id are added up in float32 in the order of the tokens and
     rounded once, the same bits from run to run; ``padding_idx``'s row gets none.  An id that is no row of the table (negative ones too)
     gives a row of NaN and takes no part in the gradient.  Differentiable once."""
-    return EmbeddingFn.apply(ids, weight, scale, padding_idx)
+    return _lib.host().embedding(ids, weight, scale, -1 if padding_idx is None else padding_idx)
 
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
-class LinearCrossEntropyFn(Function):
-    """Softmax cross entropy of hidden rows against a vocabulary, without the logits: see :func:`linear_cross_entropy`."""
-
-    @staticmethod
-    def forward(ctx, hidden: Tensor, weight: Tensor, targets: Tensor, ignore_index: int = -100, reduction: str = "mean",
-                flags: int = 0) -> Tensor:
-        if reduction not in _REDUCTIONS:
-            raise CdssmError(f"reduction must be 'none', 'mean' or 'sum', not {reduction!r}")
-        ctx.args = (int(ignore_index), _REDUCTIONS[reduction])
-        ctx.hidden_shape, ctx.flags = hidden.shape, int(flags)
-        loss, saved = _lib.host().linear_ce_fwd(hidden, weight, targets, *ctx.args, ctx.flags)
-        ctx.save_for_backward(weight, targets, saved)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_loss):
-        """(grad_hidden, grad_weight, None x 4)"""
-        weight, targets, saved = ctx.saved_tensors
-        gx, gw = _lib.host().linear_ce_bwd(grad_loss, weight, targets, saved, *ctx.args, *ctx.needs_input_grad[:2], ctx.flags)
-        return (None if gx is None else gx.view(ctx.hidden_shape), gw) + (None,) * 4
-
-
 def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ignore_index: int = -100,
-                         reduction: str = "mean") -> Tensor:
+                         reduction: str = "mean", flags: int = 0) -> Tensor:
     """Cross entropy of ``hidden @ weight.T`` against ``targets``: the LM head and the loss of a training step in one
     (cdssm/models/model.py:50-51, cdssm/training/trainer.py:219-262), with the (tokens, vocabulary) logits and their gradient never
     in memory as a whole.
@@ -241,7 +196,9 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
     reduction "mean" (NaN when every row is ignored), "sum" or "none" (targets' shape); the loss is float32.
     Products are bfloat16 ones with float32 sums, for float32 operands exact to 24 bits; the logits' gradient is rounded once to the
     products' type.  Gradients have the operands' type and are the same from run to run.  Differentiable once."""
-    return LinearCrossEntropyFn.apply(hidden, weight, targets, ignore_index, reduction)
+    if reduction not in _REDUCTIONS:
+        raise CdssmError(f"reduction must be 'none', 'mean' or 'sum', not {reduction!r}")
+    return _lib.host().linear_cross_entropy(hidden, weight, targets, ignore_index, _REDUCTIONS[reduction], flags)
 
 
 def grad_norm(grads) -> Tensor:
