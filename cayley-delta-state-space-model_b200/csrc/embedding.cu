@@ -249,13 +249,14 @@ join_tiles_kernel(const uint2* __restrict__ pairs, int n, const float* __restric
     for (long long item = blockIdx.x; item < items; item += gridDim.x) {
         const int tile_id = spans[1 + item / chunks], c = ((int)(item % chunks) * 32 + lane) * kE;
         const unsigned id = pairs[(size_t)tile_id * kTile + kTile - 1].x;
-        int lo = (tile_id + 1) * kTile, hi = n;              // first pair of another id
-        while (lo < hi) {
-            const int mid = lo + (hi - lo) / 2;
-            if (pairs[mid].x == id) lo = mid + 1;
-            else hi = mid;
+        int tiles = 1;                                       // that begin with the id
+        for (bool on = true; on;) {
+            const long long p = ((long long)tile_id + tiles + threadIdx.x) * kTile;
+            const int more = __syncthreads_count(p < n && pairs[p].x == id);
+            tiles += more;
+            on = more == 32 * kJoinParts;
         }
-        const int tiles = (lo - 1) / kTile - tile_id + 1, share = (tiles + kJoinParts - 1) / kJoinParts, q0 = y * share, q1 = min(tiles, q0 + share);
+        const int share = (tiles + kJoinParts - 1) / kJoinParts, q0 = y * share, q1 = min(tiles, q0 + share);
         float sum[kE] = {};
         if (c < d) {
 #pragma unroll 8

@@ -19,6 +19,8 @@
 #include "sm100_ptx.cuh"
 #include "tile_map.cuh"
 #include <cuda_bf16.h>
+#include <algorithm>
+#include <type_traits>
 
 namespace cdssm {
 
@@ -51,13 +53,13 @@ struct Args {
     const int* target;           // (Tp) its word, -2: outside of the vocabulary
     float *row_max, *row_inv;    // (Tp) m and 1 / s
     float* hit;                  // (Tp) z of the target
-    float2* part;                // (runs x 2, Tp) maximum and sum of a run of tiles
+    float2* part;                // (2 x runs, Tp) maximum and sum of a run of tiles, of either half of its columns
     const float* grad;           // upstream gradient: one value, or one a row of the caller
     int grad_rows, mean;
     int planes, dz_planes;
     int terms, group, folds;     // part products; depth blocks that go through all of them together; whether a group's sum is folded
     int Tp, d, V;
-    int run, n_tiles, n_runs;    // forward: tiles of a run, tiles and runs of a row
+    int n_tiles;                 // forward: vocabulary tiles
     int v0, vn, vn_tiles;        // backward: first word and words of the piece
     __nv_bfloat16* dz;           // (dz_planes, Tp, dz_pitch)
     int dz_pitch;
@@ -104,18 +106,36 @@ struct Segment {
 
 __device__ __forceinline__ int row_tiles(int count) { return max(1, (count + kM - 1) / kM); }
 
-// Forward and dz: a run of vocabulary tiles of one row tile is a pair's unit.  Row tiles change fastest, so the pairs that run
-// beside each other read the same rows of W and every row of W leaves DRAM about once.
 __device__ __forceinline__ int pair_id() { return blockIdx.x >> 1; }
 __device__ __forceinline__ int pairs() { return gridDim.x >> 1; }
 
+// Vocabulary tiles of a run: the fewest rounds of tiles, and among those few runs, whose sums have to be joined (5000 of them take as long as
+// a tile).
+constexpr int kMostRun = 8;
+__device__ __forceinline__ int best_run(int row_tiles, int n_tiles, int pairs) {
+    int best = 1;
+    float least = INFINITY;
+    for (int run = 1; run <= kMostRun; run++) {
+        const int units = row_tiles * ((n_tiles + run - 1) / run);
+        const float cost = (float)((units + pairs - 1) / pairs * min(run, n_tiles)) + (float)units * 2e-4f;
+        if (cost < least) {
+            least = cost;
+            best = run;
+        }
+    }
+    return best;
+}
+
+// Forward and dz: a run of vocabulary tiles of one row tile is a pair's unit.  Row tiles change fastest, so the pairs that
+// run beside each other read the same rows of W and every row of W leaves DRAM about once.
 struct RunWalk {
     int unit, units, mt, run_len, n_tiles, kt, n, n_end, m, run;
-    __device__ RunWalk(const Args& a, int count, int n_tiles_, int run_len_) : run_len(run_len_), n_tiles(n_tiles_) {
+    __device__ RunWalk(const Args& a, int count, int n_tiles_) : n_tiles(n_tiles_) {
         mt = row_tiles(count);
+        run_len = best_run(mt, n_tiles, pairs());
         units = mt * ((n_tiles + run_len - 1) / run_len);
         kt = (a.d + kK - 1) / kK * a.terms;
-        unit = (int)pair_id() - (int)pairs();
+        unit = pair_id() - pairs();
         n = n_end = 0;
     }
     __device__ bool next(Segment& s) {
@@ -195,7 +215,7 @@ template <> struct WalkOf<kGradProducts> { using type = SplitWalk; };
 template <int kMode>
 __device__ __forceinline__ typename WalkOf<kMode>::type make_walk(const Args& a, int count) {
     if constexpr (kMode == kGradProducts) return SplitWalk(a, count);
-    else return RunWalk(a, count, kMode == kStats ? a.n_tiles : a.vn_tiles, a.run);
+    else return RunWalk(a, count, kMode == kStats ? a.n_tiles : a.vn_tiles);
 }
 
 // ---- pairs of blocks ---------------------------------------------------------------------------
@@ -261,15 +281,34 @@ __device__ __forceinline__ void store_sector(void* p, const uint32_t (&w)[8]) {
                  : "memory");
 }
 
-// Where block k of a tile's kt stands: its place in the depth, its part product, and whether a fold ends with it.
-struct Place {
-    int kc, term;
-    bool ends;
+// The depth blocks of a segment one by one: place in the depth, part product, and whether a fold ends with the block.  (With divisions in
+// every step of producer and products, float32 ran at half of its speed.)
+struct Steps {
+    int depth, terms, group;
+    int base, n, i, term;   // of the present group: where it begins, its blocks, the block, the part product
+    __device__ Steps(const Args& a, int k0, int kt) : terms(a.terms), group(a.group) {
+        depth = terms == 1 ? kt : kt / terms;
+        const int g = k0 / (group * terms), r = k0 - g * group * terms;
+        base = g * group;
+        n = min(group, depth - base);
+        term = terms == 1 ? 0 : r / n;
+        i = r - term * n;
+    }
+    __device__ int kc() const { return base + i; }
+    __device__ bool next() {   // true: the block before was the last of its group
+        if (++i < n) return false;
+        i = 0;
+        if (++term < terms) return false;
+        term = 0;
+        base += group;
+        n = min(group, depth - base);
+        return true;
+    }
 };
-__device__ __forceinline__ Place place(const Args& a, int k, int kt) {
-    if (a.terms == 1) return {k, 0, a.folds && (k + 1) % a.group == 0};
-    const int depth = kt / a.terms, per = a.group * a.terms, c = k / per, r = k - c * per, n = min(a.group, depth - c * a.group), t = r / n;
-    return {c * a.group + r - t * n, t, a.folds && r + 1 == n * a.terms};
+// groups that blocks [k0, k1) touch
+__device__ __forceinline__ int groups_of(const Args& a, const Segment& s) {
+    const int per = a.group * a.terms;
+    return (s.k1 - 1) / per - s.k0 / per + 1;
 }
 
 struct Maps {   // kStats, kGradLogits: a x, b W; kGradProducts: (a dz, b W) for dx, (a2 dz, b2 x) for dW
@@ -286,16 +325,17 @@ __device__ __forceinline__ bool produce(Smem& sm, const Maps& maps, const Args& 
     const int rank = block_rank(), am = rank * kHalf, bn = rank * kHalf;
     const uint32_t full0 = in_first(&sm.full[0]);
     while (walk.next(s)) {
+        Steps steps(a, s.k0, s.kt);
 #pragma unroll 1
         for (int k = s.k0; k < s.k1; k++, it++) {
             const int st = it % kStages;
             if (!mbar_wait_suspend(&sm.empty[st], (it / kStages & 1) ^ 1, ab, a.wait_ns)) return false;
             if (rank == 0) mbar_arrive_expect_tx(&sm.full[st], 2 * 2 * kHalf * kK * 2);
             const uint32_t full = full0 + st * 8;
-            const Place at = place(a, k, s.kt);
             int pa, pb;
-            term_planes(a, kMode == kGradProducts, at.term, pa, pb);
-            const int kc = at.kc * kK;
+            term_planes(a, kMode == kGradProducts, steps.term, pa, pb);
+            const int kc = steps.kc() * kK;
+            steps.next();
             if (kMode != kGradProducts) {
                 tma_load_3d(sm.a[st], &maps.a, full, kc, s.m * kM + am, pa);
                 tma_load_3d(sm.b[st], &maps.b, full, kc, a.v0 + s.n * kN + bn, pb);
@@ -334,6 +374,7 @@ __device__ __forceinline__ bool multiply(Smem& sm, const Args& a, int count) {
         const uint32_t idesc = umma_idesc_bf16(kM, kN, false, false) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
         const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;
         const uint32_t a_lbo = a_mn ? 8192 : 16, b_lbo = b_mn ? 8192 : 16;
+        Steps steps(a, s.k0, s.kt);
         bool begins = true;
 #pragma unroll 1
         for (int k = s.k0; k < s.k1; k++, it++) {
@@ -346,7 +387,7 @@ __device__ __forceinline__ bool multiply(Smem& sm, const Args& a, int count) {
             for (int j = 0; j < kK / 16; j++)
                 pair_umma_elect(tm + acc * kN, da + j * a_step, db + j * b_step, idesc, !begins || j > 0);
             pair_commit_elect(&sm.empty[st]);
-            begins = k + 1 == s.k1 || place(a, k, s.kt).ends;
+            begins = (steps.next() && a.folds) || k + 1 == s.k1;
             if (begins) {
                 pair_commit_elect(&sm.acc_full[acc]);
                 tile++;
@@ -390,7 +431,7 @@ __device__ __forceinline__ void store_row(T* row, int col, int cols, const float
 
 // What all of dz has been left without.
 __device__ __forceinline__ float gradient_factor(const Args& a, int count) {
-    return a.grad_rows ? 1.f : a.mean ? a.grad[0] / (float)count : a.grad[0];
+    return a.grad_rows ? 1.f : a.mean ? a.grad[0] / (float)max(count, 1) : a.grad[0];
 }
 
 // 32 columns of a row of a finished tile of dx or dW.  dx of several pieces is summed in float32 and rounded once, by the last.
@@ -468,8 +509,7 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
         int acc = tile & 1;
         if constexpr (kFold) {
 #pragma unroll 1
-            for (int k = s.k0; k < s.k1; k++) {
-                if (!(k + 1 == s.k1 || place(a, k, s.kt).ends)) continue;
+            for (int k = groups_of(a, s); k > 0; k--) {
                 acc = tile & 1;
                 if (!mbar_wait_suspend(&sm.acc_full[acc], tile >> 1 & 1, ab, a.wait_ns)) return false;
                 tc_fence_after();
@@ -790,7 +830,7 @@ pack_rows_kernel(const T* __restrict__ x, int64_t stride, const int* __restrict_
 // 61 rows with a thread per row and eighth of the runs: 28 us).
 constexpr int kJoinRows = 8;
 __global__ void __launch_bounds__(256)
-join_runs_kernel(const float2* __restrict__ part, int n_parts, int Tp, int* header, const int* __restrict__ rows, const int* __restrict__ words,
+join_runs_kernel(const float2* __restrict__ part, int n_tiles, int pairs, int Tp, int* header, const int* __restrict__ rows, const int* __restrict__ words,
                  float* __restrict__ row_max, float* __restrict__ row_inv, const float* __restrict__ hit, float* __restrict__ loss, int reduction,
                  double* __restrict__ sums) {
     __shared__ float2 join[8][kJoinRows];
@@ -799,7 +839,7 @@ join_runs_kernel(const float2* __restrict__ part, int n_parts, int Tp, int* head
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.x * kJoinRows + (tid & 7);
     grid_launch_dependents();
     grid_dependency_wait();
-    const int count = header[0];
+    const int count = header[0], run = best_run(row_tiles(count), n_tiles, pairs), n_parts = 2 * ((n_tiles + run - 1) / run);
     const bool failed = header[1] != 0;
     float top = -INFINITY, sum = 0.f;
     auto add = [&](float2 p) {
@@ -860,17 +900,22 @@ join_runs_kernel(const float2* __restrict__ part, int n_parts, int Tp, int* head
     }
 }
 
-// dx of the rows without a target: zero.  After a wait that ran out everything is NaN.  A warp per row.
+// dx of the rows without a target: zero.  After a wait that ran out both gradients are NaN.  A warp per row.
 template <typename T>
 __global__ void __launch_bounds__(256)
-blank_rows_kernel(const int64_t* __restrict__ target, int64_t ignore, int64_t n_rows, int d, const int* __restrict__ header, T* __restrict__ dx) {
+blank_rows_kernel(const int64_t* __restrict__ target, int64_t ignore, int64_t n_rows, int d, int vocab, const int* __restrict__ header,
+                  T* __restrict__ dx, T* __restrict__ dw) {
     const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     grid_launch_dependents();
     grid_dependency_wait();
-    if (r >= n_rows) return;
-    const bool failed = header[1] != 0;
-    if (!failed && target[r] != ignore) return;
-    for (int i = threadIdx.x & 31; i < d; i += 32) dx[r * (int64_t)d + i] = failed ? T(NAN) : T(0.f);
+    if (header[1] != 0) {
+        const int64_t step = (int64_t)gridDim.x * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+        if (dx) for (int64_t i = at; i < n_rows * d; i += step) dx[i] = T(NAN);
+        if (dw) for (int64_t i = at; i < (int64_t)vocab * d; i += step) dw[i] = T(NAN);
+        return;
+    }
+    if (!dx || r >= n_rows || target[r] != ignore) return;
+    for (int i = threadIdx.x & 31; i < d; i += 32) dx[r * (int64_t)d + i] = T(0.f);
 }
 
 // ---- host ------------------------------------------------------------------------------------------
@@ -878,7 +923,7 @@ inline size_t up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
 struct Sizes {
     int64_t rows;
-    int d, V, planes, dz_planes, Tp, pitch, n_tiles, run, n_runs, pieces, vn, d_tiles;
+    int d, V, planes, dz_planes, Tp, pitch, n_tiles, pieces, vn, d_tiles;
     bool f32;
     // saved
     size_t o_rows, o_words, o_max, o_inv, o_hit, o_x, saved;
@@ -889,7 +934,6 @@ struct Sizes {
 // row's error.  Beyond, the rows' roundings average out and the product's time shows.
 constexpr int kFewRows = 256;
 constexpr size_t kPieceBytes = 512ull << 20;   // of dz, beyond which the vocabulary is cut
-constexpr int kMostRun = 8;                    // vocabulary tiles of a run: a tenth of a per cent of the row sums' traffic, still even shares
 
 bool sizes_of(int64_t rows, int d, int vocab, int dtype, int sms, Sizes& s) {
     if (rows < 1 || d < 1 || vocab < 1 || (dtype != CDSSM_BF16 && dtype != CDSSM_F32)) return false;
@@ -900,9 +944,6 @@ bool sizes_of(int64_t rows, int d, int vocab, int dtype, int sms, Sizes& s) {
     s.Tp = (int)up(rows, kM);
     s.pitch = (int)up(d, 8);
     s.n_tiles = (vocab + kN - 1) / kN;
-    const int64_t tiles = (int64_t)(s.Tp / kM) * s.n_tiles;
-    s.run = (int)std::min<int64_t>(kMostRun, std::max<int64_t>(1, tiles / (4 * (int64_t)sms)));
-    s.n_runs = (s.n_tiles + s.run - 1) / s.run;
     const size_t column = (size_t)s.Tp * 2 * s.dz_planes;
     const size_t most = std::max<size_t>(kN, kPieceBytes / column / kN * kN);
     s.pieces = (int)((up(vocab, kN) + most - 1) / most);
@@ -916,7 +957,7 @@ bool sizes_of(int64_t rows, int d, int vocab, int dtype, int sms, Sizes& s) {
     s.saved = o;
     s.w_planes = up(2ull * s.planes * (size_t)vocab * s.pitch, 256);
     o = s.w_planes;
-    s.o_part = take(8ull * 2 * s.n_runs * s.Tp); s.o_sums = take(8ull * (s.Tp / kJoinRows));
+    s.o_part = take(8ull * 2 * s.n_tiles * s.Tp); s.o_sums = take(8ull * (s.Tp / kJoinRows));
     s.fwd = o;
     o = s.w_planes;
     s.o_dz = take(column * s.vn); s.o_acc = take(s.pieces > 1 ? 4ull * s.Tp * s.d_tiles * kN : 0);
@@ -984,7 +1025,7 @@ void fill_saved(Args& a, const Sizes& s, char* saved) {
     a.row_inv = reinterpret_cast<float*>(saved + s.o_inv);
     a.hit = reinterpret_cast<float*>(saved + s.o_hit);
     a.planes = s.planes; a.dz_planes = s.dz_planes; a.Tp = s.Tp; a.d = s.d; a.V = s.V;
-    a.run = s.run; a.n_tiles = s.n_tiles; a.n_runs = s.n_runs; a.d_tiles = s.d_tiles;
+    a.n_tiles = s.n_tiles; a.d_tiles = s.d_tiles;
     a.f32 = s.f32;
     a.vec_dx = a.vec_dw = s.d % (s.f32 ? 4 : 8) == 0;
     a.wait_ns = wait_limit_ns();
@@ -1033,9 +1074,9 @@ extern "C" int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, con
         return CDSSM_ERR_CUDA;
     a.part = reinterpret_cast<float2*>(ws + s.o_part);
     a.withhold = (flags & CDSSM_SCAN_TEST_WITHHOLD) != 0;
-    const int64_t units = (int64_t)(s.Tp / ce::kM) * s.n_runs;
-    if (int rc = ce::launch_products<ce::kStats>(maps, a, 2 * (int)std::min<int64_t>(units, sms / 2), st)) return rc;
-    return launch_overlapped(ce::join_runs_kernel, dim3(s.Tp / ce::kJoinRows), dim3(256), 0, st, a.part, 2 * s.n_runs, s.Tp, header, a.rows, a.target,
+    const int pairs = (int)std::min<int64_t>((int64_t)(s.Tp / ce::kM) * s.n_tiles, sms / 2);
+    if (int rc = ce::launch_products<ce::kStats>(maps, a, 2 * pairs, st)) return rc;
+    return launch_overlapped(ce::join_runs_kernel, dim3(s.Tp / ce::kJoinRows), dim3(256), 0, st, a.part, s.n_tiles, pairs, s.Tp, header, a.rows, a.target,
                              a.row_max, a.row_inv, a.hit, loss, reduction, reinterpret_cast<double*>(ws + s.o_sums));
 }
 
@@ -1088,13 +1129,11 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
         a.terms = s.f32 ? ce::kTerms3 : s.dz_planes;
         if (int rc = launch_overlapped(ce::join_split_kernel, dim3(sms / 2, 8), dim3(256), 0, st, a, sms / 2)) return rc;
     }
-    if (grad_x) {
-        const unsigned grid = (unsigned)((rows + 7) / 8);
-        if (int rc = s.f32 ? launch_overlapped(ce::blank_rows_kernel<float>, dim3(grid), dim3(256), 0, st, target, ignore_index, rows, d, a.count,
-                                               static_cast<float*>(grad_x))
-                           : launch_overlapped(ce::blank_rows_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, st, target, ignore_index, rows, d, a.count,
-                                               static_cast<__nv_bfloat16*>(grad_x)))
-            return rc;
-    }
-    return CDSSM_OK;
+    auto blank = [&](auto* dx, auto* dw) {
+        using T = std::remove_pointer_t<decltype(dx)>;
+        return launch_overlapped(ce::blank_rows_kernel<T>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, target, ignore_index, rows, d, vocab,
+                                 a.count, dx, dw);
+    };
+    return s.f32 ? blank(static_cast<float*>(grad_x), static_cast<float*>(grad_w))
+                 : blank(static_cast<__nv_bfloat16*>(grad_x), static_cast<__nv_bfloat16*>(grad_w));
 }

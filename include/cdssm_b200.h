@@ -452,7 +452,8 @@ CDSSM_API int cdssm_b200_decode_step_reference(float* local_state, float* correc
  * saved (cdssm_b200_linear_ce_saved_bytes) is what the backward reads: keep it as it is, 256-byte aligned, as the workspace
  * (cdssm_b200_linear_ce_workspace_bytes), which is free again behind the call.  Both sizes are for the current device, 0 on
  * bad sizes.  rows <= 2^24, vocab <= 2^24, d <= 65536.  bf16 products with float32 sums; float32 operands enter as three bf16 parts.
- * flags: 0 or CDSSM_SCAN_TEST_WITHHOLD.  After a bounded wait that ran out the loss is NaN.
+ * flags: 0 or CDSSM_SCAN_TEST_WITHHOLD.  After a bounded wait that ran out the loss and its
+ * gradients are NaN.
  * Replaces the LM head and the loss of a training step: cdssm/models/model.py:50-51, cdssm/training/trainer.py:219-262. */
 #define CDSSM_CE_NONE 0
 #define CDSSM_CE_MEAN 1

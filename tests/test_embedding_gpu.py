@@ -56,3 +56,66 @@ def test_large(ops, T, V):
     g = torch.Generator(device="cuda").manual_seed(T)
     w, grad = (torch.randn(n, 16, generator=g, device="cuda").bfloat16() for n in (V, T))
     _check(ops, torch.randint(0, V, (T,), generator=g, device="cuda"), w, grad, 0.5)
+
+
+def test_tables_and_ids_anywhere(ops):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    V, d = 40, 24
+    for dtype in (torch.bfloat16, torch.float32):
+        base = torch.randn(V, d + 11, generator=g, device="cuda").to(dtype)
+        ids = torch.randint(0, V, (5, 14), generator=g, device="cuda")
+        for w in (base[:, :d], base[:, 8:8 + d], base[:, 3:3 + d], base[:, :d].t().contiguous().t(), base[::2, :d]):
+            part = ids % w.shape[0]
+            for i in (part, part.t(), part[:, ::3], part[2, 4], part[:, :0]):
+                grad = torch.randn(*i.shape, d + 1, generator=g, device="cuda").to(dtype)[..., 1:]      # an odd stride and address
+                _check(ops, i, w, grad, 1.0)
+
+
+def test_padding_and_ids_that_are_no_row(ops):
+    g = torch.Generator(device="cuda").manual_seed(2)
+    V, d, T = 60, 33, 500
+    w, grad = (torch.randn(n, d, generator=g, device="cuda") for n in (V, T))
+    ids = torch.randint(0, 9, (T,), generator=g, device="cuda")
+    _check(ops, ids, w, grad, 2.0, padding=4)
+    wrong = ids.clone()
+    wrong[[1, 7, 100]] = torch.tensor([-1, V, 2 ** 40], device="cuda")
+    ok = torch.ones(T, dtype=torch.bool, device="cuda")
+    ok[[1, 7, 100]] = False
+    w.requires_grad_()
+    out = ops.embedding(wrong, w)
+    assert out[~ok].isnan().all() and torch.equal(out[ok], w[ids[ok]])
+    spoilt = torch.where(ok[:, None], grad, float("nan"))
+    assert torch.equal(torch.autograd.grad(out, [w], [spoilt])[0], torch.autograd.grad(ops.embedding(wrong[ok], w), [w], [grad[ok]])[0])
+
+
+def test_another_stream_and_captured(ops):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    V, d, T = 1000, 64, 9000
+    w, grad = torch.randn(V, d, generator=g, device="cuda").bfloat16().requires_grad_(), torch.randn(T, d, generator=g, device="cuda").bfloat16()
+    ids = _ids("zipf", T, V, g)
+    run = lambda: [(o := ops.embedding(ids, w)).detach(), *torch.autograd.grad(o, [w], [grad])]  # noqa: E731
+    want = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        outs = run()
+    for kind in ("same", "uniform", "runs"):
+        ids.copy_(_ids(kind, T, V, g))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, run()))
+
+
+def test_refusals(ops):
+    w, ids = torch.randn(10, 8, device="cuda"), torch.arange(4, device="cuda")
+    for i, t, kw in ((ids.cpu(), w, {}), (ids, w.cpu(), {}), (ids.int(), w, {}), (ids, w.half(), {}), (ids, w[0], {}), (ids, w[:0], {}),
+                     (ids, w, dict(padding_idx=10)), (ids, w, dict(padding_idx=-2))):
+        with pytest.raises(ops.CdssmError):
+            ops.embedding(i, t, **kw)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(ops.embedding(ids, w.requires_grad_()).sum(), [w], create_graph=True)

@@ -81,3 +81,65 @@ def test_parameters(ops):
         want = g.double() * 0.5 / (n + 1e-6)
         assert ((p.grad.double() - want).abs() <= 13 * U * want.abs()).all()
     assert float(ops.clip_grad_norm_([ps[1]], 1.0)) == 0.0
+
+
+def test_values_that_are_no_numbers(ops):
+    for bad in (math.nan, math.inf, -math.inf):
+        ts = _tensors([(100,), (33,)], (torch.float32, torch.bfloat16))
+        ts[0][5] = bad
+        norm = ops.grad_norm(ts)
+        assert norm.isnan() if math.isnan(bad) else norm.isposinf()
+        out = [torch.empty_like(t) for t in ts]
+        ops.clip_grads_(ts, 1.0, out=out)
+        if math.isnan(bad):
+            assert all(t.isnan().all() for t in out)
+        else:
+            assert out[0][5].isnan() and (out[0][:5] == 0).all() and (out[1] == 0).all()
+
+
+def test_orders_streams_and_graphs(ops):
+    ts = [torch.randn(30, 40, device="cuda").t(), torch.randn(4, 5, 6, device="cuda").permute(2, 0, 1)]      # dense, in another order
+    want = [t * (0.5 / (_exact(ts) + 1e-6)) for t in ts]
+    a = [t.clone(memory_format=torch.preserve_format) for t in ts]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.clip_grads_(a, 0.5)
+    side.synchronize()
+    for x, y in zip(a, want):
+        assert ((x - y).abs() <= 13 * U * y.abs()).all()
+    src = [torch.randn(5000, device="cuda") for _ in range(60)]
+    out = [torch.empty_like(t) for t in src]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        norm = ops.clip_grads_(src, 1.0, out=out)
+    for s in (1.0, 1e-4):
+        for t in src:
+            t.normal_().mul_(s)
+        graph.replay()
+        torch.cuda.synchronize()
+        n = _exact(src)
+        assert abs(float(norm) - n) <= 6 * U * n
+        c = min(1.0, 1.0 / (n + 1e-6))
+        assert all(((o.double() - t.double() * c).abs() <= 12 * U * t.double().abs()).all() for o, t in zip(out, src))
+
+
+def test_autograd_sees_the_write(ops):
+    t = torch.randn(10, device="cuda")
+    before = t._version
+    ops.clip_grads_([t], 0.1)
+    assert t._version > before
+
+
+def test_refusals(ops):
+    t = torch.randn(100, device="cuda")
+    e = torch.empty(100, device="cuda")
+    for grads, kw in (([], {}), ([t.cpu()], {}), ([t.half()], {}), ([t[::2]], {}), ([t[:1].expand(5)], {}), ([t, t], {}), ([t, t[50:]], {}),
+                      ([t], dict(out=[e[:50]])), ([t], dict(out=[])), ([t], dict(out=[e.bfloat16()])), ([t[:99]], dict(out=[t[1:]])),
+                      ([t, e], dict(out=[e, t])), ([t, e], dict(out=[torch.empty_like(t)] * 2)), ([t.to_sparse()], {}), ([t], dict(out=[e.cpu()]))):
+        with pytest.raises(ops.CdssmError):
+            ops.clip_grads_(grads, 1.0, **kw)
+    for bound in (-1.0, math.nan):
+        with pytest.raises(ops.CdssmError):
+            ops.clip_grads_([t], bound)
+    assert float(ops.grad_norm([t, t])) == pytest.approx(math.sqrt(2) * _exact([t]), rel=6 * U)      # reading twice is no conflict
