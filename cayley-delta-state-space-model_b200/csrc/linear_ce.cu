@@ -65,7 +65,7 @@ struct Args {
     int dz_pitch;
     void *dx, *dw;
     float* acc;                  // (Tp, acc_pitch) dx of the pieces before, summed
-    int acc_pitch, d_tiles, f32, first, last, vec_dx, vec_dw;
+    int acc_pitch, d_tiles, f32, first, last, whole_sectors;
     float4* slots;               // partial tiles of the split ones: two a block
     int* status;
     unsigned long long wait_ns;
@@ -104,6 +104,8 @@ struct Segment {
     int run;
 };
 
+// Rows that are read as part of a sum: whole depth blocks.  Rows behind them are never looked at in dz.
+__device__ __forceinline__ int summed_rows(int count) { return max(1, (count + kK - 1) / kK) * kK; }
 __device__ __forceinline__ int row_tiles(int count) { return max(1, (count + kM - 1) / kM); }
 
 __device__ __forceinline__ int pair_id() { return blockIdx.x >> 1; }
@@ -154,35 +156,39 @@ struct RunWalk {
 };
 
 // dx and dW: as many whole tiles as fill the grid evenly, column tiles fastest (the pairs beside each other read the same rows of
-// dz); the depth blocks of the tiles that are left, dx before dW, are cut into as many equal shares as there are pairs.
+// dz); the depth blocks of the tiles that are left, dx before dW, are cut into as many equal shares as there are pairs.  Tiles of a small
+// depth are whole ones all: what they take is their way out (28 of 2 blocks as two pairs' shares: 61 us, a tile a pair 40).
+constexpr int kSplitDepth = 16;
 struct SplitTiles {
     int nx, nw, fx, fw, kx, kw, G, d_tiles;
-    long long rest;
+    int rest, share, more;   // depth blocks of the rest; a pair's, one more for the first ones
     __device__ SplitTiles(int mt, int vt, int d_tiles_, int kx_, int kw_, int grid) : kx(kx_), kw(kw_), G(grid), d_tiles(d_tiles_) {
         nx = mt * d_tiles;
         nw = vt * d_tiles;
-        fx = nx / G * G;
-        fw = nw / G * G;
-        rest = (long long)(nx - fx) * kx + (long long)(nw - fw) * kw;
+        fx = kx < kSplitDepth ? nx : nx / G * G;
+        fw = kw < kSplitDepth ? nw : nw / G * G;
+        rest = (nx - fx) * kx + (nw - fw) * kw;
+        share = rest / G;
+        more = rest - share * G;
     }
-    __device__ long long begin(int pair) const { return rest * pair / G; }
+    __device__ int begin(int pair) const { return pair * share + min(pair, more); }
     // the tile that depth block i of the rest belongs to, and where it begins
-    __device__ void at(long long i, int& dw, int& tile, long long& start) const {
-        const long long x = (long long)(nx - fx) * kx;
+    __device__ void at(int i, int& dw, int& tile, int& start) const {
+        const int x = (nx - fx) * kx;
         dw = i >= x;
-        const long long j = dw ? (i - x) / kw : i / kx;
-        tile = (dw ? fw : fx) + (int)j;
+        const int j = dw ? (i - x) / kw : i / kx;
+        tile = (dw ? fw : fx) + j;
         start = dw ? x + j * kw : j * kx;
     }
 };
 __device__ __forceinline__ SplitTiles split_tiles(const Args& a, int count, int grid) {
     const int mt = row_tiles(count);
-    return SplitTiles(a.dx ? mt : 0, a.dw ? (a.vn + kM - 1) / kM : 0, a.d_tiles, (a.vn + kK - 1) / kK * a.terms, mt * (kM / kK) * a.terms, grid);
+    return SplitTiles(a.dx ? mt : 0, a.dw ? (a.vn + kM - 1) / kM : 0, a.d_tiles, (a.vn + kK - 1) / kK * a.terms, summed_rows(count) / kK * a.terms, grid);
 }
 struct SplitWalk {
     SplitTiles t;
     int phase = 0, i;
-    long long at, end;
+    int at, end;
     __device__ SplitWalk(const Args& a, int count) : t(split_tiles(a, count, pairs())) {
         i = pair_id();
         at = t.begin(i);
@@ -200,12 +206,10 @@ struct SplitWalk {
             i = pair_id();
         }
         if (at >= end) return false;
-        int dw, tile;
-        long long start;
+        int dw, tile, start;
         t.at(at, dw, tile, start);
-        const int k = dw ? t.kw : t.kx;
-        const long long stop = start + k < end ? start + k : end;
-        s = {dw, tile / t.d_tiles, tile % t.d_tiles, (int)(at - start), (int)(stop - start), k, true, 0};
+        const int k = dw ? t.kw : t.kx, stop = min(start + k, end);
+        s = {dw, tile / t.d_tiles, tile % t.d_tiles, at - start, stop - start, k, true, 0};
         at = stop;
         return true;
     }
@@ -403,25 +407,31 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return reinterpret_cast<const uint32_t&>(p);
 }
 
-// 32 columns of an output row from registers; vec: 16-byte aligned and a multiple of 16 bytes wide
-template <typename T>
-__device__ __forceinline__ void store_row(T* row, int col, int cols, const float (&v)[32], bool vec) {
-    if (vec) {
-        constexpr int kE = 16 / sizeof(T);
+// Columns of an output row from registers, a sector at a time where rows begin at whole ones (aligned), else singly
+template <typename T, int kCols>
+__device__ __forceinline__ void store_row(T* row, int col, int cols, const float (&v)[kCols], bool aligned) {
+    constexpr int kE = 32 / sizeof(T);
+    if (aligned && kCols % kE == 0) {
 #pragma unroll
-        for (int j = 0; j < 32; j += kE) {
+        for (int j = 0; j + kE <= kCols; j += kE) {
             if (col + j < cols) {
-                uint4 u;
-                if constexpr (sizeof(T) == 2)
-                    u = {pack2(v[j], v[j + 1]), pack2(v[j + 2], v[j + 3]), pack2(v[j + 4], v[j + 5]), pack2(v[j + 6], v[j + 7])};
-                else
-                    u = {__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3])};
-                *reinterpret_cast<uint4*>(row + col + j) = u;
+                uint32_t w[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    if constexpr (sizeof(T) == 2) w[e] = pack2(v[j + 2 * e], v[j + 2 * e + 1]);
+                    else w[e] = __float_as_uint(v[j + e]);
+                }
+                store_sector(row + col + j, w);
             }
+        }
+    } else if (aligned) {   // four columns
+        if (col < cols) {
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(row + col) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+            else *reinterpret_cast<float4*>(row + col) = make_float4(v[0], v[1], v[2], v[3]);
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 32; j++)
+        for (int j = 0; j < kCols; j++)
             if (col + j < cols) {
                 if constexpr (sizeof(T) == 2) row[col + j] = __float2bfloat16_rn(v[j]);
                 else row[col + j] = v[j];
@@ -434,37 +444,38 @@ __device__ __forceinline__ float gradient_factor(const Args& a, int count) {
     return a.grad_rows ? 1.f : a.mean ? a.grad[0] / (float)max(count, 1) : a.grad[0];
 }
 
-// 32 columns of a row of a finished tile of dx or dW.  dx of several pieces is summed in float32 and rounded once, by the last.
-__device__ __forceinline__ void emit(const Args& a, int count, float factor, int dw, int row, int col, float (&v)[32]) {
+// Columns of a row of a finished tile of dx or dW.  dx of several pieces is summed in float32 and rounded once, by the last.
+template <int kCols>
+__device__ __forceinline__ void emit(const Args& a, int count, float factor, int dw, int row, int col, float (&v)[kCols]) {
     if (col >= a.d) return;
     if (dw) {
         if (row >= a.vn) return;
 #pragma unroll
-        for (int j = 0; j < 32; j++) v[j] *= factor;
+        for (int j = 0; j < kCols; j++) v[j] *= factor;
         const size_t at = (size_t)(a.v0 + row) * a.d;
-        if (a.f32) store_row(static_cast<float*>(a.dw) + at, col, a.d, v, a.vec_dw);
-        else store_row(static_cast<__nv_bfloat16*>(a.dw) + at, col, a.d, v, a.vec_dw);
+        if (a.f32) store_row(static_cast<float*>(a.dw) + at, col, a.d, v, a.whole_sectors);
+        else store_row(static_cast<__nv_bfloat16*>(a.dw) + at, col, a.d, v, a.whole_sectors);
         return;
     }
     if (row >= count) return;
     float* acc = a.acc + (size_t)row * a.acc_pitch + col;
     if (!a.first) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
+        for (int j = 0; j < kCols; j += 4) {
             const float4 p = *reinterpret_cast<const float4*>(acc + j);
             v[j] += p.x; v[j + 1] += p.y; v[j + 2] += p.z; v[j + 3] += p.w;
         }
     }
     if (!a.last) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(acc + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        for (int j = 0; j < kCols; j += 4) *reinterpret_cast<float4*>(acc + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
         return;
     }
 #pragma unroll
-    for (int j = 0; j < 32; j++) v[j] *= factor;
+    for (int j = 0; j < kCols; j++) v[j] *= factor;
     const size_t at = (size_t)a.rows[row] * a.d;
-    if (a.f32) store_row(static_cast<float*>(a.dx) + at, col, a.d, v, a.vec_dx);
-    else store_row(static_cast<__nv_bfloat16*>(a.dx) + at, col, a.d, v, a.vec_dx);
+    if (a.f32) store_row(static_cast<float*>(a.dx) + at, col, a.d, v, a.whole_sectors);
+    else store_row(static_cast<__nv_bfloat16*>(a.dx) + at, col, a.d, v, a.whole_sectors);
 }
 
 constexpr int kSlotFloat4 = kM * kN / 4;
@@ -536,9 +547,11 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
             }
         };
         constexpr int kUnroll = kFold ? 4 : 1;
+        const bool idle = s.m * kM + rank * kHalf + quarter * 32 >= (kMode == kStats ? count : summed_rows(count));   // rows of the warp that nobody reads
         if (kMode == kStats) {
 #pragma unroll kUnroll
             for (int c = 0; c < 4; c++) {
+                if (idle) break;
                 const int v0 = s.n * kN + half * 128 + c * 32;
                 if (v0 >= a.V) break;
                 float z[32];
@@ -570,6 +583,7 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
             const float scale = g * inv;
 #pragma unroll kUnroll
             for (int c = 0; c < 2; c++) {
+                if (idle) break;
                 const int col = s.n * kN + half * 128 + c * 64, v0 = a.v0 + col;
                 float z[64];
                 if constexpr (kFold) {
@@ -616,6 +630,7 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
             const int slot = 2 * pair_id() + (s.k0 == 0 ? 1 : 0);
 #pragma unroll kUnroll
             for (int c = 0; c < 4; c++) {
+                if (!s.dw && idle) break;
                 float v[32];
                 columns(c, v);
                 if (whole) {
@@ -646,6 +661,11 @@ product_kernel(const __grid_constant__ Maps maps, const Args a) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
     const int warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        prefetch_tmap(&maps.a);
+        prefetch_tmap(&maps.b);
+        if (kMode == kGradProducts) { prefetch_tmap(&maps.a2); prefetch_tmap(&maps.b2); }
+    }
     if ((smem_u32(smem_raw) & 1023u) != 0) {   // the swizzled tiles need 1024-byte alignment
         if (threadIdx.x == 0) atomicCAS(a.status, 0, 499);
         return;
@@ -692,41 +712,45 @@ product_kernel(const __grid_constant__ Maps maps, const Args a) {
     if (warp == 1) pair_tmem_dealloc(sm.tmem_base);
 }
 
-// Sums the shares of the tiles that were split, in the order of their depth, and hands them out.  Block (boundary, group of
-// eight warps' chunks); the first boundary inside a tile does it.  grid: pairs of the launch before.
+// Sums the shares of the tiles that were split, in the order of their depth, and hands them out: a warp for 32 rows x 4 columns, shares
+// eight at a time.  Block (boundary, 64 of those for a tile); the first boundary inside a tile does it.  grid: pairs of the launch before.
+// (32 x 32 a warp and a share at a time: 34 us where two tiles have 74 shares.)
 __global__ void __launch_bounds__(256) join_split_kernel(const Args a, int grid) {
     grid_launch_dependents();
     grid_dependency_wait();
-    const int count = *a.count, p = (int)blockIdx.x + 1, lane = threadIdx.x & 31, id = blockIdx.y * 8 + (threadIdx.x >> 5);
-    const int warp = id >> 2, chunk = id & 3;
+    const int count = *a.count, p = (int)blockIdx.x + 1, lane = threadIdx.x & 31;
     const SplitTiles t = split_tiles(a, count, grid);
-    const long long at = t.begin(p);
+    const int at = t.begin(p);
     if (at >= t.rest) return;
-    int dw, tile;
-    long long start;
+    int dw, tile, start;
     t.at(at, dw, tile, start);
-    const long long stop = start + (dw ? t.kw : t.kx);
+    const int stop = start + (dw ? t.kw : t.kx);
     if (at == start || t.begin(p - 1) > start) return;
-    // (p - 1 may begin the tile or lie before it; blocks without a share are passed over)
-    float v[32];
-    bool any = false;
-    for (int q = p - 1; q < grid; q++) {
-        const long long b = t.begin(q), e = t.begin(q + 1);
-        if (q >= p && b >= stop) break;
-        if (e <= start || b == e) continue;
-        const int slot = 2 * q + (b <= start ? 1 : 0);
+    // p - 1 has the tile's first blocks; the last share is the one that reaches its end.  (Pairs without a share are passed over: fewer depth
+    // blocks than pairs.)
+    int end = p + 1;
+    while (end < grid && t.begin(end) < stop) end++;
+    const float factor = gradient_factor(a, count);
+    const int id = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int warp = id >> 5, chunk = id >> 3 & 3, j4 = id & 7;
+    float v[4] = {};
+    constexpr int kAhead = 8;
+    for (int q0 = p - 1; q0 < end; q0 += kAhead) {
+        if (!dw && tile / t.d_tiles * kM + (warp >> 3) * kHalf + (warp & 3) * 32 >= count) return;
+        float4 x[kAhead];
+        bool on[kAhead];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float4 x = a.slots[slot_at(slot, warp, chunk, j, lane)];
-            v[4 * j] = any ? v[4 * j] + x.x : x.x;
-            v[4 * j + 1] = any ? v[4 * j + 1] + x.y : x.y;
-            v[4 * j + 2] = any ? v[4 * j + 2] + x.z : x.z;
-            v[4 * j + 3] = any ? v[4 * j + 3] + x.w : x.w;
+        for (int k = 0; k < kAhead; k++) {
+            const int q = q0 + k;
+            on[k] = q < end && t.begin(q) < t.begin(q + 1);
+            if (on[k]) x[k] = __ldcg(a.slots + slot_at(2 * q + (q < p ? 1 : 0), warp, chunk, j4, lane));
         }
-        any = true;
+#pragma unroll
+        for (int k = 0; k < kAhead; k++)
+            if (on[k]) { v[0] += x[k].x; v[1] += x[k].y; v[2] += x[k].z; v[3] += x[k].w; }
     }
-    emit(a, count, gradient_factor(a, count), dw, tile / t.d_tiles * kM + (warp >> 3) * kHalf + (warp & 3) * 32 + lane,
-         tile % t.d_tiles * kN + (warp >> 2 & 1) * 128 + chunk * 32, v);
+    emit(a, count, factor, dw, tile / t.d_tiles * kM + (warp >> 3) * kHalf + (warp & 3) * 32 + lane,
+         tile % t.d_tiles * kN + (warp >> 2 & 1) * 128 + chunk * 32 + j4 * 4, v);
 }
 
 // ---- rows in, losses out -------------------------------------------------------------------------
@@ -790,7 +814,7 @@ __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
 }
 
 // Rows of a matrix as the products read them: `pitch` bf16 values each, zeros behind the d-th, one plane a part.  rows: the caller's
-// row of each (NULL: the same), zeros where it is -1; up to *count, rounded up to a row tile, if count is given.  A warp per row.
+// row of each (NULL: the same), zeros where it is -1; the summed ones of *count if count is given.  A warp per row.
 template <typename T, int kPlanes>
 __global__ void __launch_bounds__(256)
 pack_rows_kernel(const T* __restrict__ x, int64_t stride, const int* __restrict__ rows, const int* __restrict__ count, int64_t n_rows, int d,
@@ -799,7 +823,7 @@ pack_rows_kernel(const T* __restrict__ x, int64_t stride, const int* __restrict_
     const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     grid_launch_dependents();
     grid_dependency_wait();
-    if (r >= n_rows || (count && r >= (int64_t)row_tiles(*count) * kM)) return;
+    if (r >= n_rows || (count && r >= summed_rows(*count))) return;
     const int64_t from = rows ? rows[r] : r;
     const T* const src = x + (from < 0 ? 0 : from) * stride;
     __nv_bfloat16* const dst = out + r * pitch;
@@ -1027,7 +1051,6 @@ void fill_saved(Args& a, const Sizes& s, char* saved) {
     a.planes = s.planes; a.dz_planes = s.dz_planes; a.Tp = s.Tp; a.d = s.d; a.V = s.V;
     a.n_tiles = s.n_tiles; a.d_tiles = s.d_tiles;
     a.f32 = s.f32;
-    a.vec_dx = a.vec_dw = s.d % (s.f32 ? 4 : 8) == 0;
     a.wait_ns = wait_limit_ns();
 }
 
@@ -1112,6 +1135,7 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
     a.grad_rows = reduction == CDSSM_CE_NONE;
     a.mean = reduction == CDSSM_CE_MEAN;
     a.dx = grad_x; a.dw = grad_w;
+    a.whole_sectors = s.d % (s.f32 ? 8 : 16) == 0 && (((uintptr_t)grad_x | (uintptr_t)grad_w) & 31) == 0;
     a.dz = reinterpret_cast<__nv_bfloat16*>(ws + s.o_dz);
     a.dz_pitch = s.vn;
     a.acc = reinterpret_cast<float*>(ws + s.o_acc);
@@ -1127,7 +1151,7 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
         if (int rc = ce::launch_products<ce::kGradLogits>(logits, a, sms / 2 * 2, st)) return rc;
         if (int rc = ce::launch_products<ce::kGradProducts>(grads, a, sms / 2 * 2, st)) return rc;
         a.terms = s.f32 ? ce::kTerms3 : s.dz_planes;
-        if (int rc = launch_overlapped(ce::join_split_kernel, dim3(sms / 2, 8), dim3(256), 0, st, a, sms / 2)) return rc;
+        if (int rc = launch_overlapped(ce::join_split_kernel, dim3(sms / 2 - 1, 64), dim3(256), 0, st, a, sms / 2)) return rc;
     }
     auto blank = [&](auto* dx, auto* dw) {
         using T = std::remove_pointer_t<decltype(dx)>;
