@@ -60,12 +60,16 @@ struct Args {
     int terms, group, folds;     // part products; depth blocks that go through all of them together; whether a group's sum is folded
     int Tp, d, V;
     int n_tiles;                 // forward: vocabulary tiles
+    const __nv_bfloat16* ahead;  // W, where rows of it may be asked for early
+    int64_t ahead_stride;
     int v0, vn, vn_tiles;        // backward: first word and words of the piece
     __nv_bfloat16* dz;           // (dz_planes, Tp, dz_pitch)
     int dz_pitch;
     void *dx, *dw;
     float* acc;                  // (Tp, acc_pitch) dx of the pieces before, summed
     int acc_pitch, d_tiles, f32, first, last, whole_sectors;
+    const int64_t* caller_target;   // of all rows
+    int64_t n_rows, ignore;
     float4* slots;               // partial tiles of the split ones: two a block
     int* status;
     unsigned long long wait_ns;
@@ -157,21 +161,27 @@ struct RunWalk {
 
 // dx and dW: as many whole tiles as fill the grid evenly, column tiles fastest (the pairs beside each other read the same rows of
 // dz); the depth blocks of the tiles that are left, dx before dW, are cut into as many equal shares as there are pairs.  Tiles of a small
-// depth are whole ones all: what they take is their way out (28 of 2 blocks as two pairs' shares: 61 us, a tile a pair 40).
-constexpr int kSplitDepth = 16;
+// depth are whole ones all: what they take is their way out (28 of 2 blocks as two pairs' shares: 61 us, a tile a pair 40), and pairs that
+// have one of dW more than others get so much less of dx.
+constexpr int kSplitDepth = 16, kWayOut = 10;   // depth blocks; what the way out takes in terms of them
 struct SplitTiles {
     int nx, nw, fx, fw, kx, kw, G, d_tiles;
-    int rest, share, more;   // depth blocks of the rest; a pair's, one more for the first ones
+    int rest, busy, low, share, more;   // depth blocks of the rest; pairs with a tile more and their share; the others', one more for the first ones
     __device__ SplitTiles(int mt, int vt, int d_tiles_, int kx_, int kw_, int grid) : kx(kx_), kw(kw_), G(grid), d_tiles(d_tiles_) {
         nx = mt * d_tiles;
         nw = vt * d_tiles;
         fx = kx < kSplitDepth ? nx : nx / G * G;
         fw = kw < kSplitDepth ? nw : nw / G * G;
         rest = (nx - fx) * kx + (nw - fw) * kw;
-        share = rest / G;
-        more = rest - share * G;
+        busy = fw % G;
+        low = max(0, (rest + busy * kWayOut) / G - kWayOut);
+        share = (rest - busy * low) / (G - busy);
+        more = rest - busy * low - share * (G - busy);
     }
-    __device__ int begin(int pair) const { return pair * share + min(pair, more); }
+    __device__ int begin(int pair) const {
+        const int x = pair - busy;
+        return x <= 0 ? pair * low : busy * low + x * share + min(x, more);
+    }
     // the tile that depth block i of the rest belongs to, and where it begins
     __device__ void at(int i, int& dw, int& tile, int& start) const {
         const int x = (nx - fx) * kx;
@@ -655,6 +665,15 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
     return true;
 }
 
+// The rows of W that the block's first tile reads, into L2 while the kernels before this one are under way (all that was there before the
+// call is done: index_rows_kernel).  With one row tile the first unit of a pair goes by its number alone.
+__device__ __forceinline__ void request_first_tile(const Args& a) {
+    const int run = best_run(1, a.n_tiles, pairs()), row = pair_id() * run * kN + (int)block_rank() * kHalf + (int)(threadIdx.x & 31) * 4;
+    const int bytes = (a.d * 2) & ~15;
+    for (int r = row; r < min(row + 4, a.V); r++)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.ahead + (size_t)r * a.ahead_stride), "r"(bytes) : "memory");
+}
+
 template <int kMode, bool kFold>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ Maps maps, const Args a) {
@@ -682,6 +701,7 @@ product_kernel(const __grid_constant__ Maps maps, const Args a) {
     __syncthreads();
     cluster_sync();
     tc_fence_after();
+    if (kMode == kStats && a.ahead && warp == 2) request_first_tile(a);
     grid_launch_dependents();
     grid_dependency_wait();
     const int count = *a.count;
@@ -712,45 +732,85 @@ product_kernel(const __grid_constant__ Maps maps, const Args a) {
     if (warp == 1) pair_tmem_dealloc(sm.tmem_base);
 }
 
+// dx of the rows without a target is zero.  After a wait that ran out both gradients are NaN.
+__device__ __forceinline__ void blank(const Args& a) {
+    const int64_t step = (int64_t)gridDim.x * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (*a.status != 0) {
+        auto fill = [&](void* to, int64_t n) {   // NaN, as it is in either type
+            unsigned short* const p = static_cast<unsigned short*>(to);
+            if (p) for (int64_t i = at; i < n * (a.f32 ? 2 : 1); i += step) p[i] = 0x7fff;
+        };
+        fill(a.dx, a.n_rows * a.d);
+        fill(a.dw, (int64_t)a.V * a.d);
+        return;
+    }
+    if (!a.dx) return;
+    for (int64_t r = at >> 5; r < a.n_rows; r += step >> 5) {
+        if (a.caller_target[r] != a.ignore) continue;
+        for (int i = threadIdx.x & 31; i < a.d; i += 32) {
+            if (a.f32) static_cast<float*>(a.dx)[r * a.d + i] = 0.f;
+            else static_cast<__nv_bfloat16*>(a.dx)[r * a.d + i] = __nv_bfloat16(0.f);
+        }
+    }
+}
+
 // Sums the shares of the tiles that were split, in the order of their depth, and hands them out: a warp for 32 rows x 4 columns, shares
-// eight at a time.  Block (boundary, 64 of those for a tile); the first boundary inside a tile does it.  grid: pairs of the launch before.
-// (32 x 32 a warp and a share at a time: 34 us where two tiles have 74 shares.)
+// eight at a time.  A block finds the split tiles first, the first boundary in each (up to 127 of them: a thread per boundary); then the tiles'
+// parts go round the warps.  grid: pairs of the launch before.
+// (A column of blocks per boundary: 17 us where two tiles have 74 shares, nearly all of it blocks without work; 32 x 32 a warp 34.)
+constexpr int kMostPairs = 128;
 __global__ void __launch_bounds__(256) join_split_kernel(const Args a, int grid) {
+    __shared__ int firsts[kMostPairs];
+    __shared__ unsigned found[kMostPairs / 32];
     grid_launch_dependents();
     grid_dependency_wait();
-    const int count = *a.count, p = (int)blockIdx.x + 1, lane = threadIdx.x & 31;
+    const int count = *a.count, lane = threadIdx.x & 31;
     const SplitTiles t = split_tiles(a, count, grid);
-    const int at = t.begin(p);
-    if (at >= t.rest) return;
-    int dw, tile, start;
-    t.at(at, dw, tile, start);
-    const int stop = start + (dw ? t.kw : t.kx);
-    if (at == start || t.begin(p - 1) > start) return;
-    // p - 1 has the tile's first blocks; the last share is the one that reaches its end.  (Pairs without a share are passed over: fewer depth
-    // blocks than pairs.)
-    int end = p + 1;
-    while (end < grid && t.begin(end) < stop) end++;
-    const float factor = gradient_factor(a, count);
-    const int id = blockIdx.y * 8 + (threadIdx.x >> 5);
-    const int warp = id >> 5, chunk = id >> 3 & 3, j4 = id & 7;
-    float v[4] = {};
-    constexpr int kAhead = 8;
-    for (int q0 = p - 1; q0 < end; q0 += kAhead) {
-        if (!dw && tile / t.d_tiles * kM + (warp >> 3) * kHalf + (warp & 3) * 32 >= count) return;
-        float4 x[kAhead];
-        bool on[kAhead];
-#pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            const int q = q0 + k;
-            on[k] = q < end && t.begin(q) < t.begin(q + 1);
-            if (on[k]) x[k] = __ldcg(a.slots + slot_at(2 * q + (q < p ? 1 : 0), warp, chunk, j4, lane));
-        }
-#pragma unroll
-        for (int k = 0; k < kAhead; k++)
-            if (on[k]) { v[0] += x[k].x; v[1] += x[k].y; v[2] += x[k].z; v[3] += x[k].w; }
+    // (every block has them in the same order)
+    const int p0 = threadIdx.x;
+    bool mine = false;
+    if (p0 > 0 && p0 < grid && t.begin(p0) < t.rest) {
+        int dw, tile, start;
+        t.at(t.begin(p0), dw, tile, start);
+        mine = t.begin(p0) != start && t.begin(p0 - 1) <= start;
     }
-    emit(a, count, factor, dw, tile / t.d_tiles * kM + (warp >> 3) * kHalf + (warp & 3) * 32 + lane,
-         tile % t.d_tiles * kN + (warp >> 2 & 1) * 128 + chunk * 32 + j4 * 4, v);
+    const unsigned ballot = __ballot_sync(~0u, mine);
+    if (lane == 0 && p0 < kMostPairs) found[p0 >> 5] = ballot;
+    __syncthreads();
+    int n_split = 0, before = __popc(ballot & ((1u << lane) - 1));
+    for (int w = 0; w < kMostPairs / 32; w++) {
+        if (w < p0 >> 5) before += __popc(found[w]);
+        n_split += __popc(found[w]);
+    }
+    if (mine) firsts[before] = p0;
+    __syncthreads();
+    const float factor = gradient_factor(a, count);
+    const int items = n_split * 512, warps = gridDim.x * 8;
+    for (int item = blockIdx.x * 8 + (threadIdx.x >> 5); item < items; item += warps) {
+        const int p = firsts[item >> 9], warp = item >> 5 & 15, chunk = item >> 3 & 3, j4 = item & 7;
+        int dw, tile, start;
+        t.at(t.begin(p), dw, tile, start);
+        const int stop = start + (dw ? t.kw : t.kx), row0 = tile / t.d_tiles * kM + (warp >> 3) * kHalf + (warp & 3) * 32;
+        if (!dw && row0 >= count) continue;
+        // p - 1 has the tile's first blocks; the last share is the one that reaches its end (pairs without a share are passed over)
+        float v[4] = {};
+        constexpr int kAhead = 8;
+        for (int q0 = p - 1; q0 < grid && (q0 < p || t.begin(q0) < stop); q0 += kAhead) {
+            float4 x[kAhead];
+            bool on[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                const int q = q0 + k;
+                on[k] = q < grid && (q < p || t.begin(q) < stop) && t.begin(q) < t.begin(q + 1);
+                if (on[k]) x[k] = __ldcg(a.slots + slot_at(2 * q + (q < p ? 1 : 0), warp, chunk, j4, lane));
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; k++)
+                if (on[k]) { v[0] += x[k].x; v[1] += x[k].y; v[2] += x[k].z; v[3] += x[k].w; }
+        }
+        emit(a, count, factor, dw, row0 + lane, tile % t.d_tiles * kN + (warp >> 2 & 1) * 128 + chunk * 32 + j4 * 4, v);
+    }
+    if (a.last) blank(a);
 }
 
 // ---- rows in, losses out -------------------------------------------------------------------------
@@ -758,20 +818,42 @@ constexpr int kIndexThreads = 1024;
 
 // Compact numbers of the rows that have a target, in their order: a block per 1024 rows counts the ones before its own anew (all
 // of the targets come from L2 and a second launch costs more, up to some 10^5 rows).  Rows without one lose 0.
-__global__ void __launch_bounds__(kIndexThreads)
-index_rows_kernel(const int64_t* __restrict__ target, int64_t ignore, int64_t n_rows, int Tp, int vocab, int* header, int* rows, int* words,
-                  float* loss_rows) {
+// The first kernel of a call: it lets the next ones start when all before it is done, so that they may read the caller's operands ahead.
+struct Index {
+    const int64_t* target;
+    int64_t ignore, n_rows;
+    int Tp, vocab;
+    int *header, *rows, *words;
+    float* loss_rows;
+};
+__device__ __forceinline__ void note_row(const Index& x, int at, int64_t t, int64_t y) {
+    x.rows[at] = (int)t;
+    x.words[at] = y >= 0 && y < x.vocab ? (int)y : -2;
+}
+__device__ __forceinline__ void note_end(const Index& x, int total, int tid, int threads) {
+    if (tid == 0) {
+        x.header[0] = total;   // rows that have a target
+        x.header[1] = 0;       // status
+        x.header[2] = 0;       // blocks of join_runs_kernel that are done
+    }
+    for (int i = total + tid; i < x.Tp; i += threads) {
+        x.rows[i] = -1;
+        x.words[i] = -1;
+    }
+}
+__global__ void __launch_bounds__(kIndexThreads) index_rows_kernel(const Index x) {
     __shared__ int warp_sum[32], before_sum[32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t base = (int64_t)blockIdx.x * kIndexThreads;
     int n = 0;
-    grid_launch_dependents();
     grid_dependency_wait();
-    for (int64_t i = tid; i < base; i += kIndexThreads) n += target[i] != ignore;
+    grid_launch_dependents();
+#pragma unroll 4
+    for (int64_t i = tid; i < base; i += kIndexThreads) n += x.target[i] != x.ignore;
     n = __reduce_add_sync(~0u, n);
     const int64_t t = base + tid;
-    const int64_t y = t < n_rows ? target[t] : ignore;
-    const bool on = t < n_rows && y != ignore;
+    const int64_t y = t < x.n_rows ? x.target[t] : x.ignore;
+    const bool on = t < x.n_rows && y != x.ignore;
     const unsigned ballot = __ballot_sync(~0u, on);
     if (lane == 0) {
         before_sum[warp] = n;
@@ -782,23 +864,9 @@ index_rows_kernel(const int64_t* __restrict__ target, int64_t ignore, int64_t n_
     const int mine = warp_sum[lane];
     const int total = before + __reduce_add_sync(~0u, mine);
     before += __reduce_add_sync(~0u, lane < warp ? mine : 0) + __popc(ballot & ((1u << lane) - 1));
-    if (on) {
-        rows[before] = (int)t;
-        words[before] = y >= 0 && y < vocab ? (int)y : -2;
-    } else if (t < n_rows && loss_rows) {
-        loss_rows[t] = 0.f;
-    }
-    if (blockIdx.x + 1 == gridDim.x) {
-        if (tid == 0) {
-            header[0] = total;   // rows that have a target
-            header[1] = 0;       // status
-            header[2] = 0;       // blocks of join_runs_kernel that are done
-        }
-        for (int i = total + tid; i < Tp; i += kIndexThreads) {
-            rows[i] = -1;
-            words[i] = -1;
-        }
-    }
+    if (on) note_row(x, before, t, y);
+    else if (t < x.n_rows && x.loss_rows) x.loss_rows[t] = 0.f;
+    if (blockIdx.x + 1 == gridDim.x) note_end(x, total, tid, kIndexThreads);
 }
 
 __device__ __forceinline__ float as_float(float x) { return x; }
@@ -813,31 +881,28 @@ __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
     p[2] = __float2bfloat16_rn(r - __bfloat162float(p[1]));
 }
 
-// Rows of a matrix as the products read them: `pitch` bf16 values each, zeros behind the d-th, one plane a part.  rows: the caller's
-// row of each (NULL: the same), zeros where it is -1; the summed ones of *count if count is given.  A warp per row.
+// A row of a matrix as the products read it: `pitch` bf16 values, zeros behind the d-th, a plane a part; src NULL: zeros.
 template <typename T, int kPlanes>
-__global__ void __launch_bounds__(256)
-pack_rows_kernel(const T* __restrict__ x, int64_t stride, const int* __restrict__ rows, const int* __restrict__ count, int64_t n_rows, int d,
-                 int pitch, __nv_bfloat16* __restrict__ out, int vec) {
+__device__ __forceinline__ void pack_row(const T* src, __nv_bfloat16* dst, int64_t plane, int d, int pitch, bool vec) {
     const int lane = threadIdx.x & 31;
-    const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    grid_launch_dependents();
-    grid_dependency_wait();
-    if (r >= n_rows || (count && r >= summed_rows(*count))) return;
-    const int64_t from = rows ? rows[r] : r;
-    const T* const src = x + (from < 0 ? 0 : from) * stride;
-    __nv_bfloat16* const dst = out + r * pitch;
     if (kPlanes == 1 && vec) {   // (bf16, 16-byte aligned rows: pitch is d)
         const uint4* s = reinterpret_cast<const uint4*>(src);
-        for (int i = lane; i < pitch / 8; i += 32) reinterpret_cast<uint4*>(dst)[i] = from < 0 ? make_uint4(0, 0, 0, 0) : s[i];
+        constexpr int kAhead = 4;
+        for (int i0 = lane; i0 < pitch / 8; i0 += 32 * kAhead) {
+            uint4 u[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) u[k] = src && i0 + 32 * k < pitch / 8 ? s[i0 + 32 * k] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int k = 0; k < kAhead; k++)
+                if (i0 + 32 * k < pitch / 8) reinterpret_cast<uint4*>(dst)[i0 + 32 * k] = u[k];
+        }
         return;
     }
-    const int64_t plane = n_rows * (int64_t)pitch;
     for (int i = 2 * lane; i < pitch; i += 64) {
         __nv_bfloat16 p[2][3];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const float v = from >= 0 && i + e < d ? as_float(src[i + e]) : 0.f;
+            const float v = src && i + e < d ? as_float(src[i + e]) : 0.f;
             if (kPlanes == 3) split3(v, p[e]);
             else p[e][0] = __float2bfloat16_rn(v);
         }
@@ -847,6 +912,59 @@ pack_rows_kernel(const T* __restrict__ x, int64_t stride, const int* __restrict_
             *reinterpret_cast<__nv_bfloat162*>(dst + q * plane + i) = both;
         }
     }
+}
+
+// All rows, a warp each.  rows: the caller's row of each (NULL: the same; -1: none); the summed ones of *count if count is given.
+template <typename T, int kPlanes>
+__global__ void __launch_bounds__(256)
+pack_rows_kernel(const T* __restrict__ x, int64_t stride, const int* __restrict__ rows, const int* __restrict__ count, int64_t n_rows, int d,
+                 int pitch, __nv_bfloat16* __restrict__ out, int vec) {
+    const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    grid_launch_dependents();
+    grid_dependency_wait();
+    if (r >= n_rows || (count && r >= summed_rows(*count))) return;
+    const int64_t from = rows ? rows[r] : r;
+    pack_row<T, kPlanes>(from < 0 ? nullptr : x + from * stride, out + r * pitch, n_rows * (int64_t)pitch, d, pitch, vec);
+}
+
+// index_rows_kernel and pack_rows_kernel in one, for up to kIndexThreads rows: a block looks all targets over for the eight rows that it
+// packs, the first one writes the numbers down as well.  (61 rows: two launches 6 us, one 4.)
+template <typename T, int kPlanes>
+__global__ void __launch_bounds__(256)
+index_and_pack_kernel(const Index x, const T* __restrict__ src, int64_t stride, int64_t n_rows, int d, int pitch, __nv_bfloat16* __restrict__ out, int vec) {
+    constexpr int kEach = kIndexThreads / 256;
+    __shared__ int warp_sum[8 * kEach], mine[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, first = blockIdx.x * 8;
+    grid_dependency_wait();
+    grid_launch_dependents();
+    if (tid < 8) mine[tid] = -1;
+    int64_t y[kEach];
+    unsigned ballot[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; k++) {
+        const int t = (warp * kEach + k) * 32 + lane;
+        y[k] = t < x.n_rows ? x.target[t] : x.ignore;
+        ballot[k] = __ballot_sync(~0u, y[k] != x.ignore);
+        if (lane == 0) warp_sum[warp * kEach + k] = __popc(ballot[k]);
+    }
+    __syncthreads();
+    const int sums = warp_sum[lane], total = __reduce_add_sync(~0u, sums);
+#pragma unroll
+    for (int k = 0; k < kEach; k++) {
+        const int t = (warp * kEach + k) * 32 + lane;
+        const int at = __reduce_add_sync(~0u, lane < warp * kEach + k ? sums : 0) + __popc(ballot[k] & ((1u << lane) - 1));
+        const bool on = y[k] != x.ignore;
+        if (on && at >= first && at < first + 8) mine[at - first] = t;
+        if (blockIdx.x == 0) {
+            if (on) note_row(x, at, t, y[k]);
+            else if (t < x.n_rows && x.loss_rows) x.loss_rows[t] = 0.f;
+        }
+    }
+    if (blockIdx.x == 0) note_end(x, total, tid, 256);
+    __syncthreads();
+    const int64_t r = first + warp;
+    if (r >= n_rows || r >= summed_rows(total)) return;
+    pack_row<T, kPlanes>(mine[warp] < 0 ? nullptr : src + mine[warp] * stride, out + r * pitch, n_rows * (int64_t)pitch, d, pitch, vec);
 }
 
 // Joins the runs of a row: m, 1 / s and the loss, and (mean, sum) the losses' sum: every block leaves its own, the last one to come adds
@@ -924,24 +1042,6 @@ join_runs_kernel(const float2* __restrict__ part, int n_tiles, int pairs, int Tp
     }
 }
 
-// dx of the rows without a target: zero.  After a wait that ran out both gradients are NaN.  A warp per row.
-template <typename T>
-__global__ void __launch_bounds__(256)
-blank_rows_kernel(const int64_t* __restrict__ target, int64_t ignore, int64_t n_rows, int d, int vocab, const int* __restrict__ header,
-                  T* __restrict__ dx, T* __restrict__ dw) {
-    const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    grid_launch_dependents();
-    grid_dependency_wait();
-    if (header[1] != 0) {
-        const int64_t step = (int64_t)gridDim.x * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-        if (dx) for (int64_t i = at; i < n_rows * d; i += step) dx[i] = T(NAN);
-        if (dw) for (int64_t i = at; i < (int64_t)vocab * d; i += step) dw[i] = T(NAN);
-        return;
-    }
-    if (!dx || r >= n_rows || target[r] != ignore) return;
-    for (int i = threadIdx.x & 31; i < d; i += 32) dx[r * (int64_t)d + i] = T(0.f);
-}
-
 // ---- host ------------------------------------------------------------------------------------------
 inline size_t up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
@@ -995,7 +1095,16 @@ int checked_sizes(int64_t rows, int d, int vocab, int dtype, Sizes& s) {
     if (rows > (1 << 24) || d > (1 << 16) || vocab > (1 << 24)) return CDSSM_ERR_UNSUPPORTED;   // (tile numbers and row numbers in 32 bits)
     int sms = 0;
     if (int rc = sm_count(sms)) return rc;
+    if (sms / 2 > kMostPairs) return CDSSM_ERR_UNSUPPORTED;
     return sizes_of(rows, d, vocab, dtype, sms, s) ? CDSSM_OK : CDSSM_ERR_BAD_ARG;
+}
+
+// Tensor maps are made by the driver, which wants a context in this thread: a backward pass runs in one of its own, where no runtime call may
+// have brought it about yet (allocations come from the framework's cache).
+int bind_context() {
+    int dev = 0;
+    if (int rc = check_cuda(cudaGetDevice(&dev))) return rc;
+    return check_cuda(cudaSetDevice(dev));
 }
 
 // (planes, rows, cols) bf16, boxes of box_r rows x box_c columns
@@ -1036,6 +1145,15 @@ int pack(const void* x, int64_t stride, const int* rows, const int* count, int64
 int pack_any(const void* x, int64_t stride, const int* rows, const int* count, int64_t n, const Sizes& s, void* out, cudaStream_t st) {
     if (s.f32) return pack<float, 3>(x, stride, rows, count, n, s, out, false, st);
     return pack<__nv_bfloat16, 1>(x, stride, rows, count, n, s, out, s.d % 8 == 0 && in_place(x, stride, CDSSM_BF16), st);
+}
+
+int index_and_pack(const Index& index, const void* x, int64_t stride, const Sizes& s, void* out, cudaStream_t st) {
+    const dim3 grid(s.Tp / 8), block(256);
+    __nv_bfloat16* const to = static_cast<__nv_bfloat16*>(out);
+    const int vec = s.d % 8 == 0 && in_place(x, stride, CDSSM_BF16);
+    return s.f32 ? launch_overlapped(index_and_pack_kernel<float, 3>, grid, block, 0, st, index, static_cast<const float*>(x), stride, s.Tp, s.d, s.pitch, to, 0)
+                 : launch_overlapped(index_and_pack_kernel<__nv_bfloat16, 1>, grid, block, 0, st, index, static_cast<const __nv_bfloat16*>(x), stride, s.Tp,
+                                     s.d, s.pitch, to, vec);
 }
 
 void fill_saved(Args& a, const Sizes& s, char* saved) {
@@ -1083,20 +1201,30 @@ extern "C" int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, con
     ce::Args a;
     ce::fill_saved(a, s, sv);
     int* header = reinterpret_cast<int*>(sv);
-    if (int rc = launch_overlapped(ce::index_rows_kernel, dim3((unsigned)((rows + ce::kIndexThreads - 1) / ce::kIndexThreads)),
-                                   dim3(ce::kIndexThreads), 0, st, target, ignore_index, rows, s.Tp, vocab, header, const_cast<int*>(a.rows),
-                                   const_cast<int*>(a.target), reduction == CDSSM_CE_NONE ? loss : nullptr))
-        return rc;
-    if (int rc = ce::pack_any(x, x_row_stride, a.rows, a.count, s.Tp, s, sv + s.o_x, st)) return rc;
+    const ce::Index index = {target, ignore_index, rows, s.Tp, vocab, header, const_cast<int*>(a.rows), const_cast<int*>(a.target),
+                             reduction == CDSSM_CE_NONE ? loss : nullptr};
+    if (rows <= ce::kIndexThreads) {
+        if (int rc = ce::index_and_pack(index, x, x_row_stride, s, sv + s.o_x, st)) return rc;
+    } else {
+        if (int rc = launch_overlapped(ce::index_rows_kernel, dim3((unsigned)((rows + ce::kIndexThreads - 1) / ce::kIndexThreads)),
+                                       dim3(ce::kIndexThreads), 0, st, index))
+            return rc;
+        if (int rc = ce::pack_any(x, x_row_stride, a.rows, a.count, s.Tp, s, sv + s.o_x, st)) return rc;
+    }
     const bool direct = ce::in_place(w, w_row_stride, dtype);
     if (!direct)
         if (int rc = ce::pack_any(w, w_row_stride, nullptr, nullptr, vocab, s, ws, st)) return rc;
+    if (int rc = ce::bind_context()) return rc;
     ce::Maps maps{};
     if (!ce::make_map(&maps.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, ce::kHalf) ||
         !ce::make_map(&maps.b, direct ? w : ws, direct ? d : s.pitch, vocab, s.planes, direct ? w_row_stride : s.pitch, ce::kK, ce::kHalf))
         return CDSSM_ERR_CUDA;
     a.part = reinterpret_cast<float2*>(ws + s.o_part);
     a.withhold = (flags & CDSSM_SCAN_TEST_WITHHOLD) != 0;
+    if (direct && s.Tp == ce::kM) {
+        a.ahead = static_cast<const __nv_bfloat16*>(w);
+        a.ahead_stride = w_row_stride;
+    }
     const int pairs = (int)std::min<int64_t>((int64_t)(s.Tp / ce::kM) * s.n_tiles, sms / 2);
     if (int rc = ce::launch_products<ce::kStats>(maps, a, 2 * pairs, st)) return rc;
     return launch_overlapped(ce::join_runs_kernel, dim3(s.Tp / ce::kJoinRows), dim3(256), 0, st, a.part, s.n_tiles, pairs, s.Tp, header, a.rows, a.target,
@@ -1121,6 +1249,7 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
         if (int rc = ce::pack_any(w, w_row_stride, nullptr, nullptr, vocab, s, ws, st)) return rc;
     const void* const wb = direct ? w : ws;
     const int64_t w_cols = direct ? d : s.pitch, w_pitch = direct ? w_row_stride : s.pitch;
+    if (int rc = ce::bind_context()) return rc;
     ce::Maps logits{}, grads{};
     if (!ce::make_map(&logits.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, ce::kHalf) ||
         !ce::make_map(&logits.b, wb, w_cols, vocab, s.planes, w_pitch, ce::kK, ce::kHalf) ||
@@ -1138,6 +1267,9 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
     a.whole_sectors = s.d % (s.f32 ? 8 : 16) == 0 && (((uintptr_t)grad_x | (uintptr_t)grad_w) & 31) == 0;
     a.dz = reinterpret_cast<__nv_bfloat16*>(ws + s.o_dz);
     a.dz_pitch = s.vn;
+    a.caller_target = target;
+    a.n_rows = rows;
+    a.ignore = ignore_index;
     a.acc = reinterpret_cast<float*>(ws + s.o_acc);
     a.acc_pitch = s.d_tiles * ce::kN;
     a.slots = reinterpret_cast<float4*>(ws + s.o_slots);
@@ -1151,13 +1283,7 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
         if (int rc = ce::launch_products<ce::kGradLogits>(logits, a, sms / 2 * 2, st)) return rc;
         if (int rc = ce::launch_products<ce::kGradProducts>(grads, a, sms / 2 * 2, st)) return rc;
         a.terms = s.f32 ? ce::kTerms3 : s.dz_planes;
-        if (int rc = launch_overlapped(ce::join_split_kernel, dim3(sms / 2 - 1, 64), dim3(256), 0, st, a, sms / 2)) return rc;
+        if (int rc = launch_overlapped(ce::join_split_kernel, dim3(4 * sms), dim3(256), 0, st, a, sms / 2)) return rc;
     }
-    auto blank = [&](auto* dx, auto* dw) {
-        using T = std::remove_pointer_t<decltype(dx)>;
-        return launch_overlapped(ce::blank_rows_kernel<T>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, target, ignore_index, rows, d, vocab,
-                                 a.count, dx, dw);
-    };
-    return s.f32 ? blank(static_cast<float*>(grad_x), static_cast<float*>(grad_w))
-                 : blank(static_cast<__nv_bfloat16*>(grad_x), static_cast<__nv_bfloat16*>(grad_w));
+    return CDSSM_OK;
 }
