@@ -80,7 +80,7 @@ embed_kernel(const int64_t* __restrict__ ids, const T* __restrict__ w, int64_t w
 }
 
 // ---- sort ------------------------------------------------------------------------------------------
-constexpr int kSortThreads = 1024, kItems = 4, kMostBits = 9, kBins = 1 << kMostBits;
+constexpr int kSortThreads = 1024, kItems = 8, kMostBits = 9, kBins = 1 << kMostBits;
 
 struct SortSmem {
     int hist[kBins];              // this block's, read by the others of the cluster
@@ -103,12 +103,16 @@ sort_and_clear_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t
     if ((int)blockIdx.x >= C) {
         const size_t step = (size_t)(gridDim.x - C) * kSortThreads;
 #pragma unroll 4
-        for (size_t i = (size_t)(blockIdx.x - C) * kSortThreads + tid; i < zero_vecs; i += step) zero[i] = make_uint4(0, 0, 0, 0);
+        for (size_t i = (size_t)(blockIdx.x - C) * kSortThreads + tid; i < zero_vecs / 2; i += step)   // 32 bytes a thread
+            asm volatile("st.global.v8.b32 [%0], {%1, %1, %1, %1, %1, %1, %1, %1};" ::"l"(zero + 2 * i), "r"(0) : "memory");
+        if ((int)blockIdx.x == C && tid == 0 && zero_vecs % 2) zero[zero_vecs - 1] = make_uint4(0, 0, 0, 0);
         if ((int)blockIdx.x == C && tid < tail_bytes) zero_tail[tid] = 0;
         return;
     }
     const int chunk = (n + C - 1) / C, lo = min(n, c * chunk), hi = min(n, lo + chunk);
     const int bins = 1 << bits;
+    const bool once = chunk <= kSortThreads * kItems;      // the block's part is one sub-tile: it is read once a pass
+    const int rounds = once ? (chunk + kSortThreads - 1) / kSortThreads : kItems;
     for (int pass = 0; pass < passes; pass++) {
         const uint2* const from = pass & 1 ? buf0 : buf1;
         uint2* const to = pass & 1 ? buf1 : buf0;
@@ -119,17 +123,67 @@ sort_and_clear_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t
         };
         const int shift = pass * bits;
         auto digit_of = [&](unsigned key) { return (int)(key >> shift) & (bins - 1); };
-        for (int b = tid; b < bins; b += kSortThreads) sm.hist[b] = 0;
-        __syncthreads();
-        for (int i = lo + tid; i < hi; i += kSortThreads) atomicAdd(&sm.hist[digit_of(pair_at(i).x)], 1);
+        uint2 pair[kItems];
+        int digit[kItems], rank[kItems], here = 0;
+        // the sub-tile at s: its pairs, a warp's in a row; their ranks among the warp's of their digit; the digits' counts, of the warps before and in all
+        auto count_up = [&](int s) {
+            for (int i = tid; i < 32 * kBins / 2; i += kSortThreads) reinterpret_cast<unsigned*>(sm.count)[i] = 0;
+#pragma unroll
+            for (int k = 0; k < kItems; k++) {
+                const int i = s + (warp * rounds + k) * 32 + lane;
+                const bool on = k < rounds && i < hi;
+                pair[k] = on ? pair_at(i) : make_uint2(0, 0);
+                digit[k] = on ? digit_of(pair[k].x) : bins;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kItems; k++) {
+                if (k >= rounds) break;
+                // lanes of the same digit, by a ballot a bit (65 536 keys: 36 us, by the match instruction 40)
+                unsigned same = ~0u;
+#pragma unroll
+                for (int b = 0; b <= kMostBits; b++) {
+                    if (b > bits) break;
+                    const bool bit = digit[k] >> b & 1;
+                    const unsigned vote = __ballot_sync(~0u, bit);
+                    same &= bit ? vote : ~vote;
+                }
+                const int old = digit[k] < bins ? sm.count[warp][digit[k]] : 0;
+                rank[k] = old + __popc(same & ((1u << lane) - 1));
+                __syncwarp();
+                if (digit[k] < bins && lane == __ffs(same) - 1) sm.count[warp][digit[k]] = (unsigned short)(old + __popc(same));
+                __syncwarp();
+            }
+            __syncthreads();
+            here = 0;
+            if (tid < bins) {
+#pragma unroll
+                for (int q = 0; q < 32; q++) {
+                    const int x = sm.count[q][tid];
+                    sm.count[q][tid] = (unsigned short)here;
+                    here += x;
+                }
+            }
+        };
+        if (once) {
+            count_up(lo);
+            if (tid < bins) sm.hist[tid] = here;
+        } else {
+            for (int b = tid; b < bins; b += kSortThreads) sm.hist[b] = 0;
+            __syncthreads();
+#pragma unroll 4
+            for (int i = lo + tid; i < hi; i += kSortThreads) atomicAdd(&sm.hist[digit_of(pair_at(i).x)], 1);
+        }
         cluster.sync();
         int before = 0, total = 0;
-        if (tid < bins)
-            for (int q = 0; q < C; q++) {
-                const int h = cluster.map_shared_rank(sm.hist, q)[tid];
+        if (tid < bins) {
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                const int h = q < C ? cluster.map_shared_rank(sm.hist, q)[tid] : 0;
                 total += h;
                 if (q < c) before += h;
             }
+        }
         int scan = total;   // over the digits
         for (int o = 1; o < 32; o <<= 1) {
             const int x = __shfl_up_sync(~0u, scan, o);
@@ -141,40 +195,13 @@ sort_and_clear_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t
         warps_before = __reduce_add_sync(~0u, warps_before);
         if (tid < bins) sm.base[tid] = warps_before + scan - total + before;
         for (int s = lo; s < hi; s += kSortThreads * kItems) {
-            for (int i = tid; i < 32 * kBins / 2; i += kSortThreads) reinterpret_cast<unsigned*>(sm.count)[i] = 0;
-            __syncthreads();
-            uint2 pair[kItems];
-            int digit[kItems], rank[kItems];
-#pragma unroll
-            for (int k = 0; k < kItems; k++) {   // a warp's keys lie in a row
-                const int i = s + (warp * kItems + k) * 32 + lane;
-                pair[k] = i < hi ? pair_at(i) : make_uint2(0, 0);
-                digit[k] = i < hi ? digit_of(pair[k].x) : bins;
-            }
-#pragma unroll
-            for (int k = 0; k < kItems; k++) {
-                const unsigned same = __match_any_sync(~0u, digit[k]);
-                const int old = digit[k] < bins ? sm.count[warp][digit[k]] : 0;
-                rank[k] = old + __popc(same & ((1u << lane) - 1));
-                __syncwarp();
-                if (digit[k] < bins && lane == __ffs(same) - 1) sm.count[warp][digit[k]] = (unsigned short)(old + __popc(same));
-                __syncwarp();
-            }
-            __syncthreads();
-            int here = 0;
-            if (tid < bins)
-                for (int q = 0; q < 32; q++) {
-                    const int x = sm.count[q][tid];
-                    sm.count[q][tid] = (unsigned short)here;
-                    here += x;
-                }
+            if (!once) count_up(s);
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < kItems; k++)
-                if (digit[k] < bins) to[sm.base[digit[k]] + sm.count[warp][digit[k]] + rank[k]] = pair[k];
+                if (k < rounds && digit[k] < bins) to[sm.base[digit[k]] + sm.count[warp][digit[k]] + rank[k]] = pair[k];
             __syncthreads();
             if (tid < bins) sm.base[tid] += here;
-            __syncthreads();
         }
         __threadfence();
         cluster.sync();
@@ -360,7 +387,7 @@ extern "C" int cdssm_b200_embedding_bwd(const int64_t* ids, const void* grad, vo
                                         int vocab, int d, int64_t padding_idx, float scale, int dtype, void* stream) {
     if (!ids || !grad || !grad_w || !workspace) return CDSSM_ERR_BAD_ARG;
     if (int rc = emb::check_sizes(n, vocab, d, dtype)) return rc;
-    if (((uintptr_t)grad | (uintptr_t)grad_w) & 15) return CDSSM_ERR_BAD_ARG;
+    if (((uintptr_t)grad & 15) || ((uintptr_t)grad_w & 31)) return CDSSM_ERR_BAD_ARG;
     const emb::Layout l = emb::layout(n, d);
     if (workspace_bytes < l.bytes || ((uintptr_t)workspace & 255)) return CDSSM_ERR_WORKSPACE;
     const cudaStream_t st = (cudaStream_t)stream;
@@ -372,8 +399,8 @@ extern "C" int cdssm_b200_embedding_bwd(const int64_t* ids, const void* grad, vo
     while ((int64_t)1 << bits <= vocab) bits++;   // keys 0 .. vocab
     const int passes = (bits + emb::kMostBits - 1) / emb::kMostBits, per_pass = (bits + passes - 1) / passes;
     const size_t bytes = (size_t)vocab * d * (dtype == CDSSM_BF16 ? 2 : 4);
-    // one sub-tile of a block needs no cluster; eight blocks are the most that every launch may ask for
-    const int cluster = n > emb::kSortThreads * emb::kItems ? 8 : 1;
+    // what one block sorts in four rounds needs no cluster; eight blocks are the most that every launch may ask for
+    const int cluster = n > emb::kSortThreads * 4 ? 8 : 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(cluster * std::max(2, sms / cluster)));
     cfg.blockDim = dim3(emb::kSortThreads);
