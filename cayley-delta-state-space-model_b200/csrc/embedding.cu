@@ -85,16 +85,35 @@ constexpr int kSortThreads = 1024, kItems = 8, kMostBits = 9, kBins = 1 << kMost
 struct SortSmem {
     int hist[kBins];              // this block's, read by the others of the cluster
     int base[kBins];              // where this block's next key of a digit goes
+    int local[kBins];             // where a digit begins in the sorted sub-tile
     int warp_total[32];
     unsigned short count[32][kBins];   // keys of a digit in a warp's part of the sub-tile, then in the warps before
+    unsigned lanes[32][kBins];    // of a warp that have a digit in this round; zero between rounds
+    uint2 sorted[kSortThreads * kItems];   // the sub-tile by digit: it leaves in runs (pair by pair, a sector each, 65 536 pairs took 36 us)
 };
+
+// Sum of x over the threads before this one (the block's 1024).
+__device__ __forceinline__ int block_scan(int x, int* warp_total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int scan = x;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(~0u, scan, o);
+        if (lane >= o) scan += y;
+    }
+    if (lane == 31) warp_total[warp] = scan;
+    __syncthreads();
+    const int before = __reduce_add_sync(~0u, lane < warp ? warp_total[lane] : 0);
+    __syncthreads();
+    return before + scan - x;
+}
 
 // The cluster of blocks 0 .. clusterDim - 1 sorts (key, token) pairs by key, stable, `bits` bits a pass, each block a contiguous part
 // of the pairs; the other clusters write zeros.  Ids that take no part (no row of the table, `skip`) get the key vocab: behind all others.
 __global__ void __launch_bounds__(kSortThreads)
 sort_and_clear_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t skip, int bits, int passes, uint2* buf0, uint2* buf1,
                       uint4* __restrict__ zero, size_t zero_vecs, unsigned char* zero_tail, int tail_bytes, int* spans) {
-    __shared__ SortSmem sm;
+    extern __shared__ __align__(16) unsigned char sort_smem[];
+    SortSmem& sm = *reinterpret_cast<SortSmem*>(sort_smem);
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), c = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     grid_launch_dependents();
@@ -111,6 +130,7 @@ sort_and_clear_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t
     }
     const int chunk = (n + C - 1) / C, lo = min(n, c * chunk), hi = min(n, lo + chunk);
     const int bins = 1 << bits;
+    for (int i = tid; i < 32 * kBins / 4; i += kSortThreads) reinterpret_cast<uint4*>(sm.lanes)[i] = make_uint4(0, 0, 0, 0);
     const bool once = chunk <= kSortThreads * kItems;      // the block's part is one sub-tile: it is read once a pass
     const int rounds = once ? (chunk + kSortThreads - 1) / kSortThreads : kItems;
     for (int pass = 0; pass < passes; pass++) {
@@ -139,19 +159,18 @@ sort_and_clear_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t
 #pragma unroll
             for (int k = 0; k < kItems; k++) {
                 if (k >= rounds) break;
-                // lanes of the same digit, by a ballot a bit (65 536 keys: 36 us, by the match instruction 40)
-                unsigned same = ~0u;
-#pragma unroll
-                for (int b = 0; b <= kMostBits; b++) {
-                    if (b > bits) break;
-                    const bool bit = digit[k] >> b & 1;
-                    const unsigned vote = __ballot_sync(~0u, bit);
-                    same &= bit ? vote : ~vote;
-                }
-                const int old = digit[k] < bins ? sm.count[warp][digit[k]] : 0;
+                // (lanes of the same digit find each other in shared memory: 65 536 pairs 34 us by ballots, 40 by the match instruction, this 26)
+                const bool on = digit[k] < bins;
+                if (on) atomicOr(&sm.lanes[warp][digit[k]], 1u << lane);
+                __syncwarp();
+                const unsigned same = on ? sm.lanes[warp][digit[k]] : 0u;
+                const int old = on ? sm.count[warp][digit[k]] : 0;
                 rank[k] = old + __popc(same & ((1u << lane) - 1));
                 __syncwarp();
-                if (digit[k] < bins && lane == __ffs(same) - 1) sm.count[warp][digit[k]] = (unsigned short)(old + __popc(same));
+                if (on && lane == __ffs(same) - 1) {
+                    sm.lanes[warp][digit[k]] = 0;
+                    sm.count[warp][digit[k]] = (unsigned short)(old + __popc(same));
+                }
                 __syncwarp();
             }
             __syncthreads();
@@ -184,22 +203,22 @@ sort_and_clear_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t
                 if (q < c) before += h;
             }
         }
-        int scan = total;   // over the digits
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(~0u, scan, o);
-            if (lane >= o) scan += x;
-        }
-        if (lane == 31) sm.warp_total[warp] = scan;
-        __syncthreads();
-        int warps_before = lane < warp ? sm.warp_total[lane] : 0;
-        warps_before = __reduce_add_sync(~0u, warps_before);
-        if (tid < bins) sm.base[tid] = warps_before + scan - total + before;
+        const int start = block_scan(total, sm.warp_total) + before;
+        if (tid < bins) sm.base[tid] = start;
         for (int s = lo; s < hi; s += kSortThreads * kItems) {
             if (!once) count_up(s);
+            const int local = block_scan(tid < bins ? here : 0, sm.warp_total);
+            if (tid < bins) sm.local[tid] = local;
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < kItems; k++)
-                if (k < rounds && digit[k] < bins) to[sm.base[digit[k]] + sm.count[warp][digit[k]] + rank[k]] = pair[k];
+                if (k < rounds && digit[k] < bins) sm.sorted[sm.local[digit[k]] + sm.count[warp][digit[k]] + rank[k]] = pair[k];
+            __syncthreads();
+            for (int i = tid; i < min(hi - s, kSortThreads * kItems); i += kSortThreads) {
+                const uint2 p = sm.sorted[i];
+                const int d = digit_of(p.x);
+                to[sm.base[d] + i - sm.local[d]] = p;
+            }
             __syncthreads();
             if (tid < bins) sm.base[tid] += here;
         }
@@ -401,9 +420,11 @@ extern "C" int cdssm_b200_embedding_bwd(const int64_t* ids, const void* grad, vo
     const size_t bytes = (size_t)vocab * d * (dtype == CDSSM_BF16 ? 2 : 4);
     // what one block sorts in four rounds needs no cluster; eight blocks are the most that every launch may ask for
     const int cluster = n > emb::kSortThreads * 4 ? 8 : 1;
+    if (int rc = allow_smem<emb::SortSmem>((const void*)emb::sort_and_clear_kernel, sizeof(emb::SortSmem))) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(cluster * std::max(2, sms / cluster)));
     cfg.blockDim = dim3(emb::kSortThreads);
+    cfg.dynamicSmemBytes = sizeof(emb::SortSmem);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
