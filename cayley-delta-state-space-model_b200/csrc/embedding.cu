@@ -3,10 +3,11 @@
 // out_t = scale * W[id_t];   dW[v] = scale * sum over t with id_t = v of g_t, in the order of t.
 // The gradient without atomics: (id, t) pairs are sorted, every kTile of them are summed in their order, and an id that goes on over
 // tiles is joined from the tiles' float32 partial sums, again in order: the same bits from run to run.  While one cluster of blocks
-// sorts (a few microseconds of latency for a few KB), the others fill dW with the zeros that most of its rows keep.
+// sorts (a few microseconds of latency for a few KB), a second kernel fills dW with the zeros that most of its rows keep.
 #include "cdssm_common.cuh"
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
+#include <algorithm>
 
 namespace cdssm {
 namespace emb {
@@ -107,30 +108,19 @@ __device__ __forceinline__ int block_scan(int x, int* warp_total) {
     return before + scan - x;
 }
 
-// The cluster of blocks 0 .. clusterDim - 1 sorts (key, token) pairs by key, stable, `bits` bits a pass, each block a contiguous part
-// of the pairs; the other clusters write zeros.  Ids that take no part (no row of the table, `skip`) get the key vocab: behind all others.
+// One cluster sorts (key, token) pairs by key, stable, `bits` bits a pass, each block a contiguous part of the pairs.  Ids that take no part (no row of the table, `skip`) get the key vocab: behind all others.
 __global__ void __launch_bounds__(kSortThreads)
-sort_and_clear_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t skip, int bits, int passes, uint2* buf0, uint2* buf1,
-                      uint4* __restrict__ zero, size_t zero_vecs, unsigned char* zero_tail, int tail_bytes, int* spans) {
+sort_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t skip, int bits, int passes, uint2* buf0, uint2* buf1, int* spans) {
     extern __shared__ __align__(16) unsigned char sort_smem[];
     SortSmem& sm = *reinterpret_cast<SortSmem*>(sort_smem);
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), c = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i < 32 * kBins / 4; i += kSortThreads) reinterpret_cast<uint4*>(sm.lanes)[i] = make_uint4(0, 0, 0, 0);
+    grid_dependency_wait();     // first, so that the next kernel may write where those before this one have read
     grid_launch_dependents();
-    grid_dependency_wait();
-    if (blockIdx.x == 0 && tid == 0) spans[0] = 0;
-    if ((int)blockIdx.x >= C) {
-        const size_t step = (size_t)(gridDim.x - C) * kSortThreads;
-#pragma unroll 4
-        for (size_t i = (size_t)(blockIdx.x - C) * kSortThreads + tid; i < zero_vecs / 2; i += step)   // 32 bytes a thread
-            asm volatile("st.global.v8.b32 [%0], {%1, %1, %1, %1, %1, %1, %1, %1};" ::"l"(zero + 2 * i), "r"(0) : "memory");
-        if ((int)blockIdx.x == C && tid == 0 && zero_vecs % 2) zero[zero_vecs - 1] = make_uint4(0, 0, 0, 0);
-        if ((int)blockIdx.x == C && tid < tail_bytes) zero_tail[tid] = 0;
-        return;
-    }
+    if (c == 0 && tid == 0) spans[0] = 0;
     const int chunk = (n + C - 1) / C, lo = min(n, c * chunk), hi = min(n, lo + chunk);
     const int bins = 1 << bits;
-    for (int i = tid; i < 32 * kBins / 4; i += kSortThreads) reinterpret_cast<uint4*>(sm.lanes)[i] = make_uint4(0, 0, 0, 0);
     const bool once = chunk <= kSortThreads * kItems;      // the block's part is one sub-tile: it is read once a pass
     const int rounds = once ? (chunk + kSortThreads - 1) / kSortThreads : kItems;
     for (int pass = 0; pass < passes; pass++) {
@@ -225,6 +215,17 @@ sort_and_clear_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t
         __threadfence();
         cluster.sync();
     }
+}
+
+// Zeros beside the sort, and no sooner done than it: the sums wait for this kernel alone.  (Clusters of the sort's own launch: 65 us for 262 MB,
+// two clusters of eighteen waited for a place; this 40.)
+__global__ void __launch_bounds__(kSortThreads) clear_kernel(uint4* __restrict__ to, size_t vecs, unsigned char* tail, int tail_bytes) {
+    grid_launch_dependents();
+    const size_t i = (size_t)blockIdx.x * kSortThreads + threadIdx.x;
+    if (i < vecs) to[i] = make_uint4(0, 0, 0, 0);
+    if (blockIdx.x != 0) return;
+    if ((int)threadIdx.x < tail_bytes) tail[threadIdx.x] = 0;
+    grid_dependency_wait();   // (one block's is enough: the kernel is not done before it)
 }
 
 // ---- sums --------------------------------------------------------------------------------------------
@@ -406,7 +407,7 @@ extern "C" int cdssm_b200_embedding_bwd(const int64_t* ids, const void* grad, vo
                                         int vocab, int d, int64_t padding_idx, float scale, int dtype, void* stream) {
     if (!ids || !grad || !grad_w || !workspace) return CDSSM_ERR_BAD_ARG;
     if (int rc = emb::check_sizes(n, vocab, d, dtype)) return rc;
-    if (((uintptr_t)grad & 15) || ((uintptr_t)grad_w & 31)) return CDSSM_ERR_BAD_ARG;
+    if (((uintptr_t)grad | (uintptr_t)grad_w) & 15) return CDSSM_ERR_BAD_ARG;
     const emb::Layout l = emb::layout(n, d);
     if (workspace_bytes < l.bytes || ((uintptr_t)workspace & 255)) return CDSSM_ERR_WORKSPACE;
     const cudaStream_t st = (cudaStream_t)stream;
@@ -417,12 +418,11 @@ extern "C" int cdssm_b200_embedding_bwd(const int64_t* ids, const void* grad, vo
     int bits = 1;
     while ((int64_t)1 << bits <= vocab) bits++;   // keys 0 .. vocab
     const int passes = (bits + emb::kMostBits - 1) / emb::kMostBits, per_pass = (bits + passes - 1) / passes;
-    const size_t bytes = (size_t)vocab * d * (dtype == CDSSM_BF16 ? 2 : 4);
     // what one block sorts in four rounds needs no cluster; eight blocks are the most that every launch may ask for
     const int cluster = n > emb::kSortThreads * 4 ? 8 : 1;
-    if (int rc = allow_smem<emb::SortSmem>((const void*)emb::sort_and_clear_kernel, sizeof(emb::SortSmem))) return rc;
+    if (int rc = allow_smem<emb::SortSmem>((const void*)emb::sort_kernel, sizeof(emb::SortSmem))) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(cluster * std::max(2, sms / cluster)));
+    cfg.gridDim = dim3(cluster);
     cfg.blockDim = dim3(emb::kSortThreads);
     cfg.dynamicSmemBytes = sizeof(emb::SortSmem);
     cfg.stream = st;
@@ -434,9 +434,13 @@ extern "C" int cdssm_b200_embedding_bwd(const int64_t* ids, const void* grad, vo
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    if (int rc = counted(check_cuda(cudaLaunchKernelEx(&cfg, emb::sort_and_clear_kernel, ids, (int)n, vocab, padding_idx, per_pass, passes, b0, b1,
-                                                       static_cast<uint4*>(grad_w), bytes / 16, static_cast<unsigned char*>(grad_w) + bytes / 16 * 16,
-                                                       (int)(bytes % 16), reinterpret_cast<int*>(ws + l.spans)))))
+    if (int rc = counted(check_cuda(cudaLaunchKernelEx(&cfg, emb::sort_kernel, ids, (int)n, vocab, padding_idx, per_pass, passes, b0, b1,
+                                                       reinterpret_cast<int*>(ws + l.spans)))))
+        return rc;
+    const size_t bytes = (size_t)vocab * d * (dtype == CDSSM_BF16 ? 2 : 4), vecs = bytes / 16, blocks = std::max<size_t>(1, (vecs + emb::kSortThreads - 1) / emb::kSortThreads);
+    if (blocks > 0x7fffffff) return CDSSM_ERR_UNSUPPORTED;
+    if (int rc = launch_overlapped(emb::clear_kernel, dim3((unsigned)blocks), dim3(emb::kSortThreads), 0, st, static_cast<uint4*>(grad_w), vecs,
+                                   static_cast<unsigned char*>(grad_w) + vecs * 16, (int)(bytes % 16)))
         return rc;
     const uint2* const sorted = passes & 1 ? b0 : b1;
     if (dtype == CDSSM_BF16)

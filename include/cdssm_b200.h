@@ -479,7 +479,7 @@ CDSSM_API int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, in
 CDSSM_API int cdssm_b200_embedding_fwd(const int64_t* ids, const void* w, int64_t w_row_stride, void* out, int64_t n, int vocab,
                                        int d, float scale, int dtype, void* stream);
 /* Its backward: grad_w (vocab,d) = scale * the sum of grad (n,d) over the tokens of each id, in their order, in float32 and rounded
- * once; ids that are no row of the table and padding_idx (-1: none) take no part.  grad 16-byte, grad_w 32-byte aligned, dense; the
+ * once; ids that are no row of the table and padding_idx (-1: none) take no part.  grad and grad_w 16-byte aligned, dense; the
  * workspace of cdssm_b200_embedding_bwd_workspace_bytes 256-byte aligned. */
 CDSSM_API size_t cdssm_b200_embedding_bwd_workspace_bytes(int64_t n, int vocab, int d, int dtype);
 CDSSM_API int cdssm_b200_embedding_bwd(const int64_t* ids, const void* grad, void* grad_w, void* workspace,
