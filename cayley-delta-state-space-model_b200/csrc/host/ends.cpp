@@ -213,7 +213,8 @@ void need_apart(const std::vector<Tensor>& ins, const std::vector<Tensor>& outs)
         add(outs[i], i, true);
         if (outs[i].const_data_ptr() != ins[i].const_data_ptr() || outs[i].scalar_type() != ins[i].scalar_type()) add(ins[i], i, false);
     }
-    std::sort(r.begin(), r.end(), [](const Range& x, const Range& y) { return x.at < y.at; });
+    const auto before = [](const Range& x, const Range& y) { return x.at < y.at; };
+    if (!std::is_sorted(r.begin(), r.end(), before)) std::sort(r.begin(), r.end(), before);
     uintptr_t end = 0, end_out = 0;   // of all before, of the outputs before
     for (const Range& x : r) {
         if (x.at < (x.out ? end : end_out)) throw Error("clip_grads_: an output overlaps another tensor of the call");
@@ -230,6 +231,7 @@ PyObject* py_grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
             std::vector<Tensor> v;
             if (!PyList_Check(o)) throw Error(std::string(name) + " must be a list");
             Args items{PySequence_Fast_ITEMS(o), PyList_GET_SIZE(o)};
+            v.reserve(items.n);
             for (Py_ssize_t i = 0; i < items.n; i++) v.push_back(items.tensor(name));
             return v;
         };
@@ -244,6 +246,7 @@ PyObject* py_grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
         std::vector<void*> po;
         std::vector<int64_t> sizes;
         std::vector<int> di, dout;
+        pi.reserve(ins.size()); po.reserve(ins.size()); sizes.reserve(ins.size()); di.reserve(ins.size()); dout.reserve(ins.size());
         for (size_t i = 0; i < ins.size(); i++) {
             need_dense(ins[i], "gradients");
             need_same_device(ins[i], ins[0], "gradients");
@@ -251,6 +254,11 @@ PyObject* py_grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
             sizes.push_back(ins[i].numel());
             di.push_back(dtype_code(ins[i]));
             if (!scale) continue;
+            if (outs[i].is_same(ins[i])) {
+                po.push_back(const_cast<void*>(pi.back()));
+                dout.push_back(di.back());
+                continue;
+            }
             need_dense(outs[i], "out");
             need_same_device(outs[i], ins[0], "out");
             if (outs[i].sizes() != ins[i].sizes() || outs[i].strides() != ins[i].strides()) throw Error("out must have the gradients' shapes and strides");
