@@ -58,6 +58,7 @@ struct Args {
     int grad_rows, mean;
     int planes, dz_planes;
     int terms, group, folds;     // part products; depth blocks that go through all of them together; whether a group's sum is folded
+    int few, x_rows, stacked;    // see kFewRows: whether the second block has no rows; rows that are loaded; dx of both parts of dz in one product
     int Tp, d, V;
     int n_tiles;                 // forward: vocabulary tiles
     const __nv_bfloat16* ahead;  // W, where rows of it may be asked for early
@@ -167,13 +168,13 @@ constexpr int kSplitDepth = 16, kWayOut = 10;   // depth blocks; what the way ou
 struct SplitTiles {
     int nx, nw, fx, fw, kx, kw, G, d_tiles;
     int rest, busy, low, share, more;   // depth blocks of the rest; pairs with a tile more and their share; the others', one more for the first ones
-    __device__ SplitTiles(int mt, int vt, int d_tiles_, int kx_, int kw_, int grid) : kx(kx_), kw(kw_), G(grid), d_tiles(d_tiles_) {
+    __device__ SplitTiles(int mt, int vt, int d_tiles_, int kx_, int kw_, int grid, bool even) : kx(kx_), kw(kw_), G(grid), d_tiles(d_tiles_) {
         nx = mt * d_tiles;
         nw = vt * d_tiles;
         fx = kx < kSplitDepth ? nx : nx / G * G;
         fw = kw < kSplitDepth ? nw : nw / G * G;
         rest = (nx - fx) * kx + (nw - fw) * kw;
-        busy = fw % G;
+        busy = even ? 0 : fw % G;
         low = max(0, (rest + busy * kWayOut) / G - kWayOut);
         share = (rest - busy * low) / (G - busy);
         more = rest - busy * low - share * (G - busy);
@@ -193,7 +194,8 @@ struct SplitTiles {
 };
 __device__ __forceinline__ SplitTiles split_tiles(const Args& a, int count, int grid) {
     const int mt = row_tiles(count);
-    return SplitTiles(a.dx ? mt : 0, a.dw ? (a.vn + kM - 1) / kM : 0, a.d_tiles, (a.vn + kK - 1) / kK * a.terms, summed_rows(count) / kK * a.terms, grid);
+    return SplitTiles(a.dx ? mt : 0, a.dw ? (a.vn + kM - 1) / kM : 0, a.d_tiles, (a.vn + kK - 1) / kK * (a.stacked ? 1 : a.terms),
+                      summed_rows(count) / kK * a.terms, grid, a.stacked);
 }
 struct SplitWalk {
     SplitTiles t;
@@ -300,7 +302,8 @@ __device__ __forceinline__ void store_sector(void* p, const uint32_t (&w)[8]) {
 struct Steps {
     int depth, terms, group;
     int base, n, i, term;   // of the present group: where it begins, its blocks, the block, the part product
-    __device__ Steps(const Args& a, int k0, int kt) : terms(a.terms), group(a.group) {
+    __device__ Steps(const Args& a, const Segment& s) : terms(a.stacked && !s.dw ? 1 : a.terms), group(a.group) {
+        const int k0 = s.k0, kt = s.kt;
         depth = terms == 1 ? kt : kt / terms;
         const int g = k0 / (group * terms), r = k0 - g * group * terms;
         base = g * group;
@@ -339,22 +342,27 @@ __device__ __forceinline__ bool produce(Smem& sm, const Maps& maps, const Args& 
     const int rank = block_rank(), am = rank * kHalf, bn = rank * kHalf;
     const uint32_t full0 = in_first(&sm.full[0]);
     while (walk.next(s)) {
-        Steps steps(a, s.k0, s.kt);
+        Steps steps(a, s);
 #pragma unroll 1
         for (int k = s.k0; k < s.k1; k++, it++) {
             const int st = it % kStages;
             if (!mbar_wait_suspend(&sm.empty[st], (it / kStages & 1) ^ 1, ab, a.wait_ns)) return false;
-            if (rank == 0) mbar_arrive_expect_tx(&sm.full[st], 2 * 2 * kHalf * kK * 2);
+            // (few rows: the second block's half of them is empty, dx of two parts of dz apart: it takes the second part)
+            const bool part_each = kMode == kGradProducts && a.stacked && !s.dw, rows_here = !a.few || part_each || rank == 0;
+            if (rank == 0) {
+                const uint32_t rows = a.few && !(kMode == kGradProducts && s.dw) ? (part_each ? 2 : 1) * a.x_rows : 2 * kHalf;
+                mbar_arrive_expect_tx(&sm.full[st], (rows + 2 * kHalf) * kK * 2);
+            }
             const uint32_t full = full0 + st * 8;
             int pa, pb;
             term_planes(a, kMode == kGradProducts, steps.term, pa, pb);
             const int kc = steps.kc() * kK;
             steps.next();
             if (kMode != kGradProducts) {
-                tma_load_3d(sm.a[st], &maps.a, full, kc, s.m * kM + am, pa);
+                if (rows_here) tma_load_3d(sm.a[st], &maps.a, full, kc, s.m * kM + am, pa);
                 tma_load_3d(sm.b[st], &maps.b, full, kc, a.v0 + s.n * kN + bn, pb);
             } else if (!s.dw) {
-                tma_load_3d(sm.a[st], &maps.a, full, kc, s.m * kM + am, pa);
+                if (rows_here) tma_load_3d(sm.a[st], &maps.a, full, kc, part_each ? 0 : s.m * kM + am, part_each ? rank : pa);
 #pragma unroll
                 for (int j = 0; j < kHalf / 64; j++)
                     tma_load_3d(sm.b[st] + j * 64 * kK * 2, &maps.b, full, s.n * kN + bn + j * 64, a.v0 + kc, pb);
@@ -388,7 +396,7 @@ __device__ __forceinline__ bool multiply(Smem& sm, const Args& a, int count) {
         const uint32_t idesc = umma_idesc_bf16(kM, kN, false, false) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
         const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;
         const uint32_t a_lbo = a_mn ? 8192 : 16, b_lbo = b_mn ? 8192 : 16;
-        Steps steps(a, s.k0, s.kt);
+        Steps steps(a, s);
         bool begins = true;
 #pragma unroll 1
         for (int k = s.k0; k < s.k1; k++, it++) {
@@ -557,7 +565,8 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
             }
         };
         constexpr int kUnroll = kFold ? 4 : 1;
-        const bool idle = s.m * kM + rank * kHalf + quarter * 32 >= (kMode == kStats ? count : summed_rows(count));   // rows of the warp that nobody reads
+        const bool part_each = kMode == kGradProducts && a.stacked && !s.dw;
+        const bool idle = s.m * kM + (part_each ? 0 : rank * kHalf) + quarter * 32 >= (kMode == kStats ? count : summed_rows(count));   // nobody reads the warp's rows
         if (kMode == kStats) {
 #pragma unroll kUnroll
             for (int c = 0; c < 4; c++) {
@@ -792,6 +801,7 @@ __global__ void __launch_bounds__(256) join_split_kernel(const Args a, int grid)
         t.at(t.begin(p), dw, tile, start);
         const int stop = start + (dw ? t.kw : t.kx), row0 = tile / t.d_tiles * kM + (warp >> 3) * kHalf + (warp & 3) * 32;
         if (!dw && row0 >= count) continue;
+        const bool part_each = a.stacked && !dw;   // (every tile of dx is split then; the other part's sums are the second block's)
         // p - 1 has the tile's first blocks; the last share is the one that reaches its end (pairs without a share are passed over)
         float v[4] = {};
         constexpr int kAhead = 8;
@@ -802,7 +812,13 @@ __global__ void __launch_bounds__(256) join_split_kernel(const Args a, int grid)
             for (int k = 0; k < kAhead; k++) {
                 const int q = q0 + k;
                 on[k] = q < grid && (q < p || t.begin(q) < stop) && t.begin(q) < t.begin(q + 1);
-                if (on[k]) x[k] = __ldcg(a.slots + slot_at(2 * q + (q < p ? 1 : 0), warp, chunk, j4, lane));
+                if (on[k]) {
+                    x[k] = __ldcg(a.slots + slot_at(2 * q + (q < p ? 1 : 0), warp, chunk, j4, lane));
+                    if (part_each) {
+                        const float4 y = __ldcg(a.slots + slot_at(2 * q + (q < p ? 1 : 0), warp + 8, chunk, j4, lane));
+                        x[k] = make_float4(x[k].x + y.x, x[k].y + y.y, x[k].z + y.z, x[k].w + y.w);
+                    }
+                }
             }
 #pragma unroll
             for (int k = 0; k < kAhead; k++)
@@ -1054,9 +1070,10 @@ struct Sizes {
     // scratch of the forward (W's planes if it is not read in place) and of the backward
     size_t w_planes, o_part, o_sums, fwd, o_dz, o_acc, o_slots, bwd;
 };
-// Up to this many rows of bf16, dz keeps 16 bits: where a row has one large entry (its target's), that entry's rounding to 8 bits is all of the
-// row's error.  Beyond, the rows' roundings average out and the product's time shows.
-constexpr int kFewRows = 256;
+// Up to this many rows the second block of a pair has none of its own: it loads none, and bf16's dz keeps 16 bits, in two parts.  (Where a row has
+// one large entry, its target's, that entry's rounding to 8 bits is all of the row's error; beyond, the rows' roundings average out and the products'
+// time shows.)  dx takes a part a block, W once, if its tiles are few and deep enough that every one of them is split.
+constexpr int kFewRows = kHalf;
 constexpr size_t kPieceBytes = 512ull << 20;   // of dz, beyond which the vocabulary is cut
 
 bool sizes_of(int64_t rows, int d, int vocab, int dtype, int sms, Sizes& s) {
@@ -1166,6 +1183,8 @@ void fill_saved(Args& a, const Sizes& s, char* saved) {
     a.row_max = reinterpret_cast<float*>(saved + s.o_max);
     a.row_inv = reinterpret_cast<float*>(saved + s.o_inv);
     a.hit = reinterpret_cast<float*>(saved + s.o_hit);
+    a.few = s.rows <= kFewRows;
+    a.x_rows = a.few ? (int)up(s.rows, 32) : kHalf;
     a.planes = s.planes; a.dz_planes = s.dz_planes; a.Tp = s.Tp; a.d = s.d; a.V = s.V;
     a.n_tiles = s.n_tiles; a.d_tiles = s.d_tiles;
     a.f32 = s.f32;
@@ -1216,7 +1235,7 @@ extern "C" int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, con
         if (int rc = ce::pack_any(w, w_row_stride, nullptr, nullptr, vocab, s, ws, st)) return rc;
     if (int rc = ce::bind_context()) return rc;
     ce::Maps maps{};
-    if (!ce::make_map(&maps.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, ce::kHalf) ||
+    if (!ce::make_map(&maps.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, a.x_rows) ||
         !ce::make_map(&maps.b, direct ? w : ws, direct ? d : s.pitch, vocab, s.planes, direct ? w_row_stride : s.pitch, ce::kK, ce::kHalf))
         return CDSSM_ERR_CUDA;
     a.part = reinterpret_cast<float2*>(ws + s.o_part);
@@ -1249,17 +1268,17 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
         if (int rc = ce::pack_any(w, w_row_stride, nullptr, nullptr, vocab, s, ws, st)) return rc;
     const void* const wb = direct ? w : ws;
     const int64_t w_cols = direct ? d : s.pitch, w_pitch = direct ? w_row_stride : s.pitch;
+    ce::Args a;
+    ce::fill_saved(a, s, sv);
     if (int rc = ce::bind_context()) return rc;
     ce::Maps logits{}, grads{};
-    if (!ce::make_map(&logits.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, ce::kHalf) ||
+    if (!ce::make_map(&logits.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, a.x_rows) ||
         !ce::make_map(&logits.b, wb, w_cols, vocab, s.planes, w_pitch, ce::kK, ce::kHalf) ||
-        !ce::make_map(&grads.a, ws + s.o_dz, s.vn, s.Tp, s.dz_planes, s.vn, ce::kK, ce::kHalf) ||
+        !ce::make_map(&grads.a, ws + s.o_dz, s.vn, s.Tp, s.dz_planes, s.vn, ce::kK, a.x_rows) ||
         !ce::make_map(&grads.b, wb, w_cols, vocab, s.planes, w_pitch, 64, ce::kK) ||
         !ce::make_map(&grads.a2, ws + s.o_dz, s.vn, s.Tp, s.dz_planes, s.vn, 64, ce::kK) ||
         !ce::make_map(&grads.b2, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, 64, ce::kK))
         return CDSSM_ERR_CUDA;
-    ce::Args a;
-    ce::fill_saved(a, s, sv);
     a.grad = grad_loss;
     a.grad_rows = reduction == CDSSM_CE_NONE;
     a.mean = reduction == CDSSM_CE_MEAN;
@@ -1278,6 +1297,7 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
         a.v0 = p * s.vn;
         a.vn = std::min(s.vn, vocab - a.v0);
         a.vn_tiles = (a.vn + ce::kN - 1) / ce::kN;
+        a.stacked = s.dz_planes == 2 && (a.vn + ce::kK - 1) / ce::kK >= ce::kSplitDepth && 2 * s.d_tiles + 2 <= sms / 2;
         a.first = p == 0;
         a.last = p + 1 == s.pieces;
         if (int rc = ce::launch_products<ce::kGradLogits>(logits, a, sms / 2 * 2, st)) return rc;
