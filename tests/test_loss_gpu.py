@@ -321,3 +321,26 @@ def test_model_loss(ops, dtype):
     assert got.shape == (3, 70) and (got[:, -1] == 0).all() and (got[:, :-1].double() - rows).abs().max() <= tol
     assert abs(float(lm.loss(ids)) - float(rows.mean())) <= tol
     assert torch.equal(lm.loss(ids, torch.roll(ids, -1, 1), reduction="none")[:, :-1], got[:, :-1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("seed", range(24))
+def test_sizes_at_random(ops, dtype, seed):
+    """Sizes whose tiles go round the blocks evenly, with one left over, or with fewer tiles than blocks; rows all, some or hardly any."""
+    r = __import__("random").Random(1000 + seed)
+    size = lambda most: max(1, int(most ** r.random() + r.randint(-1, 1)))  # noqa: E731
+    T, V, d = size(1500), size(30000), size(900)
+    x, w, y = _inputs(T, V, d, dtype, seed=seed, ignored=r.choice([0.0, 0.3, 0.9]), sure=r.choice([0.0, 8.0, 30.0]))
+    y[T // 2] = 0
+    reduction = r.choice(["none", "mean", "sum"])
+    g = torch.randn(T, device="cuda") if reduction == "none" else torch.randn((), device="cuda")
+    rows = g.double() if reduction == "none" else (g.double() / ((y != -100).sum() if reduction == "mean" else 1)).expand(T)
+    want, off = _exact(x, w, y, rows)
+    got = _grads(ops, x, w, y, g, reduction=reduction)
+    if reduction == "none":
+        _check(got[0], want[0], off[0], "loss")
+    else:
+        n = (y != -100).sum() if reduction == "mean" else 1
+        assert abs(got[0].double() - want[0].sum() / n) <= (off[0].sum() + U * want[0].sum()) / n
+    _check(got[1], want[1], off[1] + 4 * U * want[1].abs(), f"grad of hidden {T} {V} {d}")
+    _check(got[2], want[2], off[2] + 4 * U * want[2].abs(), f"grad of weight {T} {V} {d}")
