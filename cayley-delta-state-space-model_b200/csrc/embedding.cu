@@ -329,6 +329,106 @@ join_tiles_kernel(const uint2* __restrict__ pairs, int n, const float* __restric
     }
 }
 
+// ---- few tokens ------------------------------------------------------------------------------------------
+// Up to kFewTokens everything in one launch, without a sort: a block per token looks all ids over; the first token of an id adds up the id's
+// rows, a warp 32 vectors of columns, or, of more rows than warps, eight contiguous parts of them beside each other and then those in order.  The
+// blocks behind clear the rows of dW that no token has.  (523 tokens, 32000 x 768, forward and backward: 18.6 us with the sort, 14.5 so; 1024 tokens 18.9 and 18.6.)
+constexpr int kFewTokens = 1024, kClearBytes = 32768;
+template <typename T, int kE>
+__global__ void __launch_bounds__(32 * kJoinParts)
+few_tokens_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t skip, const T* __restrict__ grad, T* __restrict__ dw, int d, float scale,
+                  int rows_each) {
+    __shared__ int key[kFewTokens];
+    __shared__ union {
+        unsigned marked[kClearBytes / 32 + 1];
+        struct {
+            int found[kFewTokens / 32];
+            unsigned short at[kFewTokens];
+            float part[kJoinParts][32][kE];
+        } sum;
+    } sm;
+    const int tid = threadIdx.x, lane = tid & 31, y = tid >> 5;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    for (int i = tid; i < n; i += 32 * kJoinParts) {
+        const int64_t id = ids[i];
+        key[i] = id >= 0 && id < vocab && id != skip ? (int)id : -1;
+    }
+    if ((int)blockIdx.x >= n) {
+        const int64_t row0 = (int64_t)(blockIdx.x - n) * rows_each;
+        const int rows = (int)min((int64_t)rows_each, vocab - row0);
+        for (int i = tid; i <= rows / 32; i += 32 * kJoinParts) sm.marked[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += 32 * kJoinParts) {
+            const int64_t r = key[i] - row0;
+            if (key[i] >= 0 && r >= 0 && r < rows) atomicOr(&sm.marked[r >> 5], 1u << (r & 31));
+        }
+        __syncthreads();
+        const int vecs = d / kE;
+        const float zeros[kE] = {};
+        for (int i = tid; i < rows * vecs; i += 32 * kJoinParts) {
+            const int r = i / vecs;
+            if (!(sm.marked[r >> 5] >> (r & 31) & 1)) store<T, kE>(dw + (row0 + r) * d + (i - r * vecs) * kE, zeros);
+        }
+        return;
+    }
+    const int t = blockIdx.x;
+    __syncthreads();
+    const int id = key[t];
+    if (id < 0) return;
+    // the id's tokens in their order: a warp looks through every eighth 32 of them
+    bool before = false;
+    for (int w = y; w < (n + 31) / 32; w += kJoinParts) {
+        const int p = w * 32 + lane;
+        const bool same = p < n && key[p] == id;
+        before |= same && p < t;
+        const unsigned ballot = __ballot_sync(~0u, same);
+        if (lane == 0) sm.sum.found[w] = (int)ballot;
+    }
+    if (__syncthreads_or(before)) return;
+    int count = 0;
+    for (int w = 0; w < (n + 31) / 32; w++) {
+        const unsigned ballot = (unsigned)sm.sum.found[w];
+        if (w % kJoinParts == y && ballot >> lane & 1) sm.sum.at[count + __popc(ballot & ((1u << lane) - 1))] = (unsigned short)(w * 32 + lane);
+        count += __popc(ballot);
+    }
+    __syncthreads();
+    const bool parts = count > kJoinParts;
+    const int share = parts ? (count + kJoinParts - 1) / kJoinParts : count, q0 = parts ? y * share : 0, q1 = min(count, q0 + share);
+    for (int c0 = parts ? 0 : y * 32 * kE; c0 < d; c0 += (parts ? 1 : kJoinParts) * 32 * kE) {
+        const int c = c0 + lane * kE;
+        float sum[kE] = {};
+        if (c < d) {
+            constexpr int kAhead = 4;
+            for (int q = q0; q < q1; q += kAhead) {
+                float f[kAhead][kE];
+#pragma unroll
+                for (int k = 0; k < kAhead; k++)
+                    if (q + k < q1) load<T, kE>(grad + (size_t)sm.sum.at[q + k] * d + c, f[k]);
+#pragma unroll
+                for (int k = 0; k < kAhead; k++)
+                    if (q + k < q1)
+#pragma unroll
+                        for (int e = 0; e < kE; e++) sum[e] += f[k][e];
+            }
+        }
+        if (parts) {
+            __syncthreads();   // (the part before has been read)
+#pragma unroll
+            for (int e = 0; e < kE; e++) sm.sum.part[y][lane][e] = sum[e];
+            __syncthreads();
+            if (y != 0) continue;
+            for (int i = 1; i < kJoinParts; i++)
+#pragma unroll
+                for (int e = 0; e < kE; e++) sum[e] += sm.sum.part[i][lane][e];
+        }
+        if (c >= d) continue;
+#pragma unroll
+        for (int e = 0; e < kE; e++) sum[e] *= scale;
+        store<T, kE>(dw + (size_t)id * d + c, sum);
+    }
+}
+
 // ---- host ----------------------------------------------------------------------------------------------
 inline size_t up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 // Pairs of a tile: few where there are few of them (523 tokens by 32: 10 us for 17 blocks of four rounds of loads).
@@ -360,6 +460,14 @@ template <typename T, int kE>
 int forward(const int64_t* ids, const void* w, int64_t w_stride, void* out, int64_t n, int vocab, int d, float scale, cudaStream_t st) {
     return launch_overlapped(embed_kernel<T, kE>, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, ids, static_cast<const T*>(w), w_stride,
                              static_cast<T*>(out), n, vocab, d, scale);
+}
+
+template <typename T, int kE>
+int few(const int64_t* ids, int n, int vocab, int64_t skip, const void* grad, void* dw, int d, float scale, cudaStream_t st) {
+    const int rows_each = (int)std::max<size_t>(1, kClearBytes / ((size_t)d * sizeof(T)));
+    const int64_t blocks = (int64_t)n + (vocab + rows_each - 1) / rows_each;
+    return launch_overlapped(few_tokens_kernel<T, kE>, dim3((unsigned)blocks), dim3(32 * kJoinParts), 0, st, ids, n, vocab, skip,
+                             static_cast<const T*>(grad), static_cast<T*>(dw), d, scale, rows_each);
 }
 
 template <typename T, int kE, int kTile>
@@ -411,6 +519,13 @@ extern "C" int cdssm_b200_embedding_bwd(const int64_t* ids, const void* grad, vo
     const emb::Layout l = emb::layout(n, d);
     if (workspace_bytes < l.bytes || ((uintptr_t)workspace & 255)) return CDSSM_ERR_WORKSPACE;
     const cudaStream_t st = (cudaStream_t)stream;
+    if (n <= emb::kFewTokens) {
+        if (dtype == CDSSM_BF16)
+            return d % 8 == 0 ? emb::few<__nv_bfloat16, 8>(ids, (int)n, vocab, padding_idx, grad, grad_w, d, scale, st)
+                              : emb::few<__nv_bfloat16, 1>(ids, (int)n, vocab, padding_idx, grad, grad_w, d, scale, st);
+        return d % 4 == 0 ? emb::few<float, 4>(ids, (int)n, vocab, padding_idx, grad, grad_w, d, scale, st)
+                          : emb::few<float, 1>(ids, (int)n, vocab, padding_idx, grad, grad_w, d, scale, st);
+    }
     int sms = 0;
     if (int rc = sm_count(sms)) return rc;
     char* const ws = static_cast<char*>(workspace);

@@ -38,8 +38,9 @@ constexpr int kTmemCols = 2 * kN;
 
 enum Mode { kStats, kGradLogits, kGradProducts };
 
-// Depth blocks after which a sum is folded.  Loss, width 768 / 2048 in one piece: off by 7.5e-7 / 1.4e-6 of itself (float32 sums in
-// registers 2.9e-7).  Sums of bf16 gradients run on: they are rounded to 2^-8 in the end.
+// Depth blocks after which a sum is folded.  Losses of width 768 in one piece are off by 7e-7 of themselves (float32 sums in registers 3e-7), in
+// pieces of 4 blocks by 3e-7, but those take 28 % longer (8 x 2048 rows: 579 -> 740 us; 61 rows: 26.1 -> 33.4).  Sums of bf16 gradients run on: they
+// are rounded to 2^-8 in the end.
 constexpr int kFoldLogits = 12, kFold3 = 4;
 
 // Part products in the order in which they are added up: the small ones first, so that they are not lost beside the large one's rounding.
@@ -534,6 +535,8 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
                 if (row < count) g = target == -2 ? NAN : a.grad_rows ? a.grad[a.rows[row]] : 1.f;   // (-2: a target that is no word)
             }
         }
+        const bool part_each = kMode == kGradProducts && a.stacked && !s.dw;
+        const bool idle = s.m * kM + (part_each ? 0 : rank * kHalf) + quarter * 32 >= (kMode == kStats ? count : summed_rows(count));   // nobody reads the warp's rows
         float folded[kFold ? 128 : 1] = {};
         int acc = tile & 1;
         if constexpr (kFold) {
@@ -544,6 +547,7 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
                 tc_fence_after();
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
+                    if (idle && (kMode != kGradProducts || !s.dw)) break;
                     float z[32];
                     tmem_ld32(tm + acc * kN + c * 32, z);
 #pragma unroll
@@ -565,8 +569,6 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
             }
         };
         constexpr int kUnroll = kFold ? 4 : 1;
-        const bool part_each = kMode == kGradProducts && a.stacked && !s.dw;
-        const bool idle = s.m * kM + (part_each ? 0 : rank * kHalf) + quarter * 32 >= (kMode == kStats ? count : summed_rows(count));   // nobody reads the warp's rows
         if (kMode == kStats) {
 #pragma unroll kUnroll
             for (int c = 0; c < 4; c++) {
