@@ -161,17 +161,28 @@ struct RunWalk {
     }
 };
 
-// dx and dW: as many whole tiles as fill the grid evenly, column tiles fastest (the pairs beside each other read the same rows of
-// dz); the depth blocks of the tiles that are left, dx before dW, are cut into as many equal shares as there are pairs.  Tiles of a small
-// depth are whole ones all: what they take is their way out (28 of 2 blocks as two pairs' shares: 61 us, a tile a pair 40), and pairs that
-// have one of dW more than others get so much less of dx.
+// dx and dW.  Pairs form groups as wide as a row of column tiles (group_width()), a column a pair: a group reads its rows of dz at one time and
+// dz leaves DRAM once for either product.  (Column tiles as work of their own, cut where it suits the grid: 1.28 GB read instead of 0.83 for dz of
+// 262 MB.)  Of the tile rows as many whole ones as fill the groups evenly; the depth blocks of the rows that are left, dx before dW, are cut into as
+// many equal shares as there are groups.  Rows of a small depth are whole ones all: what they take is their way out (28 of 2 blocks as two
+// shares: 61 us, whole 40), and groups that have one of dW more than others get so much less of dx.
 constexpr int kSplitDepth = 16, kWayOut = 10;   // depth blocks; what the way out takes in terms of them
+// The widest part of a row of column tiles that leaves at most a tenth of the pairs without a group.
+__host__ __device__ inline int group_width(int d_tiles, int pairs) {
+    for (int w = d_tiles < 16 ? d_tiles : 16; w > 1; w--)
+        if (d_tiles % w == 0 && w <= pairs && pairs / w * w * 10 >= pairs * 9) return w;
+    return 1;
+}
 struct SplitTiles {
-    int nx, nw, fx, fw, kx, kw, G, d_tiles;
-    int rest, busy, low, share, more;   // depth blocks of the rest; pairs with a tile more and their share; the others', one more for the first ones
-    __device__ SplitTiles(int mt, int vt, int d_tiles_, int kx_, int kw_, int grid, bool even) : kx(kx_), kw(kw_), G(grid), d_tiles(d_tiles_) {
-        nx = mt * d_tiles;
-        nw = vt * d_tiles;
+    int wide, parts;         // pairs of a group; groups' widths of a row of tiles
+    int nx, nw, fx, fw, kx, kw, G;
+    int rest, busy, low, share, more;   // depth blocks of the rest; groups with a row more and their share; the others', one more for the first ones
+    __device__ SplitTiles(int mt, int vt, int d_tiles, int kx_, int kw_, int pairs, bool even) : kx(kx_), kw(kw_) {
+        wide = group_width(d_tiles, pairs);
+        parts = d_tiles / wide;
+        G = pairs / wide;
+        nx = mt * parts;
+        nw = vt * parts;
         fx = kx < kSplitDepth ? nx : nx / G * G;
         fw = kw < kSplitDepth ? nw : nw / G * G;
         rest = (nx - fx) * kx + (nw - fw) * kw;
@@ -180,49 +191,57 @@ struct SplitTiles {
         share = (rest - busy * low) / (G - busy);
         more = rest - busy * low - share * (G - busy);
     }
-    __device__ int begin(int pair) const {
-        const int x = pair - busy;
-        return x <= 0 ? pair * low : busy * low + x * share + min(x, more);
+    __device__ int begin(int group) const {
+        const int x = group - busy;
+        return x <= 0 ? group * low : busy * low + x * share + min(x, more);
     }
-    // the tile that depth block i of the rest belongs to, and where it begins
-    __device__ void at(int i, int& dw, int& tile, int& start) const {
+    // the row that depth block i of the rest belongs to, and where it begins
+    __device__ void at(int i, int& dw, int& row, int& start) const {
         const int x = (nx - fx) * kx;
         dw = i >= x;
         const int j = dw ? (i - x) / kw : i / kx;
-        tile = (dw ? fw : fx) + j;
+        row = (dw ? fw : fx) + j;
         start = dw ? x + j * kw : j * kx;
     }
+    __device__ int tile_m(int row) const { return row / parts; }
+    __device__ int tile_n(int row, int member) const { return row % parts * wide + member; }
 };
-__device__ __forceinline__ SplitTiles split_tiles(const Args& a, int count, int grid) {
+__device__ __forceinline__ SplitTiles split_tiles(const Args& a, int count, int pairs) {
     const int mt = row_tiles(count);
     return SplitTiles(a.dx ? mt : 0, a.dw ? (a.vn + kM - 1) / kM : 0, a.d_tiles, (a.vn + kK - 1) / kK * (a.stacked ? 1 : a.terms),
-                      summed_rows(count) / kK * a.terms, grid, a.stacked);
+                      summed_rows(count) / kK * a.terms, pairs, a.stacked);
 }
 struct SplitWalk {
     SplitTiles t;
-    int phase = 0, i;
+    int phase = 0, i, member, group;
     int at, end;
     __device__ SplitWalk(const Args& a, int count) : t(split_tiles(a, count, pairs())) {
-        i = pair_id();
-        at = t.begin(i);
-        end = t.begin(i + 1);
+        group = pair_id() / t.wide;
+        member = pair_id() % t.wide;
+        i = group;
+        at = end = 0;
+        if (group < t.G) {
+            at = t.begin(group);
+            end = t.begin(group + 1);
+        }
     }
     __device__ bool next(Segment& s) {
+        if (group >= t.G) return false;
         while (phase < 2) {
             if (i < (phase ? t.fw : t.fx)) {
                 const int k = phase ? t.kw : t.kx;
-                s = {phase, i / t.d_tiles, i % t.d_tiles, 0, k, k, true, 0};
+                s = {phase, t.tile_m(i), t.tile_n(i, member), 0, k, k, true, 0};
                 i += t.G;
                 return true;
             }
             phase++;
-            i = pair_id();
+            i = group;
         }
         if (at >= end) return false;
-        int dw, tile, start;
-        t.at(at, dw, tile, start);
+        int dw, row, start;
+        t.at(at, dw, row, start);
         const int k = dw ? t.kw : t.kx, stop = min(start + k, end);
-        s = {dw, tile / t.d_tiles, tile % t.d_tiles, at - start, stop - start, k, true, 0};
+        s = {dw, t.tile_m(row), t.tile_n(row, member), at - start, stop - start, k, true, 0};
         at = stop;
         return true;
     }
@@ -250,8 +269,10 @@ __device__ __forceinline__ uint32_t in_first(const void* bar) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
     return r;
 }
+// (Of this block's scope: what it orders is the reading of tensor memory, behind tcgen05's own fence.  At the cluster's it waits for the warp's
+// stores to DRAM.)
 __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+    asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 __device__ __forceinline__ void pair_tmem_alloc(uint32_t* dst) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(kTmemCols) : "memory");
@@ -568,6 +589,11 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
                 tmem_ld32(tm + acc * kN + c * 32, z);
             }
         };
+        bool held = !kFold;                              // the accumulator: let go when its last columns are in registers
+        auto let_go = [&] {
+            if (held) release(acc);
+            held = false;
+        };
         constexpr int kUnroll = kFold ? 4 : 1;
         if (kMode == kStats) {
 #pragma unroll kUnroll
@@ -577,6 +603,7 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
                 if (v0 >= a.V) break;
                 float z[32];
                 columns(c, z);
+                if (c == 3) let_go();
                 if (v0 + 32 > a.V) {
 #pragma unroll
                     for (int j = 0; j < 32; j++)
@@ -613,6 +640,7 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
                 } else {
                     tmem_ld32x2(tm + acc * kN + c * 64, z, tm + acc * kN + c * 64 + 32, z + 32);
                 }
+                if (c == 1) let_go();
 #pragma unroll
                 for (int j = 0; j < 64; j++) z[j] = ex2((z[j] - mx) * kLog2e) * scale;
                 // (1 is taken from the target's p in float32: nothing is lost where p is near one)
@@ -654,6 +682,7 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
                 if (!s.dw && idle) break;
                 float v[32];
                 columns(c, v);
+                if (c == 3) let_go();
                 if (whole) {
                     emit(a, count, factor, s.dw, row, s.n * kN + half * 128 + c * 32, v);
                 } else {
@@ -663,10 +692,8 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
                 }
             }
         }
-        if constexpr (!kFold) {
-            release(acc);
-            tile++;
-        }
+        let_go();
+        if constexpr (!kFold) tile++;
         if (kMode == kStats && s.last) {
             a.part[(size_t)(2 * s.run + half) * a.Tp + row] = make_float2(top, sum);
             top = -INFINITY;
@@ -766,23 +793,23 @@ __device__ __forceinline__ void blank(const Args& a) {
 }
 
 // Sums the shares of the tiles that were split, in the order of their depth, and hands them out: a warp for 32 rows x 4 columns, shares
-// eight at a time.  A block finds the split tiles first, the first boundary in each (up to 127 of them: a thread per boundary); then the tiles'
-// parts go round the warps.  grid: pairs of the launch before.
+// eight at a time.  A block finds the split rows first, the first boundary in each (up to 127 of them: a thread per boundary); then their tiles'
+// parts go round the warps.  pairs: of the launch before.
 // (A column of blocks per boundary: 17 us where two tiles have 74 shares, nearly all of it blocks without work; 32 x 32 a warp 34.)
 constexpr int kMostPairs = 128;
-__global__ void __launch_bounds__(256) join_split_kernel(const Args a, int grid) {
+__global__ void __launch_bounds__(256) join_split_kernel(const Args a, int pairs) {
     __shared__ int firsts[kMostPairs];
     __shared__ unsigned found[kMostPairs / 32];
     grid_launch_dependents();
     grid_dependency_wait();
     const int count = *a.count, lane = threadIdx.x & 31;
-    const SplitTiles t = split_tiles(a, count, grid);
+    const SplitTiles t = split_tiles(a, count, pairs);
     // (every block has them in the same order)
     const int p0 = threadIdx.x;
     bool mine = false;
-    if (p0 > 0 && p0 < grid && t.begin(p0) < t.rest) {
-        int dw, tile, start;
-        t.at(t.begin(p0), dw, tile, start);
+    if (p0 > 0 && p0 < t.G && t.begin(p0) < t.rest) {
+        int dw, row, start;
+        t.at(t.begin(p0), dw, row, start);
         mine = t.begin(p0) != start && t.begin(p0 - 1) <= start;
     }
     const unsigned ballot = __ballot_sync(~0u, mine);
@@ -796,28 +823,29 @@ __global__ void __launch_bounds__(256) join_split_kernel(const Args a, int grid)
     if (mine) firsts[before] = p0;
     __syncthreads();
     const float factor = gradient_factor(a, count);
-    const int items = n_split * 512, warps = gridDim.x * 8;
+    const int items = n_split * t.wide * 512, warps = gridDim.x * 8;
     for (int item = blockIdx.x * 8 + (threadIdx.x >> 5); item < items; item += warps) {
-        const int p = firsts[item >> 9], warp = item >> 5 & 15, chunk = item >> 3 & 3, j4 = item & 7;
-        int dw, tile, start;
-        t.at(t.begin(p), dw, tile, start);
-        const int stop = start + (dw ? t.kw : t.kx), row0 = tile / t.d_tiles * kM + (warp >> 3) * kHalf + (warp & 3) * 32;
+        const int tile = item >> 9, p = firsts[tile / t.wide], member = tile % t.wide, warp = item >> 5 & 15, chunk = item >> 3 & 3, j4 = item & 7;
+        int dw, row, start;
+        t.at(t.begin(p), dw, row, start);
+        const int stop = start + (dw ? t.kw : t.kx), row0 = t.tile_m(row) * kM + (warp >> 3) * kHalf + (warp & 3) * 32;
         if (!dw && row0 >= count) continue;
-        const bool part_each = a.stacked && !dw;   // (every tile of dx is split then; the other part's sums are the second block's)
-        // p - 1 has the tile's first blocks; the last share is the one that reaches its end (pairs without a share are passed over)
+        const bool part_each = a.stacked && !dw;   // (every row of dx is split then; the other part's sums are the second block's)
+        // p - 1 has the row's first blocks; the last share is the one that reaches its end (groups without a share are passed over)
         float v[4] = {};
         constexpr int kAhead = 8;
-        for (int q0 = p - 1; q0 < grid && (q0 < p || t.begin(q0) < stop); q0 += kAhead) {
+        for (int q0 = p - 1; q0 < t.G && (q0 < p || t.begin(q0) < stop); q0 += kAhead) {
             float4 x[kAhead];
             bool on[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; k++) {
                 const int q = q0 + k;
-                on[k] = q < grid && (q < p || t.begin(q) < stop) && t.begin(q) < t.begin(q + 1);
+                on[k] = q < t.G && (q < p || t.begin(q) < stop) && t.begin(q) < t.begin(q + 1);
                 if (on[k]) {
-                    x[k] = __ldcg(a.slots + slot_at(2 * q + (q < p ? 1 : 0), warp, chunk, j4, lane));
+                    const int slot = 2 * (q * t.wide + member) + (q < p ? 1 : 0);
+                    x[k] = __ldcg(a.slots + slot_at(slot, warp, chunk, j4, lane));
                     if (part_each) {
-                        const float4 y = __ldcg(a.slots + slot_at(2 * q + (q < p ? 1 : 0), warp + 8, chunk, j4, lane));
+                        const float4 y = __ldcg(a.slots + slot_at(slot, warp + 8, chunk, j4, lane));
                         x[k] = make_float4(x[k].x + y.x, x[k].y + y.y, x[k].z + y.z, x[k].w + y.w);
                     }
                 }
@@ -826,7 +854,7 @@ __global__ void __launch_bounds__(256) join_split_kernel(const Args a, int grid)
             for (int k = 0; k < kAhead; k++)
                 if (on[k]) { v[0] += x[k].x; v[1] += x[k].y; v[2] += x[k].z; v[3] += x[k].w; }
         }
-        emit(a, count, factor, dw, row0 + lane, tile % t.d_tiles * kN + (warp >> 2 & 1) * 128 + chunk * 32 + j4 * 4, v);
+        emit(a, count, factor, dw, row0 + lane, t.tile_n(row, member) * kN + (warp >> 2 & 1) * 128 + chunk * 32 + j4 * 4, v);
     }
     if (a.last) blank(a);
 }
@@ -1299,7 +1327,8 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
         a.v0 = p * s.vn;
         a.vn = std::min(s.vn, vocab - a.v0);
         a.vn_tiles = (a.vn + ce::kN - 1) / ce::kN;
-        a.stacked = s.dz_planes == 2 && (a.vn + ce::kK - 1) / ce::kK >= ce::kSplitDepth && 2 * s.d_tiles + 2 <= sms / 2;
+        const int wide = ce::group_width(s.d_tiles, sms / 2);
+        a.stacked = s.dz_planes == 2 && (a.vn + ce::kK - 1) / ce::kK >= ce::kSplitDepth && 2 * (s.d_tiles / wide) + 2 <= sms / 2 / wide;
         a.first = p == 0;
         a.last = p + 1 == s.pieces;
         if (int rc = ce::launch_products<ce::kGradLogits>(logits, a, sms / 2 * 2, st)) return rc;
