@@ -14,13 +14,14 @@ namespace emb {
 
 namespace cg = cooperative_groups;
 
+// (No pointer here is __restrict__ and no load a read-only one: a kernel that starts before its predecessors are done reads what they write.)
 // ---- values of a 16-byte vector, or single ones where rows are no multiple of it ---------------------
 template <typename T, int kE> __device__ __forceinline__ void load(const T* p, float (&f)[kE]) {
     if constexpr (kE == 1) {
         if constexpr (sizeof(T) == 2) f[0] = __bfloat162float(*p);
         else f[0] = *p;
     } else if constexpr (sizeof(T) == 2) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -28,7 +29,7 @@ template <typename T, int kE> __device__ __forceinline__ void load(const T* p, f
             f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
     } else {
-        const float4 u = __ldg(reinterpret_cast<const float4*>(p));
+        const float4 u = *reinterpret_cast<const float4*>(p);
         f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
     }
 }
@@ -55,7 +56,7 @@ template <typename T, int kE> __device__ __forceinline__ void store(T* p, const 
 // A warp per row; an id that is no row of the table gives NaN.
 template <typename T, int kE>
 __global__ void __launch_bounds__(256)
-embed_kernel(const int64_t* __restrict__ ids, const T* __restrict__ w, int64_t w_stride, T* __restrict__ out, int64_t n, int vocab, int d, float scale) {
+embed_kernel(const int64_t* ids, const T* w, int64_t w_stride, T* out, int64_t n, int vocab, int d, float scale) {
     const int64_t t = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     grid_launch_dependents();
     grid_dependency_wait();
@@ -110,7 +111,7 @@ __device__ __forceinline__ int block_scan(int x, int* warp_total) {
 
 // One cluster sorts (key, token) pairs by key, stable, `bits` bits a pass, each block a contiguous part of the pairs.  Ids that take no part (no row of the table, `skip`) get the key vocab: behind all others.
 __global__ void __launch_bounds__(kSortThreads)
-sort_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t skip, int bits, int passes, uint2* buf0, uint2* buf1, int* spans) {
+sort_kernel(const int64_t* ids, int n, int vocab, int64_t skip, int bits, int passes, uint2* buf0, uint2* buf1, int* spans) {
     extern __shared__ __align__(16) unsigned char sort_smem[];
     SortSmem& sm = *reinterpret_cast<SortSmem*>(sort_smem);
     cg::cluster_group cluster = cg::this_cluster();
@@ -219,7 +220,7 @@ sort_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t skip, int
 
 // Zeros beside the sort, and no sooner done than it: the sums wait for this kernel alone.  (Clusters of the sort's own launch: 65 us for 262 MB,
 // two clusters of eighteen waited for a place; this 40.)
-__global__ void __launch_bounds__(kSortThreads) clear_kernel(uint4* __restrict__ to, size_t vecs, unsigned char* tail, int tail_bytes) {
+__global__ void __launch_bounds__(kSortThreads) clear_kernel(uint4* to, size_t vecs, unsigned char* tail, int tail_bytes) {
     grid_launch_dependents();
     const size_t i = (size_t)blockIdx.x * kSortThreads + threadIdx.x;
     if (i < vecs) to[i] = make_uint4(0, 0, 0, 0);
@@ -233,8 +234,8 @@ __global__ void __launch_bounds__(kSortThreads) clear_kernel(uint4* __restrict__
 // one that came from the tile before the sum goes to head, of one that goes on into the next (and began here) to tail, and the tile is listed
 // in spans (their number first).
 template <typename T, int kE, int kTile>
-__global__ void sum_tiles_kernel(const uint2* __restrict__ pairs, int n, int vocab, const T* __restrict__ grad, T* __restrict__ dw,
-                                 float* __restrict__ head, float* __restrict__ tail, int* __restrict__ spans, int d, float scale) {
+__global__ void sum_tiles_kernel(const uint2* pairs, int n, int vocab, const T* grad, T* dw,
+                                 float* head, float* tail, int* spans, int d, float scale) {
     __shared__ uint2 tile[kTile + 2];   // with the neighbours of either side
     const int tile_id = blockIdx.x, p0 = tile_id * kTile;
     grid_launch_dependents();
@@ -286,8 +287,8 @@ __global__ void sum_tiles_kernel(const uint2* __restrict__ pairs, int n, int voc
 constexpr int kJoinParts = 8;
 template <typename T, int kE, int kTile>
 __global__ void __launch_bounds__(32 * kJoinParts)
-join_tiles_kernel(const uint2* __restrict__ pairs, int n, const float* __restrict__ head, const float* __restrict__ tail, const int* __restrict__ spans,
-                  T* __restrict__ dw, int d, float scale) {
+join_tiles_kernel(const uint2* pairs, int n, const float* head, const float* tail, const int* spans,
+                  T* dw, int d, float scale) {
     __shared__ float part[kJoinParts][32][kE];
     grid_launch_dependents();
     grid_dependency_wait();
@@ -336,7 +337,7 @@ join_tiles_kernel(const uint2* __restrict__ pairs, int n, const float* __restric
 constexpr int kFewTokens = 1024, kClearBytes = 32768;
 template <typename T, int kE>
 __global__ void __launch_bounds__(32 * kJoinParts)
-few_tokens_kernel(const int64_t* __restrict__ ids, int n, int vocab, int64_t skip, const T* __restrict__ grad, T* __restrict__ dw, int d, float scale,
+few_tokens_kernel(const int64_t* ids, int n, int vocab, int64_t skip, const T* grad, T* dw, int d, float scale,
                   int rows_each) {
     __shared__ int key[kFewTokens];
     __shared__ union {

@@ -103,7 +103,7 @@ __device__ __forceinline__ double chunk_squares(const T* p, int n) {
         uint4 u[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; k++)
-            if (i0 + k * kThreads < vecs) u[k] = __ldg(v + i0 + k * kThreads);
+            if (i0 + k * kThreads < vecs) u[k] = v[i0 + k * kThreads];
 #pragma unroll
         for (int k = 0; k < kAhead; k++)
             if (i0 + k * kThreads < vecs) {
@@ -128,7 +128,7 @@ __device__ __forceinline__ double block_sum(double x) {   // valid in thread 0
 }
 
 template <int kMost>
-__global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ Table<kMost> t, double* __restrict__ sums) {
+__global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ Table<kMost> t, double* sums) {
     const Piece p = piece(t, blockIdx.x);
     grid_launch_dependents();
     grid_dependency_wait();
@@ -143,7 +143,7 @@ __device__ __forceinline__ float clip_factor(float norm, float max_norm) {
     return c > 1.f ? 1.f : c;
 }
 
-__global__ void __launch_bounds__(1024) norm_kernel(const double* __restrict__ sums, int64_t n, float max_norm, float* norm, float* factor) {
+__global__ void __launch_bounds__(1024) norm_kernel(const double* sums, int64_t n, float max_norm, float* norm, float* factor) {
     grid_launch_dependents();
     grid_dependency_wait();
     double s = 0.0;
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(const double* __restrict__ s
     for (int64_t i = threadIdx.x; i < n; i += 1024 * kAhead) {
         double x[kAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; k++) x[k] = i + 1024 * k < n ? __ldg(sums + i + 1024 * k) : 0.0;
+        for (int k = 0; k < kAhead; k++) x[k] = i + 1024 * k < n ? __ldcg(sums + i + 1024 * k) : 0.0;
 #pragma unroll
         for (int k = 0; k < kAhead; k++) s += x[k];
     }
@@ -223,8 +223,8 @@ __device__ __forceinline__ void chunk_scale(const T* p, O* o, int n, float c) {
 // small enough to find that out quickly (26 000 blocks: 31 us).
 // few > 0: so many sums, few enough for every block to add up (kFewSums), and there was no norm_kernel.
 template <int kMost>
-__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table<kMost> t, const float* __restrict__ factor, int chunks, int in_place,
-                                                         const double* __restrict__ sums, int few, float max_norm, float* norm) {
+__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table<kMost> t, const float* factor, int chunks, int in_place,
+                                                         const double* sums, int few, float max_norm, float* norm) {
     grid_launch_dependents();
     grid_dependency_wait();
     float c;

@@ -39,7 +39,7 @@ constexpr int kTmemCols = 2 * kN;
 enum Mode { kStats, kGradLogits, kGradProducts };
 
 // Depth blocks after which a sum is folded.  Losses of width 768 in one piece are off by 7e-7 of themselves (float32 sums in registers 3e-7), in
-// pieces of 4 blocks by 3e-7, but those take 28 % longer (8 x 2048 rows: 579 -> 740 us; 61 rows: 26.1 -> 33.4).  Sums of bf16 gradients run on: they
+// pieces of 4 blocks by 3e-7, but those take an eighth longer (8 x 2048 rows: 571 -> 645 us; 61 rows: 25.8 -> 28.8).  Sums of bf16 gradients run on: they
 // are rounded to 2^-8 in the end.
 constexpr int kFoldLogits = 12, kFold3 = 4;
 
@@ -567,14 +567,15 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
                 if (!mbar_wait_suspend(&sm.acc_full[acc], tile >> 1 & 1, ab, a.wait_ns)) return false;
                 tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < 2; c++) {
                     if (idle && (kMode != kGradProducts || !s.dw)) break;
-                    float z[32];
-                    tmem_ld32(tm + acc * kN + c * 32, z);
+                    float z[64];
+                    tmem_ld32x2(tm + acc * kN + c * 64, z, tm + acc * kN + c * 64 + 32, z + 32);
+                    if (c == 1) release(acc);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) folded[c * 32 + j] += z[j];
+                    for (int j = 0; j < 64; j++) folded[c * 64 + j] += z[j];
                 }
-                release(acc);
+                if (idle && (kMode != kGradProducts || !s.dw)) release(acc);
                 tile++;
             }
         } else {
@@ -708,7 +709,7 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
 __device__ __forceinline__ void request_first_tile(const Args& a) {
     const int run = best_run(1, a.n_tiles, pairs()), row = pair_id() * run * kN + (int)block_rank() * kHalf + (int)(threadIdx.x & 31) * 4;
     const int bytes = (a.d * 2) & ~15;
-    for (int r = row; r < min(row + 4, a.V); r++)
+    for (int r = row; bytes && r < min(row + 4, a.V); r++)
         asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.ahead + (size_t)r * a.ahead_stride), "r"(bytes) : "memory");
 }
 
@@ -963,8 +964,8 @@ __device__ __forceinline__ void pack_row(const T* src, __nv_bfloat16* dst, int64
 // All rows, a warp each.  rows: the caller's row of each (NULL: the same; -1: none); the summed ones of *count if count is given.
 template <typename T, int kPlanes>
 __global__ void __launch_bounds__(256)
-pack_rows_kernel(const T* __restrict__ x, int64_t stride, const int* __restrict__ rows, const int* __restrict__ count, int64_t n_rows, int d,
-                 int pitch, __nv_bfloat16* __restrict__ out, int vec) {
+pack_rows_kernel(const T* x, int64_t stride, const int* rows, const int* count, int64_t n_rows, int d,
+                 int pitch, __nv_bfloat16* out, int vec) {
     const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     grid_launch_dependents();
     grid_dependency_wait();
@@ -977,7 +978,7 @@ pack_rows_kernel(const T* __restrict__ x, int64_t stride, const int* __restrict_
 // packs, the first one writes the numbers down as well.  (61 rows: two launches 6 us, one 4.)
 template <typename T, int kPlanes>
 __global__ void __launch_bounds__(256)
-index_and_pack_kernel(const Index x, const T* __restrict__ src, int64_t stride, int64_t n_rows, int d, int pitch, __nv_bfloat16* __restrict__ out, int vec) {
+index_and_pack_kernel(const Index x, const T* src, int64_t stride, int64_t n_rows, int d, int pitch, __nv_bfloat16* out, int vec) {
     constexpr int kEach = kIndexThreads / 256;
     __shared__ int warp_sum[8 * kEach], mine[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, first = blockIdx.x * 8;
@@ -1018,9 +1019,9 @@ index_and_pack_kernel(const Index x, const T* __restrict__ src, int64_t stride, 
 // 61 rows with a thread per row and eighth of the runs: 28 us).
 constexpr int kJoinRows = 8;
 __global__ void __launch_bounds__(256)
-join_runs_kernel(const float2* __restrict__ part, int n_tiles, int pairs, int Tp, int* header, const int* __restrict__ rows, const int* __restrict__ words,
-                 float* __restrict__ row_max, float* __restrict__ row_inv, const float* __restrict__ hit, float* __restrict__ loss, int reduction,
-                 double* __restrict__ sums) {
+join_runs_kernel(const float2* part, int n_tiles, int pairs, int Tp, int* header, const int* rows, const int* words,
+                 float* row_max, float* row_inv, const float* hit, float* loss, int reduction,
+                 double* sums) {
     __shared__ float2 join[8][kJoinRows];
     __shared__ double warp_sum[8];
     __shared__ bool is_last;
@@ -1040,7 +1041,7 @@ join_runs_kernel(const float2* __restrict__ part, int n_tiles, int pairs, int Tp
         for (int i = tid >> 3; i < n_parts; i += 32 * kAhead) {
             float2 p[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; k++) p[k] = i + 32 * k < n_parts ? __ldg(part + (size_t)(i + 32 * k) * Tp + r) : make_float2(-INFINITY, 0.f);
+            for (int k = 0; k < kAhead; k++) p[k] = i + 32 * k < n_parts ? __ldcg(part + (size_t)(i + 32 * k) * Tp + r) : make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int k = 0; k < kAhead; k++) add(p[k]);
         }
