@@ -32,7 +32,7 @@ using namespace sm100;
 
 constexpr int kM = 256, kN = 256, kK = 64;              // rows and columns of a pair's tile, depth of a stage
 constexpr int kHalf = 128;                              // of either, a block's
-constexpr int kStages = 7;
+constexpr int kStages = 7, kSoloStages = 4;             // of 32 KB, of 48
 constexpr int kEpilogueWarps = 8, kThreads = 128 + 32 * kEpilogueWarps;
 constexpr int kTmemCols = 2 * kN;
 
@@ -59,7 +59,7 @@ struct Args {
     int grad_rows, mean;
     int planes, dz_planes;
     int terms, group, folds;     // part products; depth blocks that go through all of them together; whether a group's sum is folded
-    int few, x_rows, stacked;    // see kFewRows: whether the second block has no rows; rows that are loaded; dx of both parts of dz in one product
+    int few, x_rows, stacked;    // see kFewRows: whether there are few rows; the rows that are loaded; dx of both parts of dz in one product
     int Tp, d, V;
     int n_tiles;                 // forward: vocabulary tiles
     const __nv_bfloat16* ahead;  // W, where rows of it may be asked for early
@@ -78,9 +78,13 @@ struct Args {
     int withhold;
 };
 
-struct __align__(1024) Smem {
+// kSolo: a block by itself (few rows, z alone): 128 rows and all 256 columns of a tile.  The second block of a pair would multiply rows that are not
+// there, so two blocks take two tiles in the time of a pair's one (16 rows, 32000 words of width 2048: 39.9 us as pairs, 35.8 so; 61 rows,
+// 50257 words of width 768: 25.9 and 25.2).
+template <bool kSolo> struct __align__(1024) Smem {
+    static constexpr int kStages = kSolo ? kSoloStages : ce::kStages;
     uint8_t a[kStages][kHalf * kK * 2];
-    uint8_t b[kStages][kHalf * kK * 2];
+    uint8_t b[kStages][(kSolo ? kN : kHalf) * kK * 2];
     // full and acc_empty: of both blocks, the first one's; empty and acc_full: arrived at in both by the first one's products
     uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
     uint32_t tmem_base;
@@ -136,19 +140,21 @@ __device__ __forceinline__ int best_run(int row_tiles, int n_tiles, int pairs) {
 
 // Forward and dz: a run of vocabulary tiles of one row tile is a pair's unit.  Row tiles change fastest, so the pairs that
 // run beside each other read the same rows of W and every row of W leaves DRAM about once.
-struct RunWalk {
+template <bool kSolo> __device__ __forceinline__ int worker_id() { return kSolo ? (int)blockIdx.x : pair_id(); }
+template <bool kSolo> __device__ __forceinline__ int workers() { return kSolo ? (int)gridDim.x : pairs(); }
+template <bool kSolo> struct RunWalk {
     int unit, units, mt, run_len, n_tiles, kt, n, n_end, m, run;
     __device__ RunWalk(const Args& a, int count, int n_tiles_) : n_tiles(n_tiles_) {
         mt = row_tiles(count);
-        run_len = best_run(mt, n_tiles, pairs());
+        run_len = best_run(mt, n_tiles, workers<kSolo>());
         units = mt * ((n_tiles + run_len - 1) / run_len);
         kt = (a.d + kK - 1) / kK * a.terms;
-        unit = pair_id() - pairs();
+        unit = worker_id<kSolo>() - workers<kSolo>();
         n = n_end = 0;
     }
     __device__ bool next(Segment& s) {
         if (n >= n_end) {
-            unit += pairs();
+            unit += workers<kSolo>();
             if (unit >= units) return false;
             run = unit / mt;
             m = unit - run * mt;
@@ -246,12 +252,12 @@ struct SplitWalk {
         return true;
     }
 };
-template <int kMode> struct WalkOf { using type = RunWalk; };
-template <> struct WalkOf<kGradProducts> { using type = SplitWalk; };
-template <int kMode>
-__device__ __forceinline__ typename WalkOf<kMode>::type make_walk(const Args& a, int count) {
+template <int kMode, bool kSolo> struct WalkOf { using type = RunWalk<kSolo>; };
+template <> struct WalkOf<kGradProducts, false> { using type = SplitWalk; };
+template <int kMode, bool kSolo>
+__device__ __forceinline__ typename WalkOf<kMode, kSolo>::type make_walk(const Args& a, int count) {
     if constexpr (kMode == kGradProducts) return SplitWalk(a, count);
-    else return RunWalk(a, count, kMode == kStats ? a.n_tiles : a.vn_tiles);
+    else return RunWalk<kSolo>(a, count, kMode == kStats ? a.n_tiles : a.vn_tiles);
 }
 
 // ---- pairs of blocks ---------------------------------------------------------------------------
@@ -303,6 +309,13 @@ __device__ __forceinline__ void pair_commit_elect(uint64_t* bar) {
         : "memory");
 }
 
+// A tile into this block's shared memory; its bytes are counted at its own barrier.
+__device__ __forceinline__ void solo_load_3d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
 // A tile into this block's shared memory; its bytes are counted at the first block's barrier.
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, uint32_t bar, int c0, int c1, int c2) {
     asm volatile(
@@ -355,24 +368,37 @@ struct Maps {   // kStats, kGradLogits: a x, b W; kGradProducts: (a dz, b W) for
 };
 
 // ---- producer: one thread of either block ------------------------------------------------------
-template <int kMode>
-__device__ __forceinline__ bool produce(Smem& sm, const Maps& maps, const Args& a, int count) {
+template <int kMode, bool kSolo>
+__device__ __forceinline__ bool produce(Smem<kSolo>& sm, const Maps& maps, const Args& a, int count) {
+    constexpr int kStages = Smem<kSolo>::kStages;
     volatile int* ab = &sm.abort_flag;
-    auto walk = make_walk<kMode>(a, count);
+    auto walk = make_walk<kMode, kSolo>(a, count);
     Segment s;
     uint32_t it = 0;
-    const int rank = block_rank(), am = rank * kHalf, bn = rank * kHalf;
-    const uint32_t full0 = in_first(&sm.full[0]);
+    const int rank = kSolo ? 0 : block_rank(), am = rank * kHalf, bn = rank * kHalf;
+    const uint32_t full0 = kSolo ? 0 : in_first(&sm.full[0]);
     while (walk.next(s)) {
         Steps steps(a, s);
 #pragma unroll 1
         for (int k = s.k0; k < s.k1; k++, it++) {
             const int st = it % kStages;
             if (!mbar_wait_suspend(&sm.empty[st], (it / kStages & 1) ^ 1, ab, a.wait_ns)) return false;
-            // (few rows: the second block's half of them is empty, dx of two parts of dz apart: it takes the second part)
-            const bool part_each = kMode == kGradProducts && a.stacked && !s.dw, rows_here = !a.few || part_each || rank == 0;
+            if constexpr (kSolo) {
+                mbar_arrive_expect_tx(&sm.full[st], (a.x_rows + kN) * kK * 2);
+                int pa, pb;
+                term_planes(a, false, steps.term, pa, pb);
+                const int kc = steps.kc() * kK;
+                steps.next();
+                solo_load_3d(sm.a[st], &maps.a, &sm.full[st], kc, 0, pa);
+#pragma unroll
+                for (int j = 0; j < kN / kHalf; j++)
+                    solo_load_3d(sm.b[st] + j * kHalf * kK * 2, &maps.b, &sm.full[st], kc, a.v0 + s.n * kN + j * kHalf, pb);
+                continue;
+            }
+            // (dx of few rows: the second block has none, or takes the second part of dz)
+            const bool few = kMode == kGradProducts && a.few && !s.dw, part_each = few && a.stacked, rows_here = !few || part_each || rank == 0;
             if (rank == 0) {
-                const uint32_t rows = a.few && !(kMode == kGradProducts && s.dw) ? (part_each ? 2 : 1) * a.x_rows : 2 * kHalf;
+                const uint32_t rows = few ? (part_each ? 2 : 1) * a.x_rows : 2 * kHalf;
                 mbar_arrive_expect_tx(&sm.full[st], (rows + 2 * kHalf) * kK * 2);
             }
             const uint32_t full = full0 + st * 8;
@@ -381,7 +407,7 @@ __device__ __forceinline__ bool produce(Smem& sm, const Maps& maps, const Args& 
             const int kc = steps.kc() * kK;
             steps.next();
             if (kMode != kGradProducts) {
-                if (rows_here) tma_load_3d(sm.a[st], &maps.a, full, kc, s.m * kM + am, pa);
+                tma_load_3d(sm.a[st], &maps.a, full, kc, s.m * kM + am, pa);
                 tma_load_3d(sm.b[st], &maps.b, full, kc, a.v0 + s.n * kN + bn, pb);
             } else if (!s.dw) {
                 if (rows_here) tma_load_3d(sm.a[st], &maps.a, full, kc, part_each ? 0 : s.m * kM + am, part_each ? rank : pa);
@@ -404,10 +430,11 @@ __device__ __forceinline__ bool produce(Smem& sm, const Maps& maps, const Args& 
 }
 
 // ---- products: one warp of the first block -------------------------------------------------------
-template <int kMode>
-__device__ __forceinline__ bool multiply(Smem& sm, const Args& a, int count) {
+template <int kMode, bool kSolo>
+__device__ __forceinline__ bool multiply(Smem<kSolo>& sm, const Args& a, int count) {
+    constexpr int kStages = Smem<kSolo>::kStages;
     volatile int* ab = &sm.abort_flag;
-    auto walk = make_walk<kMode>(a, count);
+    auto walk = make_walk<kMode, kSolo>(a, count);
     Segment s;
     uint32_t it = 0, tile = 0;
     const uint32_t tm = sm.tmem_base;
@@ -415,7 +442,7 @@ __device__ __forceinline__ bool multiply(Smem& sm, const Args& a, int count) {
         // (a K-major row of a tile is 128 bytes: 16 columns are 32 bytes on; an MN-major one holds 64 rows of the operand: 16 of the
         // depth are 16 rows of 128 bytes on, the next 64 rows of the operand 8192 bytes)
         const bool a_mn = kMode == kGradProducts && s.dw, b_mn = kMode == kGradProducts;
-        const uint32_t idesc = umma_idesc_bf16(kM, kN, false, false) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+        const uint32_t idesc = umma_idesc_bf16(kSolo ? kHalf : kM, kN, false, false) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
         const uint32_t a_step = a_mn ? 2048 >> 4 : 32 >> 4, b_step = b_mn ? 2048 >> 4 : 32 >> 4;
         const uint32_t a_lbo = a_mn ? 8192 : 16, b_lbo = b_mn ? 8192 : 16;
         Steps steps(a, s);
@@ -428,12 +455,18 @@ __device__ __forceinline__ bool multiply(Smem& sm, const Args& a, int count) {
             tc_fence_after();
             const uint32_t da = desc_lo_sw128(smem_u32(sm.a[st]), a_lbo), db = desc_lo_sw128(smem_u32(sm.b[st]), b_lbo);
 #pragma unroll
-            for (int j = 0; j < kK / 16; j++)
-                pair_umma_elect(tm + acc * kN, da + j * a_step, db + j * b_step, idesc, !begins || j > 0);
-            pair_commit_elect(&sm.empty[st]);
+            for (int j = 0; j < kK / 16; j++) {
+                if constexpr (kSolo) umma_bf16_elect(tm + acc * kN, da + j * a_step, db + j * b_step, idesc, !begins || j > 0);
+                else pair_umma_elect(tm + acc * kN, da + j * a_step, db + j * b_step, idesc, !begins || j > 0);
+            }
+            auto commit = [](uint64_t* bar) {
+                if constexpr (kSolo) umma_commit_elect(bar);
+                else pair_commit_elect(bar);
+            };
+            commit(&sm.empty[st]);
             begins = (steps.next() && a.folds) || k + 1 == s.k1;
             if (begins) {
-                pair_commit_elect(&sm.acc_full[acc]);
+                commit(&sm.acc_full[acc]);
                 tile++;
             }
         }
@@ -525,14 +558,14 @@ __device__ __forceinline__ size_t slot_at(int slot, int warp, int chunk, int j4,
 }
 
 // kFold: the tile's sums come in folds and are added up here, in 128 registers a thread; else they are read from tensor memory as used.
-template <int kMode, bool kFold>
-__device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
+template <int kMode, bool kFold, bool kSolo>
+__device__ __forceinline__ bool finish(Smem<kSolo>& sm, const Args& a, int count) {
     volatile int* ab = &sm.abort_flag;
-    auto walk = make_walk<kMode>(a, count);
+    auto walk = make_walk<kMode, kSolo>(a, count);
     Segment s;
     const int warp = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31, quarter = warp & 3, half = warp >> 2;
-    const int rank = block_rank(), lrow = rank * kHalf + quarter * 32 + lane;   // row of the tile
-    const uint32_t acc_empty = in_first(&sm.acc_empty[0]);
+    const int rank = kSolo ? 0 : block_rank(), lrow = rank * kHalf + quarter * 32 + lane;   // row of the tile
+    const uint32_t acc_empty = kSolo ? smem_u32(&sm.acc_empty[0]) : in_first(&sm.acc_empty[0]);
     auto release = [&](int acc) {                        // of the accumulator: a lane of every warp
         tc_fence_before();
         __syncwarp();
@@ -706,18 +739,22 @@ __device__ __forceinline__ bool finish(Smem& sm, const Args& a, int count) {
 
 // The rows of W that the block's first tile reads, into L2 while the kernels before this one are under way (all that was there before the
 // call is done: index_rows_kernel).  With one row tile the first unit of a pair goes by its number alone.
+template <bool kSolo>
 __device__ __forceinline__ void request_first_tile(const Args& a) {
-    const int run = best_run(1, a.n_tiles, pairs()), row = pair_id() * run * kN + (int)block_rank() * kHalf + (int)(threadIdx.x & 31) * 4;
+    constexpr int kEach = kSolo ? kN / 32 : kHalf / 32;   // rows a lane
+    const int run = best_run(1, a.n_tiles, workers<kSolo>());
+    const int row = worker_id<kSolo>() * run * kN + (kSolo ? 0 : (int)block_rank() * kHalf) + (int)(threadIdx.x & 31) * kEach;
     const int bytes = (a.d * 2) & ~15;
-    for (int r = row; bytes && r < min(row + 4, a.V); r++)
+    for (int r = row; bytes && r < min(row + kEach, a.V); r++)
         asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.ahead + (size_t)r * a.ahead_stride), "r"(bytes) : "memory");
 }
 
-template <int kMode, bool kFold>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-product_kernel(const __grid_constant__ Maps maps, const Args a) {
+template <int kMode, bool kFold, bool kSolo>
+__device__ __forceinline__ void product_block(const Maps& maps, const Args& a) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+    using Sm = Smem<kSolo>;
+    Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
+    constexpr int kStages = Sm::kStages;
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         prefetch_tmap(&maps.a);
@@ -730,17 +767,20 @@ product_kernel(const __grid_constant__ Maps maps, const Args a) {
     }
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; i++) { mbar_init(&sm.full[i], 1); mbar_init(&sm.empty[i], 1); }
-        for (int i = 0; i < 2; i++) { mbar_init(&sm.acc_full[i], 1); mbar_init(&sm.acc_empty[i], 2 * kEpilogueWarps); }
+        for (int i = 0; i < 2; i++) { mbar_init(&sm.acc_full[i], 1); mbar_init(&sm.acc_empty[i], (kSolo ? 1 : 2) * kEpilogueWarps); }
         sm.abort_flag = 0;
         fence_barrier_init();
     }
-    if (warp == 1) pair_tmem_alloc(&sm.tmem_base);
+    if (warp == 1) {
+        if constexpr (kSolo) tmem_alloc(&sm.tmem_base, kTmemCols);
+        else pair_tmem_alloc(&sm.tmem_base);
+    }
     fence_proxy_async();
     tc_fence_before();
     __syncthreads();
-    cluster_sync();
+    if constexpr (!kSolo) cluster_sync();
     tc_fence_after();
-    if (kMode == kStats && a.ahead && warp == 2) request_first_tile(a);
+    if (kMode == kStats && a.ahead && warp == 2) request_first_tile<kSolo>(a);
     grid_launch_dependents();
     grid_dependency_wait();
     const int count = *a.count;
@@ -750,13 +790,13 @@ product_kernel(const __grid_constant__ Maps maps, const Args a) {
         if constexpr (kFold) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0) {
             asm volatile("fence.proxy.async.global;" ::: "memory");   // packed rows and dz were plain stores; TMA reads them
-            if ((threadIdx.x & 31) == 0 && !a.withhold) ok = produce<kMode>(sm, maps, a, count);
-        } else if (warp == 1 && block_rank() == 0) {
-            ok = multiply<kMode>(sm, a, count);
+            if ((threadIdx.x & 31) == 0 && !a.withhold) ok = produce<kMode, kSolo>(sm, maps, a, count);
+        } else if (warp == 1 && (kSolo || block_rank() == 0)) {
+            ok = multiply<kMode, kSolo>(sm, a, count);
         }
     } else {
         if constexpr (kFold) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-        ok = finish<kMode, kFold>(sm, a, count);
+        ok = finish<kMode, kFold, kSolo>(sm, a, count);
     }
     if (!ok) atomicCAS(a.status, 0, 400 + warp);
     __syncwarp();
@@ -767,8 +807,22 @@ product_kernel(const __grid_constant__ Maps maps, const Args a) {
         while (global_ns() - t0 < 2'000'000ull) __nanosleep(1000);
     }
     __syncthreads();
-    cluster_sync();
-    if (warp == 1) pair_tmem_dealloc(sm.tmem_base);
+    if constexpr (!kSolo) cluster_sync();
+    if (warp == 1) {
+        if constexpr (kSolo) tmem_dealloc(sm.tmem_base, kTmemCols);
+        else pair_tmem_dealloc(sm.tmem_base);
+    }
+}
+
+template <int kMode, bool kFold>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+product_kernel(const __grid_constant__ Maps maps, const Args a) {
+    product_block<kMode, kFold, false>(maps, a);
+}
+template <int kMode, bool kFold>
+__global__ void __launch_bounds__(kThreads, 1)
+solo_kernel(const __grid_constant__ Maps maps, const Args a) {
+    product_block<kMode, kFold, true>(maps, a);
 }
 
 // dx of the rows without a target is zero.  After a wait that ran out both gradients are NaN.
@@ -1019,7 +1073,7 @@ index_and_pack_kernel(const Index x, const T* src, int64_t stride, int64_t n_row
 // 61 rows with a thread per row and eighth of the runs: 28 us).
 constexpr int kJoinRows = 8;
 __global__ void __launch_bounds__(256)
-join_runs_kernel(const float2* part, int n_tiles, int pairs, int Tp, int* header, const int* rows, const int* words,
+join_runs_kernel(const float2* part, int n_tiles, int workers, int Tp, int* header, const int* rows, const int* words,
                  float* row_max, float* row_inv, const float* hit, float* loss, int reduction,
                  double* sums) {
     __shared__ float2 join[8][kJoinRows];
@@ -1028,7 +1082,7 @@ join_runs_kernel(const float2* part, int n_tiles, int pairs, int Tp, int* header
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.x * kJoinRows + (tid & 7);
     grid_launch_dependents();
     grid_dependency_wait();
-    const int count = header[0], run = best_run(row_tiles(count), n_tiles, pairs), n_parts = 2 * ((n_tiles + run - 1) / run);
+    const int count = header[0], run = best_run(row_tiles(count), n_tiles, workers), n_parts = 2 * ((n_tiles + run - 1) / run);
     const bool failed = header[1] != 0;
     float top = -INFINITY, sum = 0.f;
     auto add = [&](float2 p) {
@@ -1101,9 +1155,9 @@ struct Sizes {
     // scratch of the forward (W's planes if it is not read in place) and of the backward
     size_t w_planes, o_part, o_sums, fwd, o_dz, o_acc, o_slots, bwd;
 };
-// Up to this many rows the second block of a pair has none of its own: it loads none, and bf16's dz keeps 16 bits, in two parts.  (Where a row has
-// one large entry, its target's, that entry's rounding to 8 bits is all of the row's error; beyond, the rows' roundings average out and the products'
-// time shows.)  dx takes a part a block, W once, if its tiles are few and deep enough that every one of them is split.
+// Up to this many rows the second block of a pair would have none of its own: z is made by blocks by themselves (Smem), and bf16's dz keeps 16 bits, in
+// two parts.  (Where a row has one large entry, its target's, that entry's rounding to 8 bits is all of the row's error; beyond, the rows' roundings
+// average out and the products' time shows.)  dx takes a part a block, W once, if its rows of tiles are few and deep enough that every one is split.
 constexpr int kFewRows = kHalf;
 constexpr size_t kPieceBytes = 512ull << 20;   // of dz, beyond which the vocabulary is cut
 
@@ -1166,19 +1220,25 @@ bool make_map(CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int 
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int kMode, bool kFold> struct Tag {};
-template <int kMode, bool kFold>
+template <int kMode, bool kFold, bool kSolo> struct Tag {};
+template <int kMode, bool kFold, bool kSolo>
 int launch_as(const Maps& maps, const Args& a, int grid, cudaStream_t st) {
-    if (int rc = allow_smem<Tag<kMode, kFold>>((const void*)product_kernel<kMode, kFold>, sizeof(Smem))) return rc;
-    return launch_overlapped(product_kernel<kMode, kFold>, dim3(grid), dim3(kThreads), sizeof(Smem), st, maps, a);
+    void (*kernel)(Maps, Args);
+    if constexpr (kSolo) kernel = solo_kernel<kMode, kFold>;
+    else kernel = product_kernel<kMode, kFold>;
+    if (int rc = allow_smem<Tag<kMode, kFold, kSolo>>((const void*)kernel, sizeof(Smem<kSolo>))) return rc;
+    return launch_overlapped(kernel, dim3(grid), dim3(kThreads), sizeof(Smem<kSolo>), st, maps, a);
 }
+// workers: pairs, or blocks by themselves (few rows, not kGradProducts)
 template <int kMode>
-int launch_products(const Maps& maps, Args a, int grid, cudaStream_t st) {
+int launch_products(const Maps& maps, Args a, int workers, cudaStream_t st) {
     a.terms = a.planes == 3 ? kTerms3 : kMode == kGradProducts ? a.dz_planes : 1;
     // (two parts of dz: block by block, so that the other operand's comes from L2 the second time)
     a.group = a.planes == 3 ? kFold3 : kMode == kGradProducts ? 1 : kFoldLogits;
     a.folds = a.planes == 3 || (kMode != kGradProducts && a.group * kK < a.d);
-    return a.folds ? launch_as<kMode, true>(maps, a, grid, st) : launch_as<kMode, false>(maps, a, grid, st);
+    if constexpr (kMode != kGradProducts)
+        if (a.few) return a.folds ? launch_as<kMode, true, true>(maps, a, workers, st) : launch_as<kMode, false, true>(maps, a, workers, st);
+    return a.folds ? launch_as<kMode, true, false>(maps, a, 2 * workers, st) : launch_as<kMode, false, false>(maps, a, 2 * workers, st);
 }
 
 bool in_place(const void* w, int64_t stride, int dtype) {   // a matrix that TMA reads as it lies
@@ -1275,9 +1335,9 @@ extern "C" int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, con
         a.ahead = static_cast<const __nv_bfloat16*>(w);
         a.ahead_stride = w_row_stride;
     }
-    const int pairs = (int)std::min<int64_t>((int64_t)(s.Tp / ce::kM) * s.n_tiles, sms / 2);
-    if (int rc = ce::launch_products<ce::kStats>(maps, a, 2 * pairs, st)) return rc;
-    return launch_overlapped(ce::join_runs_kernel, dim3(s.Tp / ce::kJoinRows), dim3(256), 0, st, a.part, s.n_tiles, pairs, s.Tp, header, a.rows, a.target,
+    const int workers = (int)std::min<int64_t>((int64_t)(s.Tp / ce::kM) * s.n_tiles, a.few ? sms : sms / 2);
+    if (int rc = ce::launch_products<ce::kStats>(maps, a, workers, st)) return rc;
+    return launch_overlapped(ce::join_runs_kernel, dim3(s.Tp / ce::kJoinRows), dim3(256), 0, st, a.part, s.n_tiles, workers, s.Tp, header, a.rows, a.target,
                              a.row_max, a.row_inv, a.hit, loss, reduction, reinterpret_cast<double*>(ws + s.o_sums));
 }
 
@@ -1332,8 +1392,8 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
         a.stacked = s.dz_planes == 2 && (a.vn + ce::kK - 1) / ce::kK >= ce::kSplitDepth && 2 * (s.d_tiles / wide) + 2 <= sms / 2 / wide;
         a.first = p == 0;
         a.last = p + 1 == s.pieces;
-        if (int rc = ce::launch_products<ce::kGradLogits>(logits, a, sms / 2 * 2, st)) return rc;
-        if (int rc = ce::launch_products<ce::kGradProducts>(grads, a, sms / 2 * 2, st)) return rc;
+        if (int rc = ce::launch_products<ce::kGradLogits>(logits, a, a.few ? sms : sms / 2, st)) return rc;
+        if (int rc = ce::launch_products<ce::kGradProducts>(grads, a, sms / 2, st)) return rc;
         a.terms = s.f32 ? ce::kTerms3 : s.dz_planes;
         if (int rc = launch_overlapped(ce::join_split_kernel, dim3(4 * sms), dim3(256), 0, st, a, sms / 2)) return rc;
     }
