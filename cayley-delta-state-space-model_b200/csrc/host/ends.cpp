@@ -55,10 +55,11 @@ CeOut ce_forward(const Tensor& hidden, const Tensor& weight, const Tensor& targe
         if (reduction != CDSSM_CE_NONE) loss.fill_(reduction == CDSSM_CE_MEAN ? NAN : 0.0);
         return {loss, scratch(0, hidden)};
     }
-    const size_t sb = cdssm_b200_linear_ce_saved_bytes(rows, (int)d, (int)vocab, dt);
+    const Tensor w = table(weight);
+    const size_t sb = cdssm_b200_linear_ce_saved_bytes(rows, (int)d, (int)vocab, cptr(w), row_stride(w), dt);
     if (sb == 0) check(CDSSM_ERR_UNSUPPORTED, "linear_cross_entropy");
     const size_t wb = cdssm_b200_linear_ce_workspace_bytes(rows, (int)d, (int)vocab, dt, 0);
-    const Tensor x = row_matrix(hidden, d), w = table(weight), y = targets.contiguous(), ws = scratch(wb, hidden), saved = scratch(sb, hidden);
+    const Tensor x = row_matrix(hidden, d), y = targets.contiguous(), ws = scratch(wb, hidden), saved = scratch(sb, hidden);
     check(cdssm_b200_linear_ce_fwd(cptr(x), row_stride(x), cptr(w), row_stride(w), y.const_data_ptr<int64_t>(), fmut(loss), mptr(saved), sb, mptr(ws),
                                    wb, rows, (int)d, (int)vocab, ignore, (int)reduction, dt, (int)flags, stream_of(x)),
           "linear_cross_entropy");

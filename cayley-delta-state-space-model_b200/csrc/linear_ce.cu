@@ -12,9 +12,14 @@
 // own rounding to bf16 does not shift all of a gradient the same way.
 //
 // All products are tcgen05 ones of TMA tiles by pairs of blocks: 256 x 256 outputs, each block loads half of both operands and keeps 128
-// rows of the result, fp32 accumulators, two of them in tensor memory so that the epilogue of a tile runs beside the products of the next.  float32 operands enter as three bf16 parts (exact to 24 bits) and six of
-// the nine part products, the small ones first.  The tensor cores' float32 sums are cut off, not rounded, so that the error of a long sum
-// grows with its length: sums that must be good to float32 are folded into registers every so many steps (kFoldLogits, kFold3).
+// rows of the result, fp32 accumulators, two of them in tensor memory so that the epilogue of a tile runs beside the products of the next.
+// float32 operands enter as three bf16 parts (exact to 24 bits) and six of the nine part products, the small ones first.  The tensor
+// cores' float32 sums are cut off, not rounded, so that the error of a long sum grows with its length: sums that must be good to float32
+// are folded into registers every so many steps (kFoldLogits, kFold3).
+//
+// What bounds it: with many rows the power cap.  8 x 2048 rows of width 768: losses of 32000 words 567 us, 1.42 PFLOP/s (the library's products keep
+// up 1.39), a training step of 50257 words with an eighth of the rows ignored 3.14 to 3.67 ms by GPU, 1.21 to 1.41 PFLOP/s of its four products; tensor pipe
+// busy 83 / 83 / 81 % in losses / dz / dx and dW.  With few rows the dependent launches and W's way: 61 rows, 50257 words: 25 us, W alone 12.
 #include "cdssm_common.cuh"
 #include "sm100_ptx.cuh"
 #include "tile_map.cuh"
@@ -1150,10 +1155,10 @@ struct Sizes {
     int64_t rows;
     int d, V, planes, dz_planes, Tp, pitch, n_tiles, pieces, vn, d_tiles;
     bool f32;
-    // saved
-    size_t o_rows, o_words, o_max, o_inv, o_hit, o_x, saved;
-    // scratch of the forward (W's planes if it is not read in place) and of the backward
-    size_t w_planes, o_part, o_sums, fwd, o_dz, o_acc, o_slots, bwd;
+    // saved, without and with W's parts (a W that is not read in place: the backward needs them as well, which mostly follows at once)
+    size_t o_rows, o_words, o_max, o_inv, o_hit, o_x, o_w, saved, saved_w;
+    // scratch of the forward and of the backward
+    size_t o_part, o_sums, fwd, o_dz, o_acc, o_slots, bwd;
 };
 // Up to this many rows the second block of a pair would have none of its own: z is made by blocks by themselves (Smem), and bf16's dz keeps 16 bits, in
 // two parts.  (Where a row has one large entry, its target's, that entry's rounding to 8 bits is all of the row's error; beyond, the rows' roundings
@@ -1181,11 +1186,12 @@ bool sizes_of(int64_t rows, int d, int vocab, int dtype, int sms, Sizes& s) {
     s.o_rows = take(4ull * s.Tp); s.o_words = take(4ull * s.Tp); s.o_max = take(4ull * s.Tp); s.o_inv = take(4ull * s.Tp);
     s.o_hit = take(4ull * s.Tp); s.o_x = take(2ull * s.planes * s.Tp * s.pitch);
     s.saved = o;
-    s.w_planes = up(2ull * s.planes * (size_t)vocab * s.pitch, 256);
-    o = s.w_planes;
+    s.o_w = take(2ull * s.planes * (size_t)vocab * s.pitch);
+    s.saved_w = o;
+    o = 0;
     s.o_part = take(8ull * 2 * s.n_tiles * s.Tp); s.o_sums = take(8ull * (s.Tp / kJoinRows));
     s.fwd = o;
-    o = s.w_planes;
+    o = 0;
     s.o_dz = take(column * s.vn); s.o_acc = take(s.pieces > 1 ? 4ull * s.Tp * s.d_tiles * kN : 0);
     s.o_slots = take(2ull * (sms / 2) * kM * kN * 4);
     s.bwd = o;
@@ -1287,9 +1293,10 @@ void fill_saved(Args& a, const Sizes& s, char* saved) {
 
 using namespace cdssm;
 
-extern "C" size_t cdssm_b200_linear_ce_saved_bytes(int64_t rows, int d, int vocab, int dtype) {
+extern "C" size_t cdssm_b200_linear_ce_saved_bytes(int64_t rows, int d, int vocab, const void* w, int64_t w_row_stride, int dtype) {
     ce::Sizes s;
-    return ce::checked_sizes(rows, d, vocab, dtype, s) == CDSSM_OK ? s.saved : 0;
+    if (ce::checked_sizes(rows, d, vocab, dtype, s) != CDSSM_OK) return 0;
+    return ce::in_place(w, w_row_stride, dtype) ? s.saved : s.saved_w;
 }
 extern "C" size_t cdssm_b200_linear_ce_workspace_bytes(int64_t rows, int d, int vocab, int dtype, int backward) {
     ce::Sizes s;
@@ -1303,7 +1310,8 @@ extern "C" int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, con
     if (x_row_stride < 0 || w_row_stride < d) return CDSSM_ERR_BAD_ARG;
     ce::Sizes s;
     if (int rc = ce::checked_sizes(rows, d, vocab, dtype, s)) return rc;
-    if (saved_bytes < s.saved || workspace_bytes < s.fwd || ((uintptr_t)saved & 255) || ((uintptr_t)workspace & 255)) return CDSSM_ERR_WORKSPACE;
+    const bool direct = ce::in_place(w, w_row_stride, dtype);
+    if (saved_bytes < (direct ? s.saved : s.saved_w) || workspace_bytes < s.fwd || ((uintptr_t)saved & 255) || ((uintptr_t)workspace & 255)) return CDSSM_ERR_WORKSPACE;
     const cudaStream_t st = (cudaStream_t)stream;
     int sms = 0;
     if (int rc = sm_count(sms)) return rc;
@@ -1321,13 +1329,12 @@ extern "C" int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, con
             return rc;
         if (int rc = ce::pack_any(x, x_row_stride, a.rows, a.count, s.Tp, s, sv + s.o_x, st)) return rc;
     }
-    const bool direct = ce::in_place(w, w_row_stride, dtype);
     if (!direct)
-        if (int rc = ce::pack_any(w, w_row_stride, nullptr, nullptr, vocab, s, ws, st)) return rc;
+        if (int rc = ce::pack_any(w, w_row_stride, nullptr, nullptr, vocab, s, sv + s.o_w, st)) return rc;
     if (int rc = ce::bind_context()) return rc;
     ce::Maps maps{};
     if (!ce::make_map(&maps.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, a.x_rows) ||
-        !ce::make_map(&maps.b, direct ? w : ws, direct ? d : s.pitch, vocab, s.planes, direct ? w_row_stride : s.pitch, ce::kK, ce::kHalf))
+        !ce::make_map(&maps.b, direct ? w : sv + s.o_w, direct ? d : s.pitch, vocab, s.planes, direct ? w_row_stride : s.pitch, ce::kK, ce::kHalf))
         return CDSSM_ERR_CUDA;
     a.part = reinterpret_cast<float2*>(ws + s.o_part);
     a.withhold = (flags & CDSSM_SCAN_TEST_WITHHOLD) != 0;
@@ -1349,15 +1356,13 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
     if (w_row_stride < d || ((uintptr_t)grad_x & 15) || ((uintptr_t)grad_w & 15)) return CDSSM_ERR_BAD_ARG;
     ce::Sizes s;
     if (int rc = ce::checked_sizes(rows, d, vocab, dtype, s)) return rc;
-    if (saved_bytes < s.saved || workspace_bytes < s.bwd || ((uintptr_t)saved & 255) || ((uintptr_t)workspace & 255)) return CDSSM_ERR_WORKSPACE;
+    const bool direct = ce::in_place(w, w_row_stride, dtype);
+    if (saved_bytes < (direct ? s.saved : s.saved_w) || workspace_bytes < s.bwd || ((uintptr_t)saved & 255) || ((uintptr_t)workspace & 255)) return CDSSM_ERR_WORKSPACE;
     const cudaStream_t st = (cudaStream_t)stream;
     int sms = 0;
     if (int rc = sm_count(sms)) return rc;
     char *const sv = static_cast<char*>(saved), *const ws = static_cast<char*>(workspace);
-    const bool direct = ce::in_place(w, w_row_stride, dtype);
-    if (!direct)
-        if (int rc = ce::pack_any(w, w_row_stride, nullptr, nullptr, vocab, s, ws, st)) return rc;
-    const void* const wb = direct ? w : ws;
+    const void* const wb = direct ? w : sv + s.o_w;
     const int64_t w_cols = direct ? d : s.pitch, w_pitch = direct ? w_row_stride : s.pitch;
     ce::Args a;
     ce::fill_saved(a, s, sv);

@@ -214,8 +214,9 @@ class CdssmLM:
         if targets is None:
             targets = torch.full_like(ids, ignore_index, dtype=torch.int64)
             targets[:, :-1] = ids[:, 1:]
+        targets = self._ids(targets).to(device=self.device, dtype=torch.int64)
         hidden = ops._lib.host().lm_hidden(self._native(), ids, self.per_token_group_norm, scan_flags)
-        return ops.linear_cross_entropy(hidden, self.embedding, self._ids(targets), ignore_index=ignore_index, reduction=reduction)
+        return ops.linear_cross_entropy(hidden, self.embedding, targets, ignore_index=ignore_index, reduction=reduction)
 
     @torch.no_grad()
     def prefill(self, input_ids, last_only=True):

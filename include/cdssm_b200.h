@@ -450,7 +450,8 @@ CDSSM_API int cdssm_b200_decode_step_reference(float* local_state, float* correc
  * reduction: CDSSM_CE_NONE loss (rows), CDSSM_CE_MEAN (over the rows that take part; NaN without any) or CDSSM_CE_SUM one value;
  * loss is float32.  A row whose target is neither a word nor ignore_index loses NaN.
  * saved (cdssm_b200_linear_ce_saved_bytes) is what the backward reads: keep it as it is, 256-byte aligned, as the workspace
- * (cdssm_b200_linear_ce_workspace_bytes), which is free again behind the call.  Both sizes are for the current device, 0 on
+ * (cdssm_b200_linear_ce_workspace_bytes), which is free again behind the call.  It holds the rows that take part and, for a w that is not
+ * read in place (float32, or rows that are not 16-byte aligned), w's bf16 parts: 6 or 2 bytes a value.  Both sizes are for the current device, 0 on
  * bad sizes.  rows <= 2^24, vocab <= 2^24, d <= 65536.  bf16 products with float32 sums; float32 operands enter as three bf16 parts.
  * flags: 0 or CDSSM_SCAN_TEST_WITHHOLD.  After a bounded wait that ran out the loss and its
  * gradients are NaN.
@@ -458,7 +459,7 @@ CDSSM_API int cdssm_b200_decode_step_reference(float* local_state, float* correc
 #define CDSSM_CE_NONE 0
 #define CDSSM_CE_MEAN 1
 #define CDSSM_CE_SUM 2
-CDSSM_API size_t cdssm_b200_linear_ce_saved_bytes(int64_t rows, int d, int vocab, int dtype);
+CDSSM_API size_t cdssm_b200_linear_ce_saved_bytes(int64_t rows, int d, int vocab, const void* w, int64_t w_row_stride, int dtype);
 CDSSM_API size_t cdssm_b200_linear_ce_workspace_bytes(int64_t rows, int d, int vocab, int dtype, int backward);
 CDSSM_API int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, const void* w, int64_t w_row_stride,
                                        const int64_t* target, float* loss, void* saved, size_t saved_bytes, void* workspace,

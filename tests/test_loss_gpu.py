@@ -321,6 +321,7 @@ def test_model_loss(ops, dtype):
     assert got.shape == (3, 70) and (got[:, -1] == 0).all() and (got[:, :-1].double() - rows).abs().max() <= tol
     assert abs(float(lm.loss(ids)) - float(rows.mean())) <= tol
     assert torch.equal(lm.loss(ids, torch.roll(ids, -1, 1), reduction="none")[:, :-1], got[:, :-1])
+    assert torch.equal(lm.loss(ids.cpu(), reduction="none"), got) and torch.equal(lm.loss(ids.tolist(), reduction="none"), got)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
