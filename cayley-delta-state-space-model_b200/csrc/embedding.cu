@@ -111,7 +111,8 @@ __device__ __forceinline__ int block_scan(int x, int* warp_total) {
     return before + scan - x;
 }
 
-// One cluster sorts (key, token) pairs by key, stable, `bits` bits a pass, each block a contiguous part of the pairs.  Ids that take no part (no row of the table, `skip`) get the key vocab: behind all others.
+// One cluster sorts (key, token) pairs by key, stable, `bits` bits a pass, each block a contiguous part of the pairs.  Ids that take no part
+// (no row of the table, `skip`) get the key vocab: behind all others.
 __global__ void __launch_bounds__(kSortThreads)
 sort_kernel(const int64_t* ids, int n, int vocab, int64_t skip, int bits, int passes, uint2* buf0, uint2* buf1, int* spans) {
     extern __shared__ __align__(16) unsigned char sort_smem[];
@@ -555,7 +556,8 @@ extern "C" int cdssm_b200_embedding_bwd(const int64_t* ids, const void* grad, vo
     if (int rc = counted(check_cuda(cudaLaunchKernelEx(&cfg, emb::sort_kernel, ids, (int)n, vocab, padding_idx, per_pass, passes, b0, b1,
                                                        reinterpret_cast<int*>(ws + l.spans)))))
         return rc;
-    const size_t bytes = (size_t)vocab * d * (dtype == CDSSM_BF16 ? 2 : 4), vecs = bytes / 16, blocks = std::max<size_t>(1, (vecs + emb::kSortThreads - 1) / emb::kSortThreads);
+    const size_t bytes = (size_t)vocab * d * (dtype == CDSSM_BF16 ? 2 : 4), vecs = bytes / 16;
+    const size_t blocks = std::max<size_t>(1, (vecs + emb::kSortThreads - 1) / emb::kSortThreads);
     if (blocks > 0x7fffffff) return CDSSM_ERR_UNSUPPORTED;
     if (int rc = launch_overlapped(emb::clear_kernel, dim3((unsigned)blocks), dim3(emb::kSortThreads), 0, st, static_cast<uint4*>(grad_w), vecs,
                                    static_cast<unsigned char*>(grad_w) + vecs * 16, (int)(bytes % 16)))

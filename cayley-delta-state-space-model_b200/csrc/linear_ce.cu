@@ -595,7 +595,8 @@ __device__ __forceinline__ bool finish(Smem<kSolo>& sm, const Args& a, int count
             }
         }
         const bool part_each = kMode == kGradProducts && a.stacked && !s.dw;
-        const bool idle = s.m * kM + (part_each ? 0 : rank * kHalf) + quarter * 32 >= (kMode == kStats ? count : summed_rows(count));   // nobody reads the warp's rows
+        // whether nobody reads the warp's rows
+        const bool idle = s.m * kM + (part_each ? 0 : rank * kHalf) + quarter * 32 >= (kMode == kStats ? count : summed_rows(count));
         float folded[kFold ? 128 : 1] = {};
         int acc = tile & 1;
         if constexpr (kFold) {
