@@ -4,6 +4,7 @@
 """
 from . import _lib, ops  # noqa: F401
 from .ops import (CUDAConv1dSiLUOp, DynamicsFusedFn, NormalizeKQFn, IntraChunkScanFn,  # noqa: F401
-                  InterChunkScanFn, ExactCorrectionFn, scan_fused, decode_step, CdssmError)
+                  InterChunkScanFn, ExactCorrectionFn, scan_fused, decode_step, embedding, linear_cross_entropy,
+                  grad_norm, clip_grads_, clip_grad_norm_, CdssmError)
 
 __version__ = "0.1.0"

@@ -9,7 +9,9 @@
 // type into scratch, then both products that read it in one launch.  Rows without a target are left out before the first product.
 //
 // Where all rows have one upstream gradient (mean, sum) it is a factor of dx and dW, not of dz: dz holds p - [v = y] then, and a factor's
-// own rounding to bf16 does not shift all of a gradient the same way.
+// own rounding to bf16 does not shift all of a gradient the same way.  Where every row has its own, it is a factor of dx's rows and, in two bf16
+// parts, of the x in dW: dz's one large entry of a row, near -1, is hardly rounded at all so (gradients off by 2.0e-3 of themselves instead of 2.5e-3,
+// their own rounding 1.7e-3; a quarter more products).  float32, and bf16 of few rows, whose dz keeps more bits, have it in dz.
 //
 // All products are tcgen05 ones of TMA tiles by pairs of blocks: 256 x 256 outputs, each block loads half of both operands and keeps 128
 // rows of the result, fp32 accumulators, two of them in tensor memory so that the epilogue of a tile runs beside the products of the next.
@@ -61,9 +63,10 @@ struct Args {
     float* hit;                  // (Tp) z of the target
     float2* part;                // (2 x runs, Tp) maximum and sum of a run of tiles, of either half of its columns
     const float* grad;           // upstream gradient: one value, or one a row of the caller
-    int grad_rows, mean;
+    int grad_rows, mean, row_factor;   // one a row; a mean's; one a row that is no factor of dz
     int planes, dz_planes;
-    int terms, group, folds;     // part products; depth blocks that go through all of them together; whether a group's sum is folded
+    int terms, terms_dx;         // part products, of dx
+    int group, folds;            // depth blocks that go through all of them together; whether a group's sum is folded
     int few, x_rows, stacked;    // see kFewRows: whether there are few rows; the rows that are loaded; dx of both parts of dz in one product
     int Tp, d, V;
     int n_tiles;                 // forward: vocabulary tiles
@@ -96,10 +99,10 @@ template <bool kSolo> struct __align__(1024) Smem {
     int abort_flag;
 };
 
-__device__ __forceinline__ void term_planes(const Args& a, bool of_dz, int term, int& pa, int& pb) {
+__device__ __forceinline__ void term_planes(const Args& a, bool of_dz, bool of_dw, int term, int& pa, int& pb) {
     constexpr uint32_t ta = 2u | 0u << 2 | 1u << 4 | 1u << 6 | 0u << 8 | 0u << 10, tb = 0u | 2u << 2 | 1u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
-    pa = a.planes == 3 ? (ta >> (2 * term)) & 3 : of_dz ? a.dz_planes - 1 - term : 0;
-    pb = a.planes == 3 ? (tb >> (2 * term)) & 3 : 0;
+    pa = a.planes == 3 ? (ta >> (2 * term)) & 3 : of_dz && !a.row_factor ? a.dz_planes - 1 - term : 0;
+    pb = a.planes == 3 ? (tb >> (2 * term)) & 3 : of_dw && a.row_factor ? 1 - term : 0;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -219,7 +222,7 @@ struct SplitTiles {
 };
 __device__ __forceinline__ SplitTiles split_tiles(const Args& a, int count, int pairs) {
     const int mt = row_tiles(count);
-    return SplitTiles(a.dx ? mt : 0, a.dw ? (a.vn + kM - 1) / kM : 0, a.d_tiles, (a.vn + kK - 1) / kK * (a.stacked ? 1 : a.terms),
+    return SplitTiles(a.dx ? mt : 0, a.dw ? (a.vn + kM - 1) / kM : 0, a.d_tiles, (a.vn + kK - 1) / kK * a.terms_dx,
                       summed_rows(count) / kK * a.terms, pairs, a.stacked);
 }
 struct SplitWalk {
@@ -342,7 +345,7 @@ __device__ __forceinline__ void store_sector(void* p, const uint32_t (&w)[8]) {
 struct Steps {
     int depth, terms, group;
     int base, n, i, term;   // of the present group: where it begins, its blocks, the block, the part product
-    __device__ Steps(const Args& a, const Segment& s) : terms(a.stacked && !s.dw ? 1 : a.terms), group(a.group) {
+    __device__ Steps(const Args& a, const Segment& s) : terms(s.dw ? a.terms : a.terms_dx), group(a.group) {
         const int k0 = s.k0, kt = s.kt;
         depth = terms == 1 ? kt : kt / terms;
         const int g = k0 / (group * terms), r = k0 - g * group * terms;
@@ -391,7 +394,7 @@ __device__ __forceinline__ bool produce(Smem<kSolo>& sm, const Maps& maps, const
             if constexpr (kSolo) {
                 mbar_arrive_expect_tx(&sm.full[st], (a.x_rows + kN) * kK * 2);
                 int pa, pb;
-                term_planes(a, false, steps.term, pa, pb);
+                term_planes(a, false, false, steps.term, pa, pb);
                 const int kc = steps.kc() * kK;
                 steps.next();
                 solo_load_3d(sm.a[st], &maps.a, &sm.full[st], kc, 0, pa);
@@ -407,8 +410,8 @@ __device__ __forceinline__ bool produce(Smem<kSolo>& sm, const Maps& maps, const
                 mbar_arrive_expect_tx(&sm.full[st], (rows + 2 * kHalf) * kK * 2);
             }
             const uint32_t full = full0 + st * 8;
-            int pa, pb;
-            term_planes(a, kMode == kGradProducts, steps.term, pa, pb);
+            int pa = 0, pb = 0;
+            if (steps.terms > 1) term_planes(a, kMode == kGradProducts, kMode == kGradProducts && s.dw, steps.term, pa, pb);
             const int kc = steps.kc() * kK;
             steps.next();
             if (kMode != kGradProducts) {
@@ -549,9 +552,11 @@ __device__ __forceinline__ void emit(const Args& a, int count, float factor, int
         for (int j = 0; j < kCols; j += 4) *reinterpret_cast<float4*>(acc + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
         return;
     }
+    const int to = a.rows[row];
+    if (a.row_factor) factor = a.grad[to];
 #pragma unroll
     for (int j = 0; j < kCols; j++) v[j] *= factor;
-    const size_t at = (size_t)a.rows[row] * a.d;
+    const size_t at = (size_t)to * a.d;
     if (a.f32) store_row(static_cast<float*>(a.dx) + at, col, a.d, v, a.whole_sectors);
     else store_row(static_cast<__nv_bfloat16*>(a.dx) + at, col, a.d, v, a.whole_sectors);
 }
@@ -591,7 +596,7 @@ __device__ __forceinline__ bool finish(Smem<kSolo>& sm, const Args& a, int count
                 mx = a.row_max[row];
                 inv = a.row_inv[row];
                 g = 0.f;
-                if (row < count) g = target == -2 ? NAN : a.grad_rows ? a.grad[a.rows[row]] : 1.f;   // (-2: a target that is no word)
+                if (row < count) g = target == -2 ? NAN : a.grad_rows && !a.row_factor ? a.grad[a.rows[row]] : 1.f;   // (-2: no word)
             }
         }
         const bool part_each = kMode == kGradProducts && a.stacked && !s.dw;
@@ -1074,6 +1079,33 @@ index_and_pack_kernel(const Index x, const T* src, int64_t stride, int64_t n_row
     pack_row<T, kPlanes>(mine[warp] < 0 ? nullptr : src + mine[warp] * stride, out + r * pitch, n_rows * (int64_t)pitch, d, pitch, vec);
 }
 
+// Packed bf16 rows times their upstream gradients, in two parts, a warp each.
+__global__ void __launch_bounds__(256)
+scale_rows_kernel(const __nv_bfloat16* x, const int* rows, const int* count, const float* grad, int Tp, int pitch, __nv_bfloat16* out) {
+    const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    grid_launch_dependents();
+    grid_dependency_wait();
+    if (r >= summed_rows(*count)) return;
+    const int from = rows[r];
+    const float g = from < 0 ? 0.f : grad[from];
+    const uint4* const src = reinterpret_cast<const uint4*>(x + r * pitch);
+    uint4* const dst = reinterpret_cast<uint4*>(out + r * pitch);
+    uint4* const rest = reinterpret_cast<uint4*>(out + (Tp + r) * pitch);
+    for (int i = threadIdx.x & 31; i < pitch / 8; i += 32) {
+        const uint4 u = src[i];
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float a = from < 0 ? 0.f : __uint_as_float(w[e] << 16) * g, b = from < 0 ? 0.f : __uint_as_float(w[e] & 0xffff0000u) * g;
+            hi[e] = pack2(a, b);
+            lo[e] = pack2(a - __uint_as_float(hi[e] << 16), b - __uint_as_float(hi[e] & 0xffff0000u));
+        }
+        dst[i] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        rest[i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+}
+
 // Joins the runs of a row: m, 1 / s and the loss, and (mean, sum) the losses' sum: every block leaves its own, the last one to come adds
 // them up in their order.  Eight rows a block, 32 threads a row: a call of few rows has few of them and hundreds of runs each (400 runs of
 // 61 rows with a thread per row and eighth of the runs: 28 us).
@@ -1159,7 +1191,7 @@ struct Sizes {
     // saved, without and with W's parts (a W that is not read in place: the backward needs them as well, which mostly follows at once)
     size_t o_rows, o_words, o_max, o_inv, o_hit, o_x, o_w, saved, saved_w;
     // scratch of the forward and of the backward
-    size_t o_part, o_sums, fwd, o_dz, o_acc, o_slots, bwd;
+    size_t o_part, o_sums, fwd, o_dz, o_acc, o_slots, o_scaled, bwd;
 };
 // Up to this many rows the second block of a pair would have none of its own: z is made by blocks by themselves (Smem), and bf16's dz keeps 16 bits, in
 // two parts.  (Where a row has one large entry, its target's, that entry's rounding to 8 bits is all of the row's error; beyond, the rows' roundings
@@ -1195,6 +1227,7 @@ bool sizes_of(int64_t rows, int d, int vocab, int dtype, int sms, Sizes& s) {
     o = 0;
     s.o_dz = take(column * s.vn); s.o_acc = take(s.pieces > 1 ? 4ull * s.Tp * s.d_tiles * kN : 0);
     s.o_slots = take(2ull * (sms / 2) * kM * kN * 4);
+    s.o_scaled = take(s.dz_planes == 1 ? 2ull * 2 * s.Tp * s.pitch : 0);
     s.bwd = o;
     return true;
 }
@@ -1236,10 +1269,14 @@ int launch_as(const Maps& maps, const Args& a, int grid, cudaStream_t st) {
     if (int rc = allow_smem<Tag<kMode, kFold, kSolo>>((const void*)kernel, sizeof(Smem<kSolo>))) return rc;
     return launch_overlapped(kernel, dim3(grid), dim3(kThreads), sizeof(Smem<kSolo>), st, maps, a);
 }
+void set_terms(Args& a, bool grad_products) {
+    a.terms = a.planes == 3 ? kTerms3 : !grad_products ? 1 : a.row_factor ? 2 : a.dz_planes;
+    a.terms_dx = a.planes != 3 && (a.row_factor || a.stacked) ? 1 : a.terms;
+}
 // workers: pairs, or blocks by themselves (few rows, not kGradProducts)
 template <int kMode>
 int launch_products(const Maps& maps, Args a, int workers, cudaStream_t st) {
-    a.terms = a.planes == 3 ? kTerms3 : kMode == kGradProducts ? a.dz_planes : 1;
+    set_terms(a, kMode == kGradProducts);
     // (two parts of dz: block by block, so that the other operand's comes from L2 the second time)
     a.group = a.planes == 3 ? kFold3 : kMode == kGradProducts ? 1 : kFoldLogits;
     a.folds = a.planes == 3 || (kMode != kGradProducts && a.group * kK < a.d);
@@ -1367,6 +1404,7 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
     const int64_t w_cols = direct ? d : s.pitch, w_pitch = direct ? w_row_stride : s.pitch;
     ce::Args a;
     ce::fill_saved(a, s, sv);
+    a.row_factor = reduction == CDSSM_CE_NONE && s.dz_planes == 1;
     if (int rc = ce::bind_context()) return rc;
     ce::Maps logits{}, grads{};
     if (!ce::make_map(&logits.a, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, ce::kK, a.x_rows) ||
@@ -1374,7 +1412,7 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
         !ce::make_map(&grads.a, ws + s.o_dz, s.vn, s.Tp, s.dz_planes, s.vn, ce::kK, a.x_rows) ||
         !ce::make_map(&grads.b, wb, w_cols, vocab, s.planes, w_pitch, 64, ce::kK) ||
         !ce::make_map(&grads.a2, ws + s.o_dz, s.vn, s.Tp, s.dz_planes, s.vn, 64, ce::kK) ||
-        !ce::make_map(&grads.b2, sv + s.o_x, s.pitch, s.Tp, s.planes, s.pitch, 64, ce::kK))
+        !ce::make_map(&grads.b2, a.row_factor ? ws + s.o_scaled : sv + s.o_x, s.pitch, s.Tp, a.row_factor ? 2 : s.planes, s.pitch, 64, ce::kK))
         return CDSSM_ERR_CUDA;
     a.grad = grad_loss;
     a.grad_rows = reduction == CDSSM_CE_NONE;
@@ -1390,6 +1428,10 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
     a.acc_pitch = s.d_tiles * ce::kN;
     a.slots = reinterpret_cast<float4*>(ws + s.o_slots);
     a.withhold = (flags & CDSSM_SCAN_TEST_WITHHOLD) != 0;
+    if (a.row_factor && grad_w)
+        if (int rc = launch_overlapped(ce::scale_rows_kernel, dim3(s.Tp / 8), dim3(256), 0, st, reinterpret_cast<const __nv_bfloat16*>(sv + s.o_x), a.rows,
+                                       a.count, grad_loss, s.Tp, s.pitch, reinterpret_cast<__nv_bfloat16*>(ws + s.o_scaled)))
+            return rc;
     for (int p = 0; p < s.pieces; p++) {
         a.v0 = p * s.vn;
         a.vn = std::min(s.vn, vocab - a.v0);
@@ -1400,7 +1442,7 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
         a.last = p + 1 == s.pieces;
         if (int rc = ce::launch_products<ce::kGradLogits>(logits, a, a.few ? sms : sms / 2, st)) return rc;
         if (int rc = ce::launch_products<ce::kGradProducts>(grads, a, sms / 2, st)) return rc;
-        a.terms = s.f32 ? ce::kTerms3 : s.dz_planes;
+        ce::set_terms(a, true);
         if (int rc = launch_overlapped(ce::join_split_kernel, dim3(4 * sms), dim3(256), 0, st, a, sms / 2)) return rc;
     }
     return CDSSM_OK;

@@ -6,7 +6,7 @@ Tolerances.  Operands are exact in the products; sums are float32.  With u = 2^-
       roundings of exp, sum and log (16 u of 1 + |loss| + |z|).
   gradients: dz is off by the logits' error times itself and one rounding to bf16 (2^-8 of itself; none to speak of for float32, whose
       three parts keep 24 bits), the sums by their length times u, the result by its own rounding.  All of them are bounded
-      entry by entry from the absolute values of what is summed."""
+      entry by entry from the absolute values of what is summed, and doubled: with an upstream gradient a row, x is rounded with it to its two parts' 16 bits."""
 import pytest
 import torch
 
