@@ -868,6 +868,10 @@ __global__ void __launch_bounds__(256) join_split_kernel(const Args a, int pairs
     __shared__ unsigned found[kMostPairs / 32];
     grid_launch_dependents();
     grid_dependency_wait();
+    if (*a.status != 0) {   // (nothing is joined over the NaN)
+        if (a.last) blank(a);
+        return;
+    }
     const int count = *a.count, lane = threadIdx.x & 31;
     const SplitTiles t = split_tiles(a, count, pairs);
     // (every block has them in the same order)

@@ -274,10 +274,13 @@ def test_two_calls_at_once(ops):
     assert all(torch.equal(a, b) for i in range(2) for r in got[i] for a, b in zip(r, want[i]))
 
 
-def test_waits_run_out_and_the_next_call_is_right(ops):
-    """The products' loads are withheld: every wait ends, the loss says so, and nothing stays behind."""
-    T, V, d = 300, 700, 96
-    x, w, y = _inputs(T, V, d, torch.bfloat16, seed=14)
+@pytest.mark.parametrize("T,d,dtype", [(300, 96, torch.bfloat16), (20, 96, torch.bfloat16), (20, 1000, torch.bfloat16), (300, 1000, torch.bfloat16),
+                                       (300, 96, torch.float32), (20, 96, torch.float32)])
+def test_waits_run_out_and_the_next_call_is_right(ops, T, d, dtype):
+    """The products' loads are withheld, in pairs of blocks and blocks by themselves, with sums in one piece and folded: every wait ends, the loss
+    says so, and nothing stays behind."""
+    V = 700
+    x, w, y = _inputs(T, V, d, dtype, seed=14)
     one = torch.ones((), device="cuda")
     want = _grads(ops, x, w, y, one)
     old = ops.set_wait_limit_ns(2_000_000)
@@ -345,3 +348,22 @@ def test_sizes_at_random(ops, dtype, seed):
         assert abs(got[0].double() - want[0].sum() / n) <= (off[0].sum() + U * want[0].sum()) / n
     _check(got[1], want[1], off[1] + 4 * U * want[1].abs(), f"grad of hidden {T} {V} {d}")
     _check(got[2], want[2], off[2] + 4 * U * want[2].abs(), f"grad of weight {T} {V} {d}")
+
+
+def test_one_row_without_a_batch_and_a_graph_kept(ops):
+    """hidden (d,) with a target (); backward twice from one forward; memory filled beforehand as deterministic runs have it."""
+    x, w, y = _inputs(1, 90, 33, torch.float32, seed=30, ignored=0.0)
+    want = _grads(ops, x, w, y, torch.ones(1, device="cuda"), reduction="none")
+    xs, ws = x[0].clone().requires_grad_(), w.clone().requires_grad_()
+    loss = ops.linear_cross_entropy(xs, ws, y[0], reduction="none")
+    assert loss.shape == () and torch.equal(loss.detach(), want[0][0])
+    for _ in range(2):
+        gx, gw = torch.autograd.grad(loss, [xs, ws], retain_graph=True)
+        assert gx.shape == xs.shape and torch.equal(gx, want[1][0]) and torch.equal(gw, want[2])
+    torch.use_deterministic_algorithms(True)
+    try:
+        x, w, y = _inputs(700, 900, 200, torch.bfloat16, seed=31)
+        a = _grads(ops, x, w, y, torch.ones((), device="cuda"))
+    finally:
+        torch.use_deterministic_algorithms(False)
+    assert all(torch.equal(p, q) for p, q in zip(a, _grads(ops, x, w, y, torch.ones((), device="cuda"))))
