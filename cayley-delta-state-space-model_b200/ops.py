@@ -176,8 +176,11 @@ def embedding(ids: Tensor, weight: Tensor, *, scale: float = 1.0, padding_idx: i
     """scale * weight[ids] (cdssm/models/model.py:46): ids (...) int64, weight (vocab, d) bfloat16 or float32 -> (..., d).
 
     The gradient (vocab, d) is dense, in the weight's type; the rows of one id are added up in float32 in the order of the tokens and
-    rounded once, the same bits from run to run; ``padding_idx``'s row gets none.  An id that is no row of the table (negative ones too)
-    gives a row of NaN and takes no part in the gradient.  Differentiable once."""
+    rounded once, the same bits from run to run; ``padding_idx``'s row gets none (it does not count from the end: a negative one is
+    refused).  An id that is no row of the table (negative ones too) gives a row of NaN and takes no part in the gradient.
+    Differentiable once."""
+    if padding_idx is not None and padding_idx < 0:   # (the native call's -1 is none)
+        raise CdssmError(f"padding_idx must be a row of the table or None, not {padding_idx}")
     return _lib.host().embedding(ids, weight, scale, -1 if padding_idx is None else padding_idx)
 
 

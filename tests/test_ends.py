@@ -53,3 +53,11 @@ def test_arguments_of_the_abi(lib):
     assert h.cdssm_b200_grad_clip(ptrs, null, sizes, types, null, 3, 1.0, null, one, 1 << 20, null) == -1
     assert h.cdssm_b200_grad_clip(ptrs, null, sizes, (ctypes.c_int * 3)(0, 0, 7), null, 3, 1.0, one, one, 1 << 20, null) == -1
     assert h.cdssm_b200_grad_clip(ptrs, ptrs, sizes, (ctypes.c_int * 3)(1, 1, 1), types, 3, 1.0, one, one, 1 << 20, null) == -1   # float32 into bf16
+
+
+@pytest.mark.parametrize("padding_idx", [-1, -2, -5])
+def test_padding_row_does_not_count_from_the_end(lib, padding_idx):
+    """Not taken for "none" either: the row that was meant would be trained."""
+    from cdssm_b200 import ops
+    with pytest.raises(lib.CdssmError, match="padding_idx"):
+        ops.embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(5, 8), padding_idx=padding_idx)
