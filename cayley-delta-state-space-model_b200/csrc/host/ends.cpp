@@ -80,7 +80,7 @@ CeGrads ce_backward(const Tensor& grad, const Tensor& weight, const Tensor& targ
     const size_t wb = cdssm_b200_linear_ce_workspace_bytes(rows, (int)d, (int)vocab, dt, 1);
     const Tensor g = (grad.scalar_type() == at::kFloat ? grad : grad.to(at::kFloat)).contiguous(), w = table(weight), y = targets.contiguous(),
                  ws = scratch(wb, weight);
-    check(cdssm_b200_linear_ce_bwd(fptr(g), cptr(w), row_stride(w), y.const_data_ptr<int64_t>(), mptr(saved), (size_t)saved.numel(), mptr(r.x), mptr(r.w),
+    check(cdssm_b200_linear_ce_bwd(fptr(g), cptr(w), row_stride(w), y.const_data_ptr<int64_t>(), cptr(saved), (size_t)saved.numel(), mptr(r.x), mptr(r.w),
                                    mptr(ws), wb, rows, (int)d, (int)vocab, ignore, (int)reduction, dt, (int)flags, stream_of(w)),
           "linear_cross_entropy backward");
     return r;

@@ -56,7 +56,7 @@ constexpr int kTerms3 = 6;
 
 struct Args {
     // what the forward leaves for the backward; Tp: rows padded to kM
-    const int* count;            // rows that have a target
+    const int* count;            // rows that have a target; behind it, the forward's status
     const int* rows;             // (Tp) compact row -> row of the caller, -1 behind the last
     const int* target;           // (Tp) its word, -2: outside of the vocabulary
     float *row_max, *row_inv;    // (Tp) m and 1 / s
@@ -81,7 +81,10 @@ struct Args {
     const int64_t* caller_target;   // of all rows
     int64_t n_rows, ignore;
     float4* slots;               // partial tiles of the split ones: two a block
+    // where a block notes a wait that ran out.  Forward: one word, 0 before.  Backward: a word a block, which the first kernel sets, by the
+    // forward's word as well, so that nothing of one backward pass is left for the next pass over the same saved rows
     int* status;
+    int status_words;            // backward: of the first kernel's blocks, the most of any
     unsigned long long wait_ns;
     int withhold;
 };
@@ -773,7 +776,11 @@ __device__ __forceinline__ void product_block(const Maps& maps, const Args& a) {
         if (kMode == kGradProducts) { prefetch_tmap(&maps.a2); prefetch_tmap(&maps.b2); }
     }
     if ((smem_u32(smem_raw) & 1023u) != 0) {   // the swizzled tiles need 1024-byte alignment
-        if (threadIdx.x == 0) atomicCAS(a.status, 0, 499);
+        grid_dependency_wait();
+        if (threadIdx.x == 0) {
+            if (kMode == kStats) atomicCAS(a.status, 0, 499);
+            else a.status[blockIdx.x] = 499;
+        }
         return;
     }
     if (threadIdx.x == 0) {
@@ -794,7 +801,7 @@ __device__ __forceinline__ void product_block(const Maps& maps, const Args& a) {
     if (kMode == kStats && a.ahead && warp == 2) request_first_tile<kSolo>(a);
     grid_launch_dependents();
     grid_dependency_wait();
-    const int count = *a.count;
+    const int count = a.count[0], before = kMode == kGradLogits && a.first ? a.count[1] : 0;
     bool ok = true;
     // (a warpgroup's registers: 128 x 40 + 256 x 232 are the 384 x 168 of the launch)
     if (warp < 4) {
@@ -809,10 +816,14 @@ __device__ __forceinline__ void product_block(const Maps& maps, const Args& a) {
         if constexpr (kFold) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         ok = finish<kMode, kFold, kSolo>(sm, a, count);
     }
-    if (!ok) atomicCAS(a.status, 0, 400 + warp);
+    if (kMode == kStats && !ok) atomicCAS(a.status, 0, 400 + warp);
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (kMode != kStats && threadIdx.x == 0) {   // (whoever gives up sets the flag)
+        if (sm.abort_flag) a.status[blockIdx.x] = 400;
+        else if (kMode == kGradLogits && a.first) a.status[blockIdx.x] = before;
+    }
     if (sm.abort_flag) {   // copies and products that are under way end within microseconds: none outlives the pair's memory
         const uint64_t t0 = global_ns();
         while (global_ns() - t0 < 2'000'000ull) __nanosleep(1000);
@@ -837,9 +848,9 @@ solo_kernel(const __grid_constant__ Maps maps, const Args a) {
 }
 
 // dx of the rows without a target is zero.  After a wait that ran out both gradients are NaN.
-__device__ __forceinline__ void blank(const Args& a) {
+__device__ __forceinline__ void blank(const Args& a, bool failed) {
     const int64_t step = (int64_t)gridDim.x * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (*a.status != 0) {
+    if (failed) {
         auto fill = [&](void* to, int64_t n) {   // NaN, as it is in either type
             unsigned short* const p = static_cast<unsigned short*>(to);
             if (p) for (int64_t i = at; i < n * (a.f32 ? 2 : 1); i += step) p[i] = 0x7fff;
@@ -868,8 +879,10 @@ __global__ void __launch_bounds__(256) join_split_kernel(const Args a, int pairs
     __shared__ unsigned found[kMostPairs / 32];
     grid_launch_dependents();
     grid_dependency_wait();
-    if (*a.status != 0) {   // (nothing is joined over the NaN)
-        if (a.last) blank(a);
+    bool gave_up = false;
+    for (int i = threadIdx.x; i < a.status_words; i += 256) gave_up |= __ldcg(a.status + i) != 0;
+    if (__syncthreads_or(gave_up)) {   // (nothing is joined over the NaN)
+        if (a.last) blank(a, true);
         return;
     }
     const int count = *a.count, lane = threadIdx.x & 31;
@@ -926,7 +939,7 @@ __global__ void __launch_bounds__(256) join_split_kernel(const Args a, int pairs
         }
         emit(a, count, factor, dw, row0 + lane, t.tile_n(row, member) * kN + (warp >> 2 & 1) * 128 + chunk * 32 + j4 * 4, v);
     }
-    if (a.last) blank(a);
+    if (a.last) blank(a, false);
 }
 
 // ---- rows in, losses out -------------------------------------------------------------------------
@@ -1195,7 +1208,7 @@ struct Sizes {
     // saved, without and with W's parts (a W that is not read in place: the backward needs them as well, which mostly follows at once)
     size_t o_rows, o_words, o_max, o_inv, o_hit, o_x, o_w, saved, saved_w;
     // scratch of the forward and of the backward
-    size_t o_part, o_sums, fwd, o_dz, o_acc, o_slots, o_scaled, bwd;
+    size_t o_part, o_sums, fwd, o_status, o_dz, o_acc, o_slots, o_scaled, bwd;
 };
 // Up to this many rows the second block of a pair would have none of its own: z is made by blocks by themselves (Smem), and bf16's dz keeps 16 bits, in
 // two parts.  (Where a row has one large entry, its target's, that entry's rounding to 8 bits is all of the row's error; beyond, the rows' roundings
@@ -1229,6 +1242,7 @@ bool sizes_of(int64_t rows, int d, int vocab, int dtype, int sms, Sizes& s) {
     s.o_part = take(8ull * 2 * s.n_tiles * s.Tp); s.o_sums = take(8ull * (s.Tp / kJoinRows));
     s.fwd = o;
     o = 0;
+    s.o_status = take(4ull * sms);
     s.o_dz = take(column * s.vn); s.o_acc = take(s.pieces > 1 ? 4ull * s.Tp * s.d_tiles * kN : 0);
     s.o_slots = take(2ull * (sms / 2) * kM * kN * 4);
     s.o_scaled = take(s.dz_planes == 1 ? 2ull * 2 * s.Tp * s.pitch : 0);
@@ -1390,7 +1404,7 @@ extern "C" int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, con
                              a.row_max, a.row_inv, a.hit, loss, reduction, reinterpret_cast<double*>(ws + s.o_sums));
 }
 
-extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, int64_t w_row_stride, const int64_t* target, void* saved,
+extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, int64_t w_row_stride, const int64_t* target, const void* saved,
                                         size_t saved_bytes, void* grad_x, void* grad_w, void* workspace, size_t workspace_bytes, int64_t rows,
                                         int d, int vocab, int64_t ignore_index, int reduction, int dtype, int flags, void* stream) {
     if (!grad_loss || !w || !target || !saved || !workspace || (!grad_x && !grad_w) || reduction < CDSSM_CE_NONE || reduction > CDSSM_CE_SUM)
@@ -1403,11 +1417,13 @@ extern "C" int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, i
     const cudaStream_t st = (cudaStream_t)stream;
     int sms = 0;
     if (int rc = sm_count(sms)) return rc;
-    char *const sv = static_cast<char*>(saved), *const ws = static_cast<char*>(workspace);
+    char *const sv = static_cast<char*>(const_cast<void*>(saved)), *const ws = static_cast<char*>(workspace);   // (saved is read alone)
     const void* const wb = direct ? w : sv + s.o_w;
     const int64_t w_cols = direct ? d : s.pitch, w_pitch = direct ? w_row_stride : s.pitch;
     ce::Args a;
     ce::fill_saved(a, s, sv);
+    a.status = reinterpret_cast<int*>(ws + s.o_status);
+    a.status_words = a.few ? sms : sms / 2 * 2;
     a.row_factor = reduction == CDSSM_CE_NONE && s.dz_planes == 1;
     if (int rc = ce::bind_context()) return rc;
     ce::Maps logits{}, grads{};

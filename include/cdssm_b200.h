@@ -453,8 +453,8 @@ CDSSM_API int cdssm_b200_decode_step_reference(float* local_state, float* correc
  * (cdssm_b200_linear_ce_workspace_bytes), which is free again behind the call.  It holds the rows that take part and, for a w that is not
  * read in place (float32, or rows that are not 16-byte aligned), w's bf16 parts: 6 or 2 bytes a value.  Both sizes are for the current device, 0 on
  * bad sizes.  rows <= 2^24, vocab <= 2^24, d <= 65536.  bf16 products with float32 sums; float32 operands enter as three bf16 parts.
- * flags: 0 or CDSSM_SCAN_TEST_WITHHOLD.  After a bounded wait that ran out the loss and its
- * gradients are NaN.
+ * flags: 0 or CDSSM_SCAN_TEST_WITHHOLD.  After a bounded wait that ran out the loss and its gradients are NaN; of one in a backward pass
+ * that pass's gradients alone.
  * Replaces the LM head and the loss of a training step: cdssm/models/model.py:50-51, cdssm/training/trainer.py:219-262. */
 #define CDSSM_CE_NONE 0
 #define CDSSM_CE_MEAN 1
@@ -467,10 +467,11 @@ CDSSM_API int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, cons
                                        int reduction, int dtype, int flags, void* stream);
 
 /* Its backward: grad_loss (rows for CDSSM_CE_NONE, else one value) float32 -> grad_x (rows,d) and grad_w (vocab,d), dense, in the
- * storage type, 16-byte aligned; either may be NULL.  w, target and the other arguments as in the forward that left saved.
+ * storage type, 16-byte aligned; either may be NULL.  w, target and the other arguments as in the forward that left saved, which is
+ * read alone: any number of passes may follow one forward, at the same time too, each with a workspace of its own.
  * dz is formed a piece of the vocabulary at a time (at most 512 MiB of scratch while a row tile allows).  Sums run in a fixed order. */
 CDSSM_API int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, int64_t w_row_stride, const int64_t* target,
-                                       void* saved, size_t saved_bytes, void* grad_x, void* grad_w, void* workspace,
+                                       const void* saved, size_t saved_bytes, void* grad_x, void* grad_w, void* workspace,
                                        size_t workspace_bytes, int64_t rows, int d, int vocab, int64_t ignore_index,
                                        int reduction, int dtype, int flags, void* stream);
 

@@ -1,0 +1,56 @@
+"""Calls of ops.linear_cross_entropy and of its C entry points that go beyond one forward and one backward pass."""
+import pytest
+import torch
+
+from test_loss_gpu import _grads, _inputs
+
+pytestmark = pytest.mark.gpu
+
+
+class Entry:
+    """The C entry points on tensors: one forward, then any number of backward passes over what it saved."""
+
+    def __init__(self, ops, x, w, y):
+        self.h, self.ops, self.x, self.w, self.y = ops._lib.lib(), ops, x, w, y
+        self.dt = ops._lib.BF16 if x.dtype == torch.bfloat16 else ops._lib.F32
+        (self.T, self.d), self.V = x.shape, w.shape[0]
+        self.saved = self._bytes(self.h.cdssm_b200_linear_ce_saved_bytes(self.T, self.d, self.V, w.data_ptr(), w.stride(0), self.dt))
+        self.loss = torch.empty((), device="cuda")
+        ws = self._bytes(self.h.cdssm_b200_linear_ce_workspace_bytes(self.T, self.d, self.V, self.dt, 0))
+        assert self.h.cdssm_b200_linear_ce_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), y.data_ptr(), self.loss.data_ptr(),
+                                               self.saved.data_ptr(), self.saved.numel(), ws.data_ptr(), ws.numel(), self.T, self.d, self.V, -100,
+                                               1, self.dt, 0, torch.cuda.current_stream().cuda_stream) == 0
+
+    @staticmethod
+    def _bytes(n):                                                   # (what lay in the memory before is no part of a call)
+        return torch.full((n,), 255, dtype=torch.uint8, device="cuda")
+
+    def backward(self, flags=0):
+        ws = self._bytes(self.h.cdssm_b200_linear_ce_workspace_bytes(self.T, self.d, self.V, self.dt, 1))
+        gx, gw, one = torch.empty_like(self.x), torch.empty_like(self.w), torch.ones((), device="cuda")
+        assert self.h.cdssm_b200_linear_ce_bwd(one.data_ptr(), self.w.data_ptr(), self.w.stride(0), self.y.data_ptr(), self.saved.data_ptr(),
+                                               self.saved.numel(), gx.data_ptr(), gw.data_ptr(), ws.data_ptr(), ws.numel(), self.T, self.d, self.V,
+                                               -100, 1, self.dt, flags, torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()                                     # (the workspace is let go)
+        return gx, gw
+
+
+@pytest.mark.parametrize("T,V,d,dtype", [(300, 700, 96, torch.bfloat16), (20, 700, 96, torch.bfloat16), (20, 700, 1000, torch.bfloat16),
+                                         (300, 700, 96, torch.float32), (20, 700, 96, torch.float32), (65600, 8191, 8, torch.bfloat16)])
+def test_a_backward_that_gave_up_leaves_nothing_to_the_next(ops, T, V, d, dtype):
+    """One forward, a backward pass whose loads are withheld, then a whole one: its gradients are those of a forward of its own, and what the
+    forward saved is as it was.  (The last size forms the logits' gradient in three pieces.)"""
+    x, w, y = _inputs(T, V, d, dtype, seed=40)
+    want = _grads(ops, x, w, y, torch.ones((), device="cuda"))
+    e = Entry(ops, x, w, y)
+    kept = e.saved.clone()
+    assert torch.equal(e.loss, want[0])
+    assert all(torch.equal(a, b) for a, b in zip(e.backward(), want[1:]))
+    old = ops.set_wait_limit_ns(2_000_000)
+    try:
+        assert all(g.isnan().all() for g in e.backward(ops.TEST_WITHHOLD))
+    finally:
+        ops.set_wait_limit_ns(old)
+    assert torch.equal(e.saved, kept)
+    for _ in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(e.backward(), want[1:]))
