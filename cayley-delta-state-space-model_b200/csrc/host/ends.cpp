@@ -2,6 +2,7 @@
 // with their gradients, and the norm and clipping of all gradients.
 #include "host.h"
 
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/custom_function.h>
 
 #include <algorithm>
@@ -37,6 +38,11 @@ void need_table(const Tensor& w, const char* name) {
     dtype_code(w);
 }
 bool wants_grad(const Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+// A tangent (torch.autograd.forward_ad) has no formula here: kernels that read the values alone would drop it without a word.
+void need_no_tangent(const char* what, const Tensor& t) {
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined())
+        throw Error(std::string(what) + " has no forward-mode gradient");
+}
 // The gradients come from kernels that autograd does not see into: a graph of them would leave out what they depend on.
 void once_only(const char* what) {
     if (c10::GradMode::is_enabled()) throw Error(std::string(what) + " is differentiable once: no create_graph=True");
@@ -109,6 +115,7 @@ PyObject* py_linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Args in{a, n};
         const Tensor hidden = in.tensor("hidden"), weight = in.tensor("weight"), targets = in.tensor("targets");
         const int64_t ignore = in.integer(), reduction = in.integer(), flags = in.integer();
+        for (const Tensor& t : {hidden, weight}) need_no_tangent("linear_cross_entropy", t);
         need_cuda(hidden, "hidden");
         need_table(weight, "weight");
         need_cuda(targets, "targets");
@@ -179,6 +186,7 @@ PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Tensor ids = in.tensor("ids"), weight = in.tensor("weight");
         const double scale = in.number();
         const int64_t padding = in.integer();
+        need_no_tangent("embedding", weight);
         need_cuda(ids, "ids");
         need_table(weight, "weight");
         need_same_device(ids, weight, "ids");
@@ -248,6 +256,9 @@ PyObject* py_grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
         std::vector<int64_t> sizes;
         std::vector<int> di, dout;
         pi.reserve(ins.size()); po.reserve(ins.size()); sizes.reserve(ins.size()); di.reserve(ins.size()); dout.reserve(ins.size());
+        const char* const what = scale ? "clip_grads_" : "grad_norm";
+        for (const Tensor& t : ins) need_no_tangent(what, t);
+        for (const Tensor& t : outs) need_no_tangent(what, t);
         for (size_t i = 0; i < ins.size(); i++) {
             need_dense(ins[i], "gradients");
             need_same_device(ins[i], ins[0], "gradients");

@@ -178,7 +178,7 @@ def embedding(ids: Tensor, weight: Tensor, *, scale: float = 1.0, padding_idx: i
     The gradient (vocab, d) is dense, in the weight's type; the rows of one id are added up in float32 in the order of the tokens and
     rounded once, the same bits from run to run; ``padding_idx``'s row gets none (it does not count from the end: a negative one is
     refused).  An id that is no row of the table (negative ones too) gives a row of NaN and takes no part in the gradient.
-    Differentiable once."""
+    Differentiable once, backwards."""
     if padding_idx is not None and padding_idx < 0:   # (the native call's -1 is none)
         raise CdssmError(f"padding_idx must be a row of the table or None, not {padding_idx}")
     return _lib.host().embedding(ids, weight, scale, -1 if padding_idx is None else padding_idx)
@@ -198,7 +198,7 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
     they hold (infinities and NaN too).  A target that is neither a word nor ignore_index makes its row's loss NaN.
     reduction "mean" (NaN when every row is ignored), "sum" or "none" (targets' shape); the loss is float32.
     Products are bfloat16 ones with float32 sums, for float32 operands exact to 24 bits; the logits' gradient is rounded once to the
-    products' type.  Gradients have the operands' type and are the same from run to run.  Differentiable once."""
+    products' type.  Gradients have the operands' type and are the same from run to run.  Differentiable once, backwards."""
     if reduction not in _REDUCTIONS:
         raise CdssmError(f"reduction must be 'none', 'mean' or 'sum', not {reduction!r}")
     return _lib.host().linear_cross_entropy(hidden, weight, targets, ignore_index, _REDUCTIONS[reduction], flags)
@@ -206,7 +206,7 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
 
 def grad_norm(grads) -> Tensor:
     """The 2-norm of all tensors together, one float32 value on their device; squares are summed in 64 bits in a fixed order.
-    bfloat16 and float32 CUDA tensors, dense in memory, at least one."""
+    bfloat16 and float32 CUDA tensors, dense in memory, at least one.  A number to look at: it has no gradient of its own."""
     return _lib.host().grad_clip(list(grads), None, 0.0)
 
 

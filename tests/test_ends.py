@@ -61,3 +61,26 @@ def test_padding_row_does_not_count_from_the_end(lib, padding_idx):
     from cdssm_b200 import ops
     with pytest.raises(lib.CdssmError, match="padding_idx"):
         ops.embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(5, 8), padding_idx=padding_idx)
+
+
+def _calls():
+    from cdssm_b200 import ops
+    ids = torch.zeros(3, dtype=torch.int64)
+    return {"hidden": lambda t: ops.linear_cross_entropy(t, torch.zeros(5, 8), ids), "weight": lambda t: ops.linear_cross_entropy(torch.zeros(3, 8), t, ids),
+            "embedding": lambda t: ops.embedding(ids, t), "norm": lambda t: ops.grad_norm([torch.zeros(2), t]),
+            "clip": lambda t: ops.clip_grads_([t], 1.0), "out": lambda t: ops.clip_grads_([torch.zeros(3, 8)], 1.0, out=[t])}
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("call", ["hidden", "weight", "embedding", "norm", "clip", "out"])
+def test_tangents_are_refused(lib, call, requires_grad):
+    """Not lost: the kernels know values alone."""
+    import torch.autograd.forward_ad as forward_ad
+    t = torch.zeros(3, 8, requires_grad=requires_grad)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(t, torch.ones(3, 8))
+        for mode in (torch.no_grad, torch.enable_grad):
+            with mode(), pytest.raises(lib.CdssmError, match="no forward-mode gradient"):
+                _calls()[call](dual)
+        with pytest.raises(lib.CdssmError, match="CUDA tensor"):     # (a plain one is read)
+            _calls()[call](t.detach())
