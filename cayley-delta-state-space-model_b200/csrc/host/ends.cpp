@@ -2,7 +2,9 @@
 // with their gradients, and the norm and clipping of all gradients.
 #include "host.h"
 
+#include <ATen/TracerMode.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
 
 #include <algorithm>
@@ -42,6 +44,11 @@ bool wants_grad(const Tensor& t) { return c10::GradMode::is_enabled() && t.requi
 void need_no_tangent(const char* what, const Tensor& t) {
     if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined())
         throw Error(std::string(what) + " has no forward-mode gradient");
+}
+// A tracer (torch.jit.trace, make_fx) records what the dispatcher sees: the outputs' allocation, and a graph that returns memory nobody has written.
+void need_no_trace(const char* what) {
+    using c10::impl::TorchDispatchModeTLS;
+    if (at::tracer::impl::is_dispatch_enabled() || TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY)) throw Error(std::string(what) + " cannot be traced");
 }
 // The gradients come from kernels that autograd does not see into: a graph of them would leave out what they depend on.
 void once_only(const char* what) {
@@ -115,6 +122,7 @@ PyObject* py_linear_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Args in{a, n};
         const Tensor hidden = in.tensor("hidden"), weight = in.tensor("weight"), targets = in.tensor("targets");
         const int64_t ignore = in.integer(), reduction = in.integer(), flags = in.integer();
+        need_no_trace("linear_cross_entropy");
         for (const Tensor& t : {hidden, weight}) need_no_tangent("linear_cross_entropy", t);
         need_cuda(hidden, "hidden");
         need_table(weight, "weight");
@@ -186,6 +194,7 @@ PyObject* py_embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Tensor ids = in.tensor("ids"), weight = in.tensor("weight");
         const double scale = in.number();
         const int64_t padding = in.integer();
+        need_no_trace("embedding");
         need_no_tangent("embedding", weight);
         need_cuda(ids, "ids");
         need_table(weight, "weight");
@@ -257,6 +266,7 @@ PyObject* py_grad_clip(PyObject*, PyObject* const* a, Py_ssize_t n) {
         std::vector<int> di, dout;
         pi.reserve(ins.size()); po.reserve(ins.size()); sizes.reserve(ins.size()); di.reserve(ins.size()); dout.reserve(ins.size());
         const char* const what = scale ? "clip_grads_" : "grad_norm";
+        need_no_trace(what);
         for (const Tensor& t : ins) need_no_tangent(what, t);
         for (const Tensor& t : outs) need_no_tangent(what, t);
         for (size_t i = 0; i < ins.size(); i++) {

@@ -84,3 +84,13 @@ def test_tangents_are_refused(lib, call, requires_grad):
                 _calls()[call](dual)
         with pytest.raises(lib.CdssmError, match="CUDA tensor"):     # (a plain one is read)
             _calls()[call](t.detach())
+
+
+@pytest.mark.parametrize("call", ["hidden", "weight", "embedding", "norm", "clip", "out"])
+def test_tracing_is_refused(lib, call):
+    """A traced graph would return memory that nobody has written."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    with pytest.raises(lib.CdssmError, match="cannot be traced"):
+        torch.jit.trace(_calls()[call], (torch.zeros(3, 8),), check_trace=False)
+    with pytest.raises(lib.CdssmError, match="cannot be traced"):
+        make_fx(_calls()[call])(torch.zeros(3, 8))
