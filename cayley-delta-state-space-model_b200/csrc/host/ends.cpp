@@ -91,8 +91,13 @@ CeGrads ce_backward(const Tensor& grad, const Tensor& weight, const Tensor& targ
     if (want_w) r.w = rows ? empty_like_dims({vocab, d}, weight) : at::zeros({vocab, d}, weight.options());
     if (rows == 0 || (!want_x && !want_w)) return r;
     const size_t wb = cdssm_b200_linear_ce_workspace_bytes(rows, (int)d, (int)vocab, dt, 1);
-    const Tensor g = (grad.scalar_type() == at::kFloat ? grad : grad.to(at::kFloat)).contiguous(), w = table(weight), y = targets.contiguous(),
-                 ws = scratch(wb, weight);
+    Tensor w = table(weight);
+    // (a weight that the forward read in place, moved since to where it cannot be, as a hook of saved tensors may: rows apart again)
+    if ((size_t)saved.numel() < cdssm_b200_linear_ce_saved_bytes(rows, (int)d, (int)vocab, cptr(w), row_stride(w), dt)) {
+        w = empty_like_dims({vocab, (d + 7) / 8 * 8}, weight).narrow(1, 0, d);
+        w.copy_(weight);
+    }
+    const Tensor g = (grad.scalar_type() == at::kFloat ? grad : grad.to(at::kFloat)).contiguous(), y = targets.contiguous(), ws = scratch(wb, weight);
     check(cdssm_b200_linear_ce_bwd(fptr(g), cptr(w), row_stride(w), y.const_data_ptr<int64_t>(), cptr(saved), (size_t)saved.numel(), mptr(r.x), mptr(r.w),
                                    mptr(ws), wb, rows, (int)d, (int)vocab, ignore, (int)reduction, dt, (int)flags, stream_of(w)),
           "linear_cross_entropy backward");

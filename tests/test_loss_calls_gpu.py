@@ -54,3 +54,39 @@ def test_a_backward_that_gave_up_leaves_nothing_to_the_next(ops, T, V, d, dtype)
     assert torch.equal(e.saved, kept)
     for _ in range(2):
         assert all(torch.equal(a, b) for a, b in zip(e.backward(), want[1:]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [20, 300])
+def test_saved_tensors_that_move(ops, T, dtype):
+    """Hooks that keep what was saved elsewhere: the weight comes back dense, though its rows lay apart or at an odd address when the forward read it,
+    and what was dense comes back with rows apart."""
+    V, d = 200, 100
+    x, w, y = _inputs(T, V, d, dtype, seed=41)
+    apart = lambda t, pitch: torch.zeros(V, pitch, device="cuda", dtype=dtype)[:, :d].copy_(t)  # noqa: E731
+    odd = torch.zeros(V * d + 1, device="cuda", dtype=dtype)[1:].view(V, d).copy_(w)
+    g = torch.randn(T, device="cuda")
+    want = _grads(ops, x, w, y, g, reduction="none")
+
+    def through(hooks, wt):
+        a, b = x.detach().requires_grad_(), wt.detach().requires_grad_()
+        with hooks:
+            loss = ops.linear_cross_entropy(a, b, y, reduction="none")
+        return (loss.detach(), *torch.autograd.grad(loss, [a, b], [g]))
+
+    for wt in (w, apart(w, 104), apart(w, 101), odd):
+        assert all(torch.equal(p, q) for p, q in zip(through(torch.autograd.graph.save_on_cpu(), wt), want))
+        for move in (lambda t: apart(t, 104), lambda t: apart(t, 103)):
+            hooks = torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t, move=move: move(t) if t.dim() == 2 else t)
+            assert all(torch.equal(p, q) for p, q in zip(through(hooks, wt), want))
+
+
+def test_transforms_are_refused(ops):
+    """vmap, func.grad and func.jvp hand over tensors without memory of their own: an error, not a value."""
+    x, w, y = _inputs(6, 10, 16, torch.bfloat16, seed=42)
+    loss = lambda t: ops.linear_cross_entropy(t, w, y)  # noqa: E731
+    for call in (lambda: torch.vmap(loss)(torch.stack([x, x])), lambda: torch.func.grad(loss)(x), lambda: torch.func.jvp(loss, (x,), (x,)),
+                 lambda: torch.vmap(lambda t: ops.embedding(y.clamp(min=0), t))(torch.stack([w, w])),
+                 lambda: torch.vmap(lambda t: ops.grad_norm([t]))(torch.stack([w, w]))):
+        with pytest.raises(RuntimeError):
+            call()
