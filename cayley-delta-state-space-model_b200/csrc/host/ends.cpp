@@ -55,6 +55,12 @@ void once_only(const char* what) {
     if (c10::GradMode::is_enabled()) throw Error(std::string(what) + " is differentiable once: no create_graph=True");
 }
 
+// What a forward pass saved passes through the program's hooks on its way to the backward, and kernels go by what it was then.
+void need_as_saved(const char* what, const Tensor& t, at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) {
+    if (t.device() != device || t.scalar_type() != type || t.sizes() != sizes)
+        throw Error(std::string(what) + ": a saved tensor came back on another device, in another shape or of another type");
+}
+
 // ---- loss ------------------------------------------------------------------------------------------
 struct CeOut {
     Tensor loss, saved;
@@ -108,7 +114,7 @@ struct CeNode : torch::autograd::Function<CeNode> {
                           int64_t reduction, int64_t flags) {
         CeOut o = ce_forward(hidden, weight, targets, ignore, reduction, flags);
         ctx->save_for_backward({weight, targets, o.saved});
-        ctx->saved_data["args"] = std::vector<int64_t>{ignore, reduction, flags};
+        ctx->saved_data["args"] = std::vector<int64_t>{ignore, reduction, flags, weight.size(0), (int64_t)weight.scalar_type(), o.saved.numel()};
         ctx->saved_data["sizes"] = hidden.sizes().vec();
         return o.loss;
     }
@@ -116,7 +122,12 @@ struct CeNode : torch::autograd::Function<CeNode> {
         once_only("linear_cross_entropy");
         const auto saved = ctx->get_saved_variables();
         const auto args = ctx->saved_data["args"].toIntVector(), sizes = ctx->saved_data["sizes"].toIntVector();
-        CeGrads g = ce_backward(grads[0], saved[0], saved[1], saved[2], args[0], args[1], ctx->needs_input_grad(0), ctx->needs_input_grad(1), sizes, args[2]);
+        const at::IntArrayRef all(sizes);
+        const at::Device device = grads[0].device();
+        need_as_saved("linear_cross_entropy", saved[0], {args[3], all.back()}, (at::ScalarType)args[4], device);
+        need_as_saved("linear_cross_entropy", saved[1], all.slice(0, all.size() - 1), at::kLong, device);
+        need_as_saved("linear_cross_entropy", saved[2], {args[5]}, at::kByte, device);
+        CeGrads g = ce_backward(grads[0], saved[0], saved[1], saved[2].contiguous(), args[0], args[1], ctx->needs_input_grad(0), ctx->needs_input_grad(1), sizes, args[2]);
         return {g.x, g.w, Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
@@ -187,7 +198,9 @@ struct EmbedNode : torch::autograd::Function<EmbedNode> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         once_only("embedding");
         const auto args = ctx->saved_data["args"].toIntVector();
-        return {embed_backward(grads[0], ctx->get_saved_variables()[0], args[0], args[1], args[2], ctx->saved_data["scale"].toDouble()), Tensor(),
+        const Tensor ids = ctx->get_saved_variables()[0], &g = grads[0];
+        need_as_saved("embedding", ids, g.sizes().slice(0, g.dim() - 1), at::kLong, g.device());
+        return {embed_backward(g, ids, args[0], args[1], args[2], ctx->saved_data["scale"].toDouble()), Tensor(),
                 Tensor(), Tensor()};
     }
 };

@@ -90,3 +90,19 @@ def test_transforms_are_refused(ops):
                  lambda: torch.vmap(lambda t: ops.grad_norm([t]))(torch.stack([w, w]))):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_saved_tensors_that_come_back_as_something_else(ops):
+    """On the host, of another type, of another shape: an error before anything is launched."""
+    x, w, y = _inputs(20, 30, 16, torch.float32, seed=43, ignored=0.0)
+    calls = [lambda: ops.linear_cross_entropy(x.detach().requires_grad_(), w.detach().requires_grad_(), y),
+             lambda: ops.embedding(y, w.detach().requires_grad_()).sum()]
+    kinds = {"weight": lambda t: t.dim() == 2, "ids": lambda t: t.dtype == torch.int64, "rows": lambda t: t.dtype == torch.uint8}
+    other = {torch.float32: torch.bfloat16, torch.int64: torch.int32, torch.uint8: torch.int32}
+    for change in (lambda t: t.cpu(), lambda t: t[:-1], lambda t: t.to(other[t.dtype])):
+        for kind, mine in kinds.items():
+            for call in calls[:2 if kind == "ids" else 1]:
+                with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: change(t) if mine(t) else t):
+                    loss = call()
+                with pytest.raises(RuntimeError, match="a saved tensor came back"):
+                    loss.backward()
