@@ -21,15 +21,19 @@ void need_same_device(const Tensor& t, const Tensor& as, const char* name) {
     if (t.device() != as.device()) throw Error(std::string(name) + " is on " + t.device().str() + ", not on " + as.device().str());
 }
 
+// Values as they lie in memory: of the imaginary part of a conjugate, say, the sign is pending.
+Tensor signed_values(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // (rows, d) of a matrix whose rows are dense, wherever they lie; else a copy.
 Tensor row_matrix(const Tensor& t, int64_t d) {
-    const Tensor m = t.reshape({-1, d});
+    const Tensor m = signed_values(t).reshape({-1, d});
     return d == 1 || m.stride(1) == 1 ? m : m.contiguous();
 }
 int64_t row_stride(const Tensor& m) { return m.size(0) > 1 ? m.stride(0) : m.size(1); }
 
 // (vocab, d), rows dense and apart: as it lies, or a copy
-Tensor table(const Tensor& w) {
+Tensor table(const Tensor& t) {
+    const Tensor w = signed_values(t);
     return (w.size(1) == 1 || w.stride(1) == 1) && (w.size(0) == 1 || w.stride(0) >= w.size(1)) ? w : w.contiguous();
 }
 void need_table(const Tensor& w, const char* name) {
@@ -103,7 +107,7 @@ CeGrads ce_backward(const Tensor& grad, const Tensor& weight, const Tensor& targ
         w = empty_like_dims({vocab, (d + 7) / 8 * 8}, weight).narrow(1, 0, d);
         w.copy_(weight);
     }
-    const Tensor g = (grad.scalar_type() == at::kFloat ? grad : grad.to(at::kFloat)).contiguous(), y = targets.contiguous(), ws = scratch(wb, weight);
+    const Tensor g = signed_values(grad.scalar_type() == at::kFloat ? grad : grad.to(at::kFloat)).contiguous(), y = targets.contiguous(), ws = scratch(wb, weight);
     check(cdssm_b200_linear_ce_bwd(fptr(g), cptr(w), row_stride(w), y.const_data_ptr<int64_t>(), cptr(saved), (size_t)saved.numel(), mptr(r.x), mptr(r.w),
                                    mptr(ws), wb, rows, (int)d, (int)vocab, ignore, (int)reduction, dt, (int)flags, stream_of(w)),
           "linear_cross_entropy backward");
@@ -180,7 +184,7 @@ Tensor embed_backward(const Tensor& grad_, const Tensor& ids_, int64_t vocab, in
     const int dt = dtype_code(grad_);
     const size_t bytes = cdssm_b200_embedding_bwd_workspace_bytes(count, (int)vocab, (int)d, dt);
     if (bytes == 0) check(CDSSM_ERR_UNSUPPORTED, "embedding backward");
-    Tensor grad = grad_.contiguous();
+    Tensor grad = signed_values(grad_).contiguous();
     if (reinterpret_cast<uintptr_t>(grad.const_data_ptr()) & 15) grad = grad.clone();
     const Tensor ids = ids_.contiguous(), ws = scratch(bytes, grad_);
     check(cdssm_b200_embedding_bwd(ids.const_data_ptr<int64_t>(), cptr(grad), mptr(out), mptr(ws), bytes, count, (int)vocab, (int)d, padding,
@@ -229,6 +233,7 @@ void need_dense(const Tensor& t, const char* name) {
     need_cuda(t, name);
     if (t.layout() != at::kStrided) throw Error(std::string(name) + ": a sparse tensor");
     dtype_code(t);
+    if (t.is_neg()) throw Error(std::string(name) + ": a tensor whose sign is pending (resolve_neg() it)");
     if (!t.is_non_overlapping_and_dense()) throw Error(std::string(name) + ": a tensor with holes or overlaps in memory");
 }
 

@@ -106,3 +106,27 @@ def test_saved_tensors_that_come_back_as_something_else(ops):
                     loss = call()
                 with pytest.raises(RuntimeError, match="a saved tensor came back"):
                     loss.backward()
+
+
+@pytest.mark.parametrize("T,V,d", [(40, 50, 24), (40, 50, 1), (1, 1, 1)])
+def test_signs_that_are_pending(ops, T, V, d):
+    """Views whose values are the negatives of what lies in memory, as operands and as upstream gradients."""
+    x, w, y = _inputs(T, V, d, torch.float32, seed=44, ignored=0.0)
+    neg = lambda t: torch._neg_view((-t).contiguous())  # noqa: E731
+    g, ge = torch.randn(T, device="cuda"), torch.randn(T, d, device="cuda")
+    assert neg(w).is_neg() and torch.equal(neg(w), w)
+    want = _grads(ops, x, w, y, g, reduction="none")
+    assert all(torch.equal(a, b) for a, b in zip(_grads(ops, neg(x), neg(w), y, neg(g), reduction="none"), want))
+    leaf = w.clone().requires_grad_()
+    rows = ops.embedding(y, leaf)
+    assert torch.equal(rows, ops.embedding(y, neg(w)))
+    assert torch.equal(torch.autograd.grad(rows, [leaf], [neg(ge)], retain_graph=True)[0], torch.autograd.grad(rows, [leaf], [ge])[0])
+    # as they come about: the loss is an imaginary part, and what is read is its conjugate's
+    leaf = w.clone().requires_grad_()
+    loss = ops.linear_cross_entropy(x, leaf, y)
+    got, = torch.autograd.grad(torch.complex(loss, loss).conj().imag, [leaf], retain_graph=True)
+    assert torch.equal(got, -torch.autograd.grad(loss, [leaf])[0])
+    assert torch.equal(ops.grad_norm([w]), ops.grad_norm([-w]))
+    for call in (lambda: ops.grad_norm([neg(w)]), lambda: ops.clip_grads_([w.clone()], 1.0, out=[neg(w)])):
+        with pytest.raises(ops.CdssmError, match="sign is pending"):
+            call()
