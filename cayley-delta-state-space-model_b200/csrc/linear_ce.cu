@@ -46,9 +46,12 @@ constexpr int kTmemCols = 2 * kN;
 enum Mode { kStats, kGradLogits, kGradProducts };
 
 // Depth blocks after which a sum is folded.  Losses of width 768 in one piece are off by 7e-7 of themselves (float32 sums in registers 3e-7), in
-// pieces of 4 blocks by 3e-7, but those take an eighth longer (8 x 2048 rows: 571 -> 645 us; 61 rows: 25.8 -> 28.8).  Sums of bf16 gradients run on: they
-// are rounded to 2^-8 in the end.
+// pieces of 4 blocks by 3e-7, but those take an eighth longer (8 x 2048 rows: 571 -> 645 us; 61 rows: 25.8 -> 28.8).  Sums of bf16 gradients, which are
+// rounded to 2^-8 in the end, run on up to so many rows (of dW) and words (of dx).  Unfolded, sums of one sign lose 2e-5 of 16 384 rows, 1.4e-4 of
+// 65 536 and 7e-4 of 262 144, folded nothing to speak of, in the same time where there are many rows (30 000 rows, 8191 words: 1745 us both;
+// 262 144 x 4096, 1024 words: 3.19 ms both); 500 rows of 50 257 words, cut in shares anyway, 188 and 193.
 constexpr int kFoldLogits = 12, kFold3 = 4;
+constexpr int kLongRows = 16384, kLongWords = 65536, kFoldLong = 16;
 
 // Part products in the order in which they are added up: the small ones first, so that they are not lost beside the large one's rounding.
 // float32 operands: (2,1), (1,2), (2,2) are below 2^-24 of the whole.  dz of a few rows of bf16 (kFewRows): its two parts.
@@ -370,7 +373,7 @@ struct Steps {
 };
 // groups that blocks [k0, k1) touch
 __device__ __forceinline__ int groups_of(const Args& a, const Segment& s) {
-    const int per = a.group * a.terms;
+    const int per = a.group * (s.dw ? a.terms : a.terms_dx);
     return (s.k1 - 1) / per - s.k0 / per + 1;
 }
 
@@ -1296,8 +1299,9 @@ template <int kMode>
 int launch_products(const Maps& maps, Args a, int workers, cudaStream_t st) {
     set_terms(a, kMode == kGradProducts);
     // (two parts of dz: block by block, so that the other operand's comes from L2 the second time)
-    a.group = a.planes == 3 ? kFold3 : kMode == kGradProducts ? 1 : kFoldLogits;
-    a.folds = a.planes == 3 || (kMode != kGradProducts && a.group * kK < a.d);
+    const bool long_sums = kMode == kGradProducts && (a.Tp > kLongRows || a.dz_pitch > kLongWords);
+    a.group = a.planes == 3 ? kFold3 : long_sums ? kFoldLong : kMode == kGradProducts ? 1 : kFoldLogits;
+    a.folds = a.planes == 3 || long_sums || (kMode != kGradProducts && a.group * kK < a.d);
     if constexpr (kMode != kGradProducts)
         if (a.few) return a.folds ? launch_as<kMode, true, true>(maps, a, workers, st) : launch_as<kMode, false, true>(maps, a, workers, st);
     return a.folds ? launch_as<kMode, true, false>(maps, a, 2 * workers, st) : launch_as<kMode, false, false>(maps, a, 2 * workers, st);
