@@ -373,6 +373,8 @@ bool decode_small_batch(const Plan& p, const Layout& lay, const Mix& mixes, cons
     return true;
 }
 
+// (The library's indexing: ids that count from the end mean what they meant, and an id that is no row stops the program.  ops.embedding makes
+// NaN of either.)
 Tensor embed(const Plan& p, const Tensor& ids) { return at::index(p.embedding, {std::optional<Tensor>(ids)}); }
 Tensor head(const Plan& p, const Tensor& x, const Tensor& ws) {
     return linear(rms_norm(x, p.final_norm_w, kFinalEps), p.embedding, Tensor(), ws);

@@ -209,7 +209,8 @@ class CdssmLM:
     def loss(self, input_ids, targets=None, *, ignore_index=-100, reduction="mean", scan_flags=0):
         """Cross entropy of the model's predictions, as cdssm/training/trainer.py:219-262 takes it from forward()'s logits, which are
         not formed here (:func:`ops.linear_cross_entropy`).  input_ids (B,L); targets (B,L), by default the next ids of each row
-        (the last position has none).  "mean" and "sum" give one float32 value, "none" one per position."""
+        (the last position has none).  "mean" and "sum" give one float32 value, "none" one per position.  Ids are read as forward() reads
+        them: one that is no row of the table is a device assertion; as a target it makes its position's loss NaN."""
         ids = self._ids(input_ids)
         if targets is None:
             targets = torch.full_like(ids, ignore_index, dtype=torch.int64)
