@@ -19,9 +19,11 @@
 // cores' float32 sums are cut off, not rounded, so that the error of a long sum grows with its length: sums that must be good to float32
 // are folded into registers every so many steps (kFoldLogits, kFold3).
 //
-// What bounds it: with many rows the power cap.  8 x 2048 rows of width 768: losses of 32000 words 567 us, 1.42 PFLOP/s (the library's products keep
-// up 1.39), a training step of 50257 words with an eighth of the rows ignored 3.14 to 3.67 ms by GPU, 1.21 to 1.41 PFLOP/s of its four products; tensor pipe
-// busy 83 / 83 / 81 % in losses / dz / dx and dW.  With few rows the dependent launches and W's way: 61 rows, 50257 words: 25 us, W alone 12.
+// What bounds it: with many rows the power cap.  8 x 2048 rows of width 768: losses of 32000 words 567 to 582 us by GPU, 1.38 to 1.42 PFLOP/s (the
+// library's products keep up 1.39), a training step of 50257 words with an eighth of the rows ignored 3.14 to 3.81 ms, 1.16 to 1.41 PFLOP/s of its four
+// products; tensor pipe busy 83 / 83 / 81 % in losses / dz / dx and dW.  With few rows the dependent launches and W's way: 61 rows, 50257 words: 25 us, W
+// alone 12.  float32, 1531 rows of 50257 words: losses 497 us, with gradients 2.22 to 2.32 ms: z anew is six part products there, 0.5 ms, where keeping it
+// would be 0.1 ms of memory.
 #include "cdssm_common.cuh"
 #include "sm100_ptx.cuh"
 #include "tile_map.cuh"
@@ -136,7 +138,8 @@ __device__ __forceinline__ int pair_id() { return blockIdx.x >> 1; }
 __device__ __forceinline__ int pairs() { return gridDim.x >> 1; }
 
 // Vocabulary tiles of a run: the fewest rounds of tiles, and few runs, whose sums have to be joined (8 x 2048 rows, 32000 words: runs of one tile
-// 109 rounds and 586 us, of eight 112 rounds and 583; 4096 rows of width 2048: of two 28 rounds, of three 30, a tenth more).
+// 109 rounds and 586 us, of eight 112 rounds and 583; 4096 rows of width 2048: of two 28 rounds, of three 30, a tenth more; the price of a run was
+// weighed at these two).
 constexpr int kMostRun = 8;
 __device__ __forceinline__ int best_run(int row_tiles, int n_tiles, int pairs) {
     int best = 1;
@@ -185,7 +188,8 @@ template <bool kSolo> struct RunWalk {
 // dz leaves DRAM once for either product.  (Column tiles as work of their own, cut where it suits the grid: 1.28 GB read instead of 0.83 for dz of
 // 262 MB.)  Of the tile rows as many whole ones as fill the groups evenly; the depth blocks of the rows that are left, dx before dW, are cut into as
 // many equal shares as there are groups.  Rows of a small depth are whole ones all: what they take is their way out (28 of 2 blocks as two
-// shares: 61 us, whole 40), and groups that have one of dW more than others get so much less of dx.
+// shares: 61 us, whole 40), and groups that have one of dW more than others get so much less of dx (both weighed at this size, 6 rows of 32000 words of
+// width 512).
 constexpr int kSplitDepth = 16, kWayOut = 10;   // depth blocks; what the way out takes in terms of them
 // The widest part of a row of column tiles that leaves at most a tenth of the pairs without a group.
 __host__ __device__ inline int group_width(int d_tiles, int pairs) {
@@ -290,7 +294,7 @@ __device__ __forceinline__ uint32_t in_first(const void* bar) {
     return r;
 }
 // (Of this block's scope: what it orders is the reading of tensor memory, behind tcgen05's own fence.  At the cluster's it waits for the warp's
-// stores to DRAM.)
+// stores to DRAM.  Nothing that is written to memory may be handed to the other block by it.)
 __device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
@@ -949,7 +953,8 @@ __global__ void __launch_bounds__(256) join_split_kernel(const Args a, int pairs
 constexpr int kIndexThreads = 1024;
 
 // Compact numbers of the rows that have a target, in their order: a block per 1024 rows counts the ones before its own anew (all
-// of the targets come from L2 and a second launch costs more, up to some 10^5 rows).  Rows without one lose 0.
+// of the targets come from L2 and a second launch costs more, up to some 10^5 rows; of a million rows that is 4 GB read, by L2's rate some 0.5 ms beside
+// 50 ms of products).  Rows without one lose 0.
 // The first kernel of a call: it lets the next ones start when all before it is done, so that they may read the caller's operands ahead.
 struct Index {
     const int64_t* target;
@@ -1215,7 +1220,8 @@ struct Sizes {
 };
 // Up to this many rows the second block of a pair would have none of its own: z is made by blocks by themselves (Smem), and bf16's dz keeps 16 bits, in
 // two parts.  (Where a row has one large entry, its target's, that entry's rounding to 8 bits is all of the row's error; beyond, the rows' roundings
-// average out and the products' time shows.)  dx takes a part a block, W once, if its rows of tiles are few and deep enough that every one is split.
+// average out and the products' time shows.  50257 words of width 768, a training step of 128 and of 129 rows: 120 and 115 us; with an upstream gradient a
+// row 118 and 125.)  dx takes a part a block, W once, if its rows of tiles are few and deep enough that every one is split.
 constexpr int kFewRows = kHalf;
 constexpr size_t kPieceBytes = 512ull << 20;   // of dz, beyond which the vocabulary is cut
 

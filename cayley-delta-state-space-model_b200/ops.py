@@ -197,16 +197,19 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, targets: Tensor, *, ign
     targets (...) int64.  Rows whose target is ``ignore_index`` lose 0, take no part in the mean and get zero gradients, whatever
     they hold (infinities and NaN too).  A target that is neither a word nor ignore_index makes its row's loss NaN.
     reduction "mean" (NaN when every row is ignored), "sum" or "none" (targets' shape); the loss is float32.
-    Products are bfloat16 ones with float32 sums, for float32 operands exact to 24 bits; the logits' gradient is rounded once to the
-    products' type.  Gradients have the operands' type and are the same from run to run.  Differentiable once, backwards."""
+    Products are bfloat16 ones with float32 sums, for float32 operands exact to 24 bits.  The sums are cut off, not rounded: a loss of
+    bfloat16 rows of width 768 is off by some 7e-7 of itself.  The logits' gradient is rounded to bfloat16 where there are more than 128
+    rows (a gradient is off by 2.0e-3 of itself then, its own rounding being 1.7e-3), keeps 16 bits of up to 128 and 24 of float32.
+    Gradients have the operands' type and are the same from run to run.  Differentiable once, backwards."""
     if reduction not in _REDUCTIONS:
         raise CdssmError(f"reduction must be 'none', 'mean' or 'sum', not {reduction!r}")
     return _lib.host().linear_cross_entropy(hidden, weight, targets, ignore_index, _REDUCTIONS[reduction], flags)
 
 
 def grad_norm(grads) -> Tensor:
-    """The 2-norm of all tensors together, one float32 value on their device; squares are summed in 64 bits in a fixed order.
-    bfloat16 and float32 CUDA tensors, dense in memory, at least one.  A number to look at: it has no gradient of its own."""
+    """The 2-norm of all tensors together, one float32 value on their device; squares are summed in a fixed order, four or eight
+    neighbours in 32 bits and these sums in 64.  bfloat16 and float32 CUDA tensors, dense in memory, at least one.  A number to look at:
+    it has no gradient of its own."""
     return _lib.host().grad_clip(list(grads), None, 0.0)
 
 

@@ -453,6 +453,7 @@ CDSSM_API int cdssm_b200_decode_step_reference(float* local_state, float* correc
  * (cdssm_b200_linear_ce_workspace_bytes), which is free again behind the call.  It holds the rows that take part and, for a w that is not
  * read in place (float32, or rows that are not 16-byte aligned), w's bf16 parts: 6 or 2 bytes a value.  Both sizes are for the current device, 0 on
  * bad sizes.  rows <= 2^24, vocab <= 2^24, d <= 65536.  bf16 products with float32 sums; float32 operands enter as three bf16 parts.
+ * The forward's workspace is 16 bytes a row for every 256 words (0.8 GB for 262 144 rows and 50 257 words), the backward's 39 MB and more.
  * flags: 0 or CDSSM_SCAN_TEST_WITHHOLD.  After a bounded wait that ran out the loss and its gradients are NaN; of one in a backward pass
  * that pass's gradients alone.
  * Replaces the LM head and the loss of a training step: cdssm/models/model.py:50-51, cdssm/training/trainer.py:219-262. */
@@ -469,7 +470,8 @@ CDSSM_API int cdssm_b200_linear_ce_fwd(const void* x, int64_t x_row_stride, cons
 /* Its backward: grad_loss (rows for CDSSM_CE_NONE, else one value) float32 -> grad_x (rows,d) and grad_w (vocab,d), dense, in the
  * storage type, 16-byte aligned; either may be NULL.  w, target and the other arguments as in the forward that left saved, which is
  * read alone: any number of passes may follow one forward, at the same time too, each with a workspace of its own.
- * dz is formed a piece of the vocabulary at a time (at most 512 MiB of scratch while a row tile allows).  Sums run in a fixed order. */
+ * dz is formed a piece of the vocabulary at a time (at most 512 MiB of scratch while a row tile allows).  Sums run in a fixed order.
+ * dz is rounded to bf16 where there are more than 128 rows of bf16, is two bf16 parts of up to 128 and three of float32. */
 CDSSM_API int cdssm_b200_linear_ce_bwd(const float* grad_loss, const void* w, int64_t w_row_stride, const int64_t* target,
                                        const void* saved, size_t saved_bytes, void* grad_x, void* grad_w, void* workspace,
                                        size_t workspace_bytes, int64_t rows, int d, int vocab, int64_t ignore_index,
@@ -491,7 +493,8 @@ CDSSM_API int cdssm_b200_embedding_bwd(const int64_t* ids, const void* grad, voi
 /* The 2-norm of n tensors together and, where out is not NULL, their values times min(1, max_norm / (norm + 1e-6)).
  * in, out, sizes (values) and the types (CDSSM_BF16 or CDSSM_F32) are HOST arrays of n; out[i] may be in[i], or another buffer of
  * the same type or of float32, and no out may overlap another tensor of the call.  norm: one float32 in device memory.  Squares are
- * summed in float64 in a fixed order.  Where the factor is 1 tensors in place are not written.  A norm that is no number makes every
+ * summed in a fixed order, four (float32) or eight (bf16) neighbours in float32, in float64 where they leave its range, and these sums
+ * in float64.  Where the factor is 1 tensors in place are not written.  A norm that is no number makes every
  * output NaN, an infinite one zeros of what is finite.  workspace: cdssm_b200_grad_clip_workspace_bytes, 256-byte aligned.
  * Replaces clip_grad_norm_ of a training step, cdssm/training/trainer.py:219-262. */
 CDSSM_API size_t cdssm_b200_grad_clip_workspace_bytes(const int64_t* sizes, int n);
