@@ -16,8 +16,8 @@
 // All products are tcgen05 ones of TMA tiles by pairs of blocks: 256 x 256 outputs, each block loads half of both operands and keeps 128
 // rows of the result, fp32 accumulators, two of them in tensor memory so that the epilogue of a tile runs beside the products of the next.
 // float32 operands enter as three bf16 parts (exact to 24 bits) and six of the nine part products, the small ones first.  The tensor
-// cores' float32 sums are cut off, not rounded, so that the error of a long sum grows with its length: sums that must be good to float32
-// are folded into registers every so many steps (kFoldLogits, kFold3).
+// cores' float32 sums are cut off, not rounded, so that the error of a long sum grows with its length: sums that must be good to float32,
+// and long ones of any kind, are folded into registers every so many steps (kFoldLogits, kFold3, kFoldLong).
 //
 // What bounds it: with many rows the power cap.  8 x 2048 rows of width 768: losses of 32000 words 567 to 582 us by GPU, 1.38 to 1.42 PFLOP/s (the
 // library's products keep up 1.39), a training step of 50257 words with an eighth of the rows ignored 3.14 to 3.81 ms, 1.16 to 1.41 PFLOP/s of its four
@@ -113,6 +113,7 @@ __device__ __forceinline__ void term_planes(const Args& a, bool of_dz, bool of_d
     pb = a.planes == 3 ? (tb >> (2 * term)) & 3 : of_dw && a.row_factor ? 1 - term : 0;
 }
 
+// The hardware's 2^x, good to 2^-22: beside bf16's 2^-8 nothing, and of float32's gradients (4e-7) the smaller part.
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

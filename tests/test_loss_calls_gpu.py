@@ -25,13 +25,14 @@ class Entry:
     def _bytes(n):                                                   # (what lay in the memory before is no part of a call)
         return torch.full((n,), 255, dtype=torch.uint8, device="cuda")
 
-    def backward(self, flags=0):
-        ws = self._bytes(self.h.cdssm_b200_linear_ce_workspace_bytes(self.T, self.d, self.V, self.dt, 1))
+    def backward(self, flags=0, wait=True):
+        ws = self.ws = self._bytes(self.h.cdssm_b200_linear_ce_workspace_bytes(self.T, self.d, self.V, self.dt, 1))
         gx, gw, one = torch.empty_like(self.x), torch.empty_like(self.w), torch.ones((), device="cuda")
         assert self.h.cdssm_b200_linear_ce_bwd(one.data_ptr(), self.w.data_ptr(), self.w.stride(0), self.y.data_ptr(), self.saved.data_ptr(),
                                                self.saved.numel(), gx.data_ptr(), gw.data_ptr(), ws.data_ptr(), ws.numel(), self.T, self.d, self.V,
                                                -100, 1, self.dt, flags, torch.cuda.current_stream().cuda_stream) == 0
-        torch.cuda.synchronize()                                     # (the workspace is let go)
+        if wait:
+            torch.cuda.synchronize()
         return gx, gw
 
 
@@ -130,3 +131,19 @@ def test_signs_that_are_pending(ops, T, V, d):
     for call in (lambda: ops.grad_norm([neg(w)]), lambda: ops.clip_grads_([w.clone()], 1.0, out=[neg(w)])):
         with pytest.raises(ops.CdssmError, match="sign is pending"):
             call()
+
+
+def test_two_passes_at_once_over_one_forward(ops):
+    """On two streams, each with a workspace of its own."""
+    x, w, y = _inputs(900, 2000, 64, torch.bfloat16, seed=45)
+    want = _grads(ops, x, w, y, torch.ones((), device="cuda"))[1:]
+    e = Entry(ops, x, w, y)
+    streams, kept, got = [torch.cuda.Stream() for _ in range(2)], [], []
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append(e.backward(wait=False))
+            kept.append(e.ws)                                        # (its memory is nobody else's while a stream may read it)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
